@@ -14,6 +14,8 @@ Artefacts (all land inside the package so gpurun snapshots carry them):
   ``KGS_PMC_CROSSCHECK=1``; it keeps one HSA helper thread spinning).
 * ``kube_gpu_stats_amd/lib/libkgs_load.so`` – hand-written gfx950 HIP kernels
   (MFMA-bound, HBM-stream, xGMI peer copy) used as the synthetic load.
+* ``kube_gpu_stats_amd/lib/libkgs_decoder.so`` – the decoder block's operators
+  (attention, swiglu, add_norm; ``ops/decoder.py``).
 
 Rebuilds are incremental on source/header mtimes.  ``python -m
 kube_gpu_stats_amd.native.build [--force]`` builds everything.
@@ -36,6 +38,10 @@ OFFLOAD_ARCH = "gfx950"
 
 CXXFLAGS = ["-std=c++17", "-O2", "-g1", "-fPIC", "-pthread", "-Wall", "-Wextra", "-Wno-unused-parameter",
             "-fvisibility=hidden"]
+# Packed float instructions off: some of their forms have given wrong results on gfx950.  (hipcc's
+# host pass warns that it does not know the feature.)
+HIPFLAGS = [f"--offload-arch={OFFLOAD_ARCH}", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang",
+            "-packed-fp32-ops"]
 
 
 def ext_suffix() -> str:
@@ -56,6 +62,10 @@ def pmc_aql_lib_path() -> str:
 
 def load_lib_path() -> str:
     return os.path.join(LIB, "libkgs_load.so")
+
+
+def decoder_lib_path() -> str:
+    return os.path.join(LIB, "libkgs_decoder.so")
 
 
 def _stale(out: str, deps: list[str]) -> bool:
@@ -165,8 +175,36 @@ def build_load(force: bool = False, verbose: bool = False) -> str:
         return out
     os.makedirs(LIB, exist_ok=True)
     tmp = f"{out}.{os.getpid()}.tmp"  # concurrent builders (one per rank) never share a temp file
-    _run([os.path.join(ROCM, "bin", "hipcc"), f"--offload-arch={OFFLOAD_ARCH}", "-O3", "-std=c++17", "-fPIC",
-          "-shared", src, "-o", tmp], verbose)
+    _run([os.path.join(ROCM, "bin", "hipcc"), *HIPFLAGS, "-shared", src, "-o", tmp], verbose)
+    os.replace(tmp, out)
+    return out
+
+
+def build_decoder(force: bool = False, verbose: bool = False) -> str:
+    """The decoder block's operators (ops/hip/{decoder,attention,swiglu,add_norm}.hip)."""
+    out = decoder_lib_path()
+    hip = os.path.join(PKG, "ops", "hip")
+    srcs = [os.path.join(hip, f + ".hip") for f in ("decoder", "attention", "swiglu", "add_norm")]
+    deps = [os.path.join(hip, "decoder.h"), os.path.join(hip, "decoder_common.h"), __file__]
+    if not force and not _stale(out, srcs + deps):
+        return out
+    objdir = os.path.join(HERE, "build", "obj_hip")
+    os.makedirs(objdir, exist_ok=True)
+    os.makedirs(LIB, exist_ok=True)
+    hipcc = os.path.join(ROCM, "bin", "hipcc")
+
+    def compile_one(src: str) -> str:
+        obj = os.path.join(objdir, os.path.basename(src) + ".o")
+        if force or _stale(obj, [src] + deps):
+            tmp = f"{obj}.{os.getpid()}.tmp"
+            _run([hipcc, *HIPFLAGS, "-fvisibility=default", "-c", src, "-o", tmp], verbose)
+            os.replace(tmp, obj)
+        return obj
+
+    with cf.ThreadPoolExecutor(max_workers=4) as ex:
+        objs = list(ex.map(compile_one, srcs))
+    tmp = f"{out}.{os.getpid()}.tmp"
+    _run([hipcc, f"--offload-arch={OFFLOAD_ARCH}", "-fPIC", "-shared", *objs, "-o", tmp], verbose)
     os.replace(tmp, out)
     return out
 
@@ -210,6 +248,7 @@ def build_all(force: bool = False, verbose: bool = False, hip: bool = True) -> d
         res["pmc_error"] = str(e)
     if hip:
         res["load"] = build_load(force, verbose)
+        res["decoder"] = build_decoder(force, verbose)
     return res
 
 

@@ -1,1 +1,2 @@
-"""Hand-written gfx950 HIP kernels (synthetic load for the overhead benchmark)."""
+"""Hand-written gfx950 HIP kernels: the synthetic load for the overhead benchmark (``load``) and the
+decoder block's operators, forward and backward (``decoder``)."""

@@ -1,0 +1,593 @@
+"""The decoder block's operators as gfx950 kernels, forward and backward
+(``ops/hip/attention.hip``, ``swiglu.hip``, ``add_norm.hip``).
+
+They are what a training step runs between its plain matrix products: softmax attention,
+the gated half of the feed-forward block, and the norms around a residual connection.
+With them the exporter is measured under a training step whose kernels are this
+package's own, with known operations and bytes (``bench.py --load train --train-ops hip``);
+they stand beside the synthetic kernels of ``ops/load.py``.
+
+Each operator comes three times:
+
+* ``attention``, ``swiglu``, ``add_norm`` — differentiable, for a program that uses autograd;
+* ``*_fwd`` — the forward pass, returning what a backward pass needs;
+* ``*_bwd`` — the gradients, for loops without autograd and for captured graphs.
+
+All of them launch on the current stream of their tensors' device (or on ``stream=``),
+allocate their results and workspaces from torch's allocator on that stream, never
+synchronise and keep nothing between calls, so they can be captured into a graph.
+Gradients are sums in a fixed order: equal calls give equal bits.  The autograd forms
+differentiate once.  To capture a whole autograd step, let no eager graph of the same
+leaves be alive (torch's own rule); the ``*_fwd`` / ``*_bwd`` pairs have no such rule.
+
+There is deliberately no eager fallback: on a GPU the HIP library must load, or these
+functions raise.  Wrong arguments raise ``ValueError`` or ``TypeError`` before anything
+is launched.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+import os
+import struct
+
+from ..native import build as _build
+
+_LIB: ctypes.CDLL | None = None
+
+
+def lib() -> ctypes.CDLL:
+    global _LIB
+    if _LIB is None:
+        path = _build.decoder_lib_path()
+        if not os.path.exists(path):
+            _build.build_decoder()
+        L = ctypes.CDLL(path)
+        L.kgs_decoder_last_error.restype = ctypes.c_char_p
+        for name in ("attention", "swiglu", "add_norm"):
+            for way in ("fwd", "bwd"):
+                getattr(L, f"kgs_{name}_{way}").argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+        _LIB = L
+    return _LIB
+
+
+# The C structures of ops/hip/decoder.h, field by field.
+_ATTENTION = struct.Struct("@12P24q8if")
+_SWIGLU = struct.Struct("@9P3q4i3i3i")
+_ADD_NORM = struct.Struct("@16P5q4i2f")
+
+
+def _call(entry: str, args: bytes, device, stream) -> None:
+    import torch
+
+    s = stream if stream is not None else torch.cuda.current_stream(device)
+    if getattr(lib(), entry)(args, s.cuda_stream) != 0:
+        raise RuntimeError(lib().kgs_decoder_last_error().decode())
+
+
+@contextlib.contextmanager
+def _on(device, stream):
+    """Allocations and launches on the tensors' device and on ``stream``."""
+    import torch
+
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        yield
+
+
+def _placed(device, stream):
+    import torch
+
+    if stream is None and device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    if stream is not None and stream.device != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors are on {device}")
+    return _on(device, stream)
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _type(t, name: str, allowed: str) -> int:
+    import torch
+
+    types = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+    code = types.get(t.dtype)
+    if code is None or code >= (3 if "float32" in allowed else 2):
+        raise TypeError(f"{name} must be {allowed}, not {t.dtype}")
+    return code
+
+
+def _same(first, name: str, **others) -> None:
+    for other, t in others.items():
+        if t is None:
+            continue
+        if t.dtype != first.dtype:
+            raise TypeError(f"{other} is {t.dtype}, {name} is {first.dtype}")
+        if t.device != first.device:
+            raise ValueError(f"{other} is on {t.device}, {name} is on {first.device}")
+
+
+def _on_gpu(t, name: str) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a GPU, not on {t.device}")
+
+
+def _shape(t, name: str, want) -> None:
+    if tuple(t.shape) != tuple(want):
+        raise ValueError(f"{name} must have shape {tuple(want)}, not {tuple(t.shape)}")
+
+
+# --------------------------------------------------------------------------- attention
+
+def _heads(t):
+    """``t`` [B, S, heads, D] as the kernels read it, and its strides of (B, S, heads):
+    D contiguous, positions apart, 16-byte rows.  Other layouts are copied."""
+    import torch
+
+    # A dimension of one may come with any stride; rows behind the last have to lie past it.
+    st = [t.shape[3] if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
+    if (t.stride(3) == 1 and t.shape[3] <= st[1] <= 1 << 22 and t.data_ptr() % 16 == 0
+            and not any(s % 8 for s in st)):
+        return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, list(t.stride()[:3])
+
+
+def _attention_checks(q, k, v, scale, lengths, **more):
+    import torch
+
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [batch, positions, heads, head dimension], not {tuple(t.shape)}")
+    B, S, H, D = q.shape
+    Hk = k.shape[2]
+    code = _type(q, "q", "bfloat16 or float16")
+    _same(q, "q", k=k, v=v, **{n: t for n, t in more.items() if n != "lse"})
+    _shape(k, "k", (B, S, Hk, D))
+    _shape(v, "v", (B, S, Hk, D))
+    for name, t in more.items():
+        _shape(t, name, (B, H, S) if name == "lse" else (B, S, H, D))
+    if D not in (64, 128):
+        raise ValueError(f"the head dimension must be 64 or 128, not {D}")
+    if H == 0 or Hk == 0 or H % Hk:
+        raise ValueError(f"{H} query heads cannot share {Hk} key heads")
+    if S >= 1 << 30:
+        raise ValueError(f"at most {(1 << 30) - 1} positions, not {S}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError(f"scale must be finite and positive, not {scale}")
+    if lengths is not None:
+        if lengths.dtype != torch.int32:
+            raise TypeError(f"lengths must be int32, not {lengths.dtype}")
+        _shape(lengths, "lengths", (B,))
+        if lengths.device != q.device:
+            raise ValueError(f"lengths is on {lengths.device}, q is on {q.device}")
+        lengths = lengths.contiguous()
+    if "lse" in more:
+        lse = more["lse"]
+        if lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
+            raise ValueError("lse must be the float32 tensor that attention_fwd returned")
+    _on_gpu(q, "q")
+    return B, S, H, Hk, D, code, scale, lengths
+
+
+def attention(q, k, v, *, causal: bool = True, scale: float | None = None, lengths=None):
+    """softmax(scale · q kᵀ) v over each sequence's own tokens; differentiable in q, k, v.
+
+    q [B, S, H, D], k and v [B, S, Hk, D] of bfloat16 or float16, D 64 or 128, H a multiple
+    of Hk (each key head serves H / Hk query heads); any strides with D contiguous and
+    16-byte aligned rows are read in place, so q, k and v may be views of one projection's
+    output (other layouts are copied first).  ``causal``: position i sees positions up to i.
+    ``scale``: D^-½ if None.  ``lengths`` [B] int32 on the GPU: sequence b is its first
+    lengths[b] positions (clamped to 0..S); nothing behind them is read, the result and the
+    gradients are zero there.  Returns [B, S, H, D], contiguous.
+
+    A position that is masked by ``causal`` alone is multiplied by a zero probability, as in
+    a plain matrix product: its v must be finite.
+    """
+    import torch
+
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _functions()[0].apply(q, k, v, causal, scale, lengths)
+    return _attention_fwd(q, k, v, causal, scale, lengths, None, False)[0]
+
+
+def attention_qkv(qkv, heads: int, *, causal: bool = True, scale: float | None = None, lengths=None):
+    """``attention`` of one projection's output [B, S, heads + 2 Hk, D], the query heads
+    first, then the key heads, then the value heads; differentiable, with one gradient of
+    the same layout (no gradients of views to be put together)."""
+    import torch
+
+    q, k, v = _split_qkv(qkv, heads)
+    if torch.is_grad_enabled() and qkv.requires_grad:
+        return _functions()[1].apply(qkv, heads, causal, scale, lengths)
+    return _attention_fwd(q, k, v, causal, scale, lengths, None, False)[0]
+
+
+def _split_qkv(qkv, heads: int):
+    if qkv.dim() != 4 or heads <= 0 or qkv.shape[2] <= heads or (qkv.shape[2] - heads) % 2:
+        raise ValueError(f"qkv must be [batch, positions, {heads} + 2 key heads, head dimension], "
+                         f"not {tuple(qkv.shape)}")
+    kv = (qkv.shape[2] - heads) // 2
+    return qkv[:, :, :heads], qkv[:, :, heads:heads + kv], qkv[:, :, heads + kv:]
+
+
+def attention_fwd(q, k, v, *, causal: bool = True, scale: float | None = None, lengths=None, stream=None):
+    """``attention`` without autograd: (out, lse), lse [B, H, S] float32 the base-2 logarithm
+    of each row's sum (-inf behind a sequence's end), for ``attention_bwd``."""
+    return _attention_fwd(q, k, v, causal, scale, lengths, stream, True)
+
+
+def _attention_fwd(q, k, v, causal, scale, lengths, stream, keep):
+    import torch
+
+    B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths)
+    with _placed(q.device, stream):
+        (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
+        out = torch.empty(B, S, H, D, dtype=q.dtype, device=q.device)
+        lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device) if keep else None
+        args = _ATTENTION.pack(_ptr(q), _ptr(k), _ptr(v), _ptr(out), 0, 0, 0, 0, _ptr(lse), 0, 0, _ptr(lengths),
+                               *qs, *ks, *vs, S * H * D, H * D, D, *([0] * 12), B, S, H, Hk, D, code, int(causal), 1,
+                               scale)
+        if out.numel():
+            _call("kgs_attention_fwd", args, q.device, stream)
+    return out, lse
+
+
+def _dkv_splits(B: int, S: int, H: int, Hk: int) -> int:
+    """Parts that the walk over query rows is cut into for dk and dv: with fewer workgroups
+    (one per 128 keys and key head) than the chip holds at once, two per CU, it is cut, as
+    long as a part keeps 16 steps of 32 rows."""
+    groups = max(1, B * Hk * -(-S // 128))
+    steps = (H // Hk) * -(-S // 32)
+    return max(1, min(512 // groups, steps // 16, 8))
+
+
+def attention_bwd(dout, q, k, v, out, lse, *, causal: bool = True, scale: float | None = None, lengths=None,
+                  stream=None):
+    """(dq, dk, dv) of ``attention`` from the gradient of its result, with ``out`` and ``lse``
+    of ``attention_fwd`` and the same keywords; the probabilities are computed again."""
+    return _attention_bwd(dout, q, k, v, out, lse, causal, scale, lengths, stream, None)
+
+
+def _attention_bwd(dout, q, k, v, out, lse, causal, scale, lengths, stream, into):
+    import torch
+
+    B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths, dout=dout, out=out, lse=lse)
+    with _placed(q.device, stream):
+        (q, qs), (k, ks), (v, vs), (out, os_), (dout, gs) = _heads(q), _heads(k), _heads(v), _heads(out), _heads(dout)
+        if into is None:
+            into = [torch.empty(B, S, n, D, dtype=q.dtype, device=q.device) for n in (H, Hk, Hk)]
+        splits = _dkv_splits(B, S, H, Hk)
+        # delta, then the parts of a split walk
+        parts = splits * 2 * B * S * Hk * D if splits > 1 else 0
+        rows = (B * H * S + 3) // 4 * 4  # the parts are read 16 bytes at a time
+        work = torch.empty(rows + parts, dtype=torch.float32, device=q.device)
+        st = [s for t in into for s in t.stride()[:3]]
+        args = _ATTENTION.pack(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), *(_ptr(t) for t in into), _ptr(lse),
+                               _ptr(work), _ptr(work) + rows * 4 if parts else 0, _ptr(lengths), *qs, *ks, *vs, *os_,
+                               *gs, *st, B, S, H, Hk, D, code, int(causal), splits, scale)
+        if q.numel():
+            _call("kgs_attention_bwd", args, q.device, stream)
+    return tuple(into)
+
+
+# ------------------------------------------------------------------------------ swiglu
+
+def _matrix(t):
+    """``t`` [..., n] as rows the kernels read, and their stride: rows contiguous, apart, 16-byte
+    aligned.  Other layouts are copied."""
+    import torch
+
+    n = t.shape[-1]
+    m = t.reshape(-1, n)
+    ld = n if m.shape[0] == 1 else m.stride(0)
+    if m.stride(1) == 1 and n <= ld <= 1 << 21 and ld % 8 == 0 and m.data_ptr() % 16 == 0:
+        return m, ld
+    return m.clone(memory_format=torch.contiguous_format), n
+
+
+def _swiglu_checks(x, w, **more):
+    if x.dim() < 1 or w.dim() != 2:
+        raise ValueError(f"x must be [..., width] and w [2 inner, width], not {tuple(x.shape)} and {tuple(w.shape)}")
+    K, F = x.shape[-1], w.shape[0] // 2
+    code = _type(x, "x", "bfloat16 or float16")
+    _same(x, "x", w=w, **more)
+    _shape(w, "w", (2 * F, K))
+    if K == 0 or F == 0 or K % 8 or F % 8 or K > 1 << 20 or F > 1 << 20:
+        raise ValueError(f"width and inner must be multiples of 8, at most {1 << 20}, not {K} and {F}")
+    for name, t in more.items():
+        _shape(t, name, (*x.shape[:-1], F if name == "dh" else 2 * F))
+    T = x.numel() // K
+    if T >= 1 << 30:
+        raise ValueError(f"at most {(1 << 30) - 1} rows, not {T}")
+    _on_gpu(x, "x")
+    return T, K, F, code
+
+
+PRODUCT_TILES = (0, 1)  # the tiles of swiglu.hip's product: 128 x 128, 256 x 256
+
+
+def _product_plan(M: int, N: int, K: int) -> tuple[int, int]:
+    """(tile, splits) of an [M, N] product over K: the 256 x 256 tile where its workgroups fill
+    the CUs, else 128 x 128, with the sum cut into parts while the CUs have room for two
+    workgroups each and a part keeps 8 steps of 64."""
+    if -(-M // 256) * -(-N // 256) >= 200:
+        return 1, 1
+    tiles = -(-M // 128) * -(-N // 128)
+    return 0, max(1, min(512 // tiles, K // 512, 16))
+
+
+def swiglu(x, w):
+    """silu(x Wgᵀ) · (x Wuᵀ) with w = [Wg; Wu]; differentiable in x and w.
+
+    x [..., width], w [2 inner, width] (the gate's rows first) of bfloat16 or float16, width
+    and inner multiples of 8; any row strides with contiguous, 16-byte aligned rows are read
+    in place.  Returns [..., inner].  With a gradient wanted the two projections are kept,
+    rounded to the tensors' type, for the backward pass.
+    """
+    import torch
+
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        return _functions()[2].apply(x, w)
+    return _swiglu_fwd(x, w, None, False)[0]
+
+
+def swiglu_fwd(x, w, *, stream=None):
+    """``swiglu`` without autograd: (h, saved), saved [..., 2 inner] for ``swiglu_bwd``."""
+    return _swiglu_fwd(x, w, stream, True)
+
+
+def _swiglu_fwd(x, w, stream, keep):
+    import torch
+
+    T, K, F, code = _swiglu_checks(x, w)
+    with _placed(x.device, stream):
+        h = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
+        saved = torch.empty(*x.shape[:-1], 2 * F, dtype=x.dtype, device=x.device) if keep else None
+        if T:
+            (x, x_ld), (w, w_ld) = _matrix(x), _matrix(w)
+            tile, splits = _product_plan(T, 2 * F, K)
+            part = torch.empty(splits * T * 2 * F, dtype=torch.float32, device=x.device) if splits > 1 else None
+            args = _SWIGLU.pack(_ptr(x), _ptr(w), _ptr(h), _ptr(saved), 0, 0, 0, 0, _ptr(part), x_ld, w_ld, 0, T, K, F,
+                                code, tile, 0, 0, splits, 1, 1)
+            _call("kgs_swiglu_fwd", args, x.device, stream)
+    return h, saved
+
+
+def swiglu_bwd(dh, x, w, saved, *, stream=None):
+    """(dx, dw) of ``swiglu`` from the gradient of its result and what ``swiglu_fwd`` saved."""
+    return _swiglu_bwd(dh, x, w, saved, True, True, stream)
+
+
+def _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, stream):
+    import torch
+
+    T, K, F, code = _swiglu_checks(x, w, dh=dh, saved=saved)
+    with _placed(x.device, stream):
+        new = torch.empty if T else torch.zeros
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
+        dw = new(w.shape, dtype=x.dtype, device=x.device) if want_dw else None
+        if T and (want_dx or want_dw):
+            (x, x_ld), (w, w_ld), (dh, dh_ld) = _matrix(x), _matrix(w), _matrix(dh)
+            saved = saved.contiguous()
+            if saved.data_ptr() % 16:
+                saved = saved.clone()
+            tx, sx = _product_plan(T, K, 2 * F)
+            tw, sw = _product_plan(2 * F, K, T)
+            size = max(sx * T * K if sx > 1 and want_dx else 0, sw * 2 * F * K if sw > 1 and want_dw else 0)
+            part = torch.empty(size, dtype=torch.float32, device=x.device) if size else None
+            dgu = torch.empty(T, 2 * F, dtype=x.dtype, device=x.device)
+            args = _SWIGLU.pack(_ptr(x), _ptr(w), 0, _ptr(saved), _ptr(dh), _ptr(dgu), _ptr(dx), _ptr(dw), _ptr(part),
+                                x_ld, w_ld, dh_ld, T, K, F, code, 0, tx, tw, 1, sx, sw)
+            _call("kgs_swiglu_bwd", args, x.device, stream)
+    return dx, dw
+
+
+# ---------------------------------------------------------------------------- add_norm
+
+MAX_NORM_WIDTH = 16384
+
+
+def _lines(t):
+    """``t`` [..., C] as rows and their stride; rows that are not contiguous are copied."""
+    import torch
+
+    m = t.reshape(-1, t.shape[-1])
+    if m.stride(1) != 1 and m.shape[1] > 1:
+        m = m.clone(memory_format=torch.contiguous_format)
+    return m, m.stride(0)
+
+
+def _add_norm_checks(first, name, weight, post_weight, gate, scale, eps, **rows):
+    if first.dim() < 1:
+        raise ValueError(f"{name} must be [..., width], not a single value")
+    C = first.shape[-1]
+    code = _type(first, name, "bfloat16, float16 or float32")
+    for other, t in rows.items():
+        if t is not None:
+            _shape(t, other, first.shape)
+    for other, t in (("weight", weight), ("post_weight", post_weight), ("gate", gate)):
+        if t is not None:
+            _shape(t, other, (C,))
+    _same(first, name, weight=weight, post_weight=post_weight, gate=gate, **rows)
+    if not 0 < C <= MAX_NORM_WIDTH:
+        raise ValueError(f"the width must be 1 to {MAX_NORM_WIDTH}, not {C}")
+    T = first.numel() // C
+    if T >= 1 << 30:
+        raise ValueError(f"at most {(1 << 30) - 1} rows, not {T}")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, not {scale}")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError(f"eps must be finite and not negative, not {eps}")
+    _on_gpu(first, name)
+    return T, C, code
+
+
+def add_norm(residual, branch, weight, *, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-6):
+    """(stream, out): stream = residual + scale · gate · norm(branch), out = norm(stream).
+
+    The step between two halves of a decoder block: ``branch`` (a half's result) is
+    normalised by its root mean square and multiplied by ``post_weight`` (left as it is if
+    None), multiplied by ``gate`` (ones if None) and ``scale``, and added to the residual
+    stream, which is then normalised with ``weight`` for the next half.  residual, branch
+    [..., C], weight, post_weight, gate [C], all of one type (bfloat16, float16, float32),
+    C up to 16384, of any row stride.  Differentiable in all five tensors.
+    """
+    import torch
+
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (residual, branch, weight, post_weight, gate)):
+        return _functions()[3].apply(residual, branch, weight, post_weight, gate, scale, eps)
+    return _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, False)[:2]
+
+
+def add_norm_fwd(residual, branch, weight, *, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-6,
+                 stream=None):
+    """``add_norm`` without autograd: (stream, out, saved), saved for ``add_norm_bwd``."""
+    return _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, True)
+
+
+def _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, keep):
+    import torch
+
+    T, C, code = _add_norm_checks(residual, "residual", weight, post_weight, gate, scale, eps, branch=branch)
+    with _placed(residual.device, stream):
+        s = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
+        out = torch.empty_like(s)
+        saved = torch.empty(2, T, dtype=torch.float32, device=residual.device) if keep else None
+        if T:
+            (r, r_ld), (b, b_ld) = _lines(residual), _lines(branch)
+            w, pw, g = (None if t is None else t.contiguous() for t in (weight, post_weight, gate))
+            args = _ADD_NORM.pack(_ptr(r), _ptr(b), _ptr(w), _ptr(pw), _ptr(g), _ptr(s), _ptr(out), _ptr(saved),
+                                  *([0] * 8), r_ld, b_ld, C, 0, 0, T, C, code, 0, scale, eps)
+            _call("kgs_add_norm_fwd", args, residual.device, stream)
+    return s, out, saved
+
+
+def _norm_parts(T: int, C: int) -> int:
+    """Parts that the backward's column sums come in: one a workgroup (of rows up to 512
+    wide, four rows a workgroup and a part a row), a workgroup taking rows in turn."""
+    rows = 4 if C <= 512 else 1
+    threads = 256 if C <= 4096 else 512 if C <= 8192 else 1024
+    return rows * min(-(-T // rows), 256 * 1024 // threads)
+
+
+def add_norm_bwd(dstream, dout, stream_, branch, weight, saved, *, post_weight=None, gate=None, scale: float = 1.0,
+                 eps: float = 1e-6, stream=None):
+    """(dresidual, dbranch, dweight, dpost_weight, dgate) of ``add_norm`` from the gradients of
+    its two results (either may be None: zero), its stream ``stream_``, and ``saved`` of
+    ``add_norm_fwd`` with the same keywords.  Without post_weight, gate and scale dbranch is
+    dresidual, the same tensor; gradients of absent weights are None."""
+    import torch
+
+    if dstream is None and dout is None:
+        raise ValueError("one of dstream and dout must be given")
+    T, C, code = _add_norm_checks(stream_, "stream_", weight, post_weight, gate, scale, eps, dstream=dstream, dout=dout,
+                                  branch=branch)
+    if saved.dtype != torch.float32 or tuple(saved.shape) != (2, T) or not saved.is_contiguous():
+        raise ValueError("saved must be the float32 tensor that add_norm_fwd returned")
+    if saved.device != stream_.device:
+        raise ValueError(f"saved is on {saved.device}, stream_ is on {stream_.device}")
+    with _placed(stream_.device, stream):
+        def new(like, zero=False):
+            return (torch.zeros if zero else torch.empty)(like.shape, dtype=like.dtype, device=like.device)
+
+        full = post_weight is not None or gate is not None or scale != 1.0
+        dr = new(stream_)
+        db = new(stream_) if full else dr
+        grads = [None if t is None else new(t, zero=not T) for t in (weight, post_weight, gate)]
+        if T:
+            (s, s_ld), (b, b_ld) = _lines(stream_), _lines(branch)
+            (ds, ds_ld), (dy, dy_ld) = (_lines(t) if t is not None else (None, 0) for t in (dstream, dout))
+            w, pw, g = (None if t is None else t.contiguous() for t in (weight, post_weight, gate))
+            parts = _norm_parts(T, C)
+            work = torch.empty(parts * 3 * C, dtype=torch.float32, device=s.device)
+            args = _ADD_NORM.pack(0, _ptr(b), _ptr(w), _ptr(pw), _ptr(g), _ptr(s), 0, _ptr(saved), _ptr(ds), _ptr(dy),
+                                  _ptr(dr), _ptr(db), *(_ptr(t) for t in grads), _ptr(work), 0, b_ld, s_ld, ds_ld, dy_ld,
+                                  T, C, code, parts, scale, eps)
+            _call("kgs_add_norm_bwd", args, s.device, stream)
+    return dr, db, *grads
+
+
+# ---------------------------------------------------------------------------- autograd
+
+_FUNCTIONS = None
+
+
+def _functions():
+    """The autograd functions, made on first use (importing this module needs no torch)."""
+    global _FUNCTIONS
+    if _FUNCTIONS is not None:
+        return _FUNCTIONS
+    import torch
+    from torch.autograd.function import once_differentiable
+
+    class Attention(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k, v, causal, scale, lengths):
+            out, lse = _attention_fwd(q, k, v, causal, scale, lengths, None, True)
+            ctx.save_for_backward(q, k, v, out, lse, lengths)
+            ctx.options = causal, scale
+            return out
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, dout):
+            q, k, v, out, lse, lengths = ctx.saved_tensors
+            grads = _attention_bwd(dout, q, k, v, out, lse, *ctx.options, lengths, None, None)
+            return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
+
+    class AttentionQkv(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, qkv, heads, causal, scale, lengths):
+            out, lse = _attention_fwd(*_split_qkv(qkv, heads), causal, scale, lengths, None, True)
+            ctx.save_for_backward(qkv, out, lse, lengths)
+            ctx.options = heads, causal, scale
+            return out
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, dout):
+            qkv, out, lse, lengths = ctx.saved_tensors
+            heads, causal, scale = ctx.options
+            grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+            _attention_bwd(dout, *_split_qkv(qkv, heads), out, lse, causal, scale, lengths, None,
+                           _split_qkv(grad, heads))
+            return grad, None, None, None, None
+
+    class Swiglu(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            h, saved = _swiglu_fwd(x, w, None, True)
+            ctx.save_for_backward(x, w, saved)
+            return h
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, dh):
+            return _swiglu_bwd(dh, *ctx.saved_tensors, *ctx.needs_input_grad, None)
+
+    class AddNorm(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, residual, branch, weight, post_weight, gate, scale, eps):
+            stream, out, saved = _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, True)
+            ctx.save_for_backward(stream, branch, weight, saved, post_weight, gate)
+            ctx.options = scale, eps
+            ctx.set_materialize_grads(False)
+            return stream, out
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, dstream, dout):
+            if dstream is None and dout is None:
+                return (None,) * 7
+            stream, branch, weight, saved, post_weight, gate = ctx.saved_tensors
+            grads = add_norm_bwd(dstream, dout, stream, branch, weight, saved, post_weight=post_weight, gate=gate,
+                                 scale=ctx.options[0], eps=ctx.options[1])
+            return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)
+
+    _FUNCTIONS = Attention, AttentionQkv, Swiglu, AddNorm
+    return _FUNCTIONS

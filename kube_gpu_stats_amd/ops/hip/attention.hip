@@ -1,0 +1,493 @@
+// Softmax attention over a padded batch, forward and backward, for gfx950.
+//
+//   s_ij = c q_i.k_j  for j < n_b (j <= i if causal),  i < n_b
+//   o_i = sum_j softmax_j(s_i) v_j,   lse_i = log2 sum_j 2^(s_ij log2 e)
+//   delta_i = do_i.o_i,  p_ij = 2^(s_ij log2 e - lse_i),  ds_ij = p_ij (do_i.v_j - delta_i)
+//   dq_i = c sum_j ds_ij k_j,  dk_j = c sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
+//
+// All three kernels hold one side of the score matrix in registers, 32 rows a wave, and
+// walk the other side through LDS.  The product is taken the way round that leaves the
+// wave's own rows in the lanes (column = lane % 32): softmax statistics are then one
+// value a lane, a row's sum one exchange with lane ^ 32, and the probabilities lie in
+// the registers as the next product's second operand wants them, up to an order of the
+// summed index that Tile::columns reads the first operand in as well.  So the scores
+// and probabilities never leave the registers.
+//
+// Scores, statistics, sums and accumulators are 32 bits.  Rounded to the tensors' type:
+// p and ds, as operands of a matrix instruction (half a step each, independent from
+// term to term), and the outputs.
+#include "decoder.h"
+#include "decoder_common.h"
+
+namespace kgs {
+namespace {
+
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
+constexpr int kRows = kWaves * 32;  // rows a workgroup holds
+constexpr int kStep = 64;           // keys a step of forward and dq
+
+__device__ __forceinline__ int length_of(const KgsAttention& a, int b) {
+  if (!a.lengths) return a.S;
+  const int n = __builtin_amdgcn_readfirstlane(a.lengths[b]);
+  return n < 0 ? 0 : n > a.S ? a.S : n;
+}
+
+template <class T> __device__ __forceinline__ const char* at(const void* p, const int64_t* st, int b, int s, int h) {
+  return reinterpret_cast<const char*>(static_cast<const T*>(p) + b * st[0] + s * st[1] + h * st[2]);
+}
+
+// Bytes from row s to the end of row n - 1.
+template <class T, int D> __device__ __forceinline__ int64_t span(int n, int s, int64_t stride) {
+  return n > s ? ((n - 1 - s) * stride + D) * static_cast<int64_t>(sizeof(T)) : 0;
+}
+
+// Stores a wave's accumulator (lane % 32 = row, registers = elements) times f to rows
+// of memory, the rows up to `rows` only.
+template <class T, int D>
+__device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float f, char* p, int64_t stride, int rows,
+                                           int lane) {
+  using x4 = typename El<T>::x4;
+  if ((lane & 31) >= rows) return;
+  T* row = reinterpret_cast<T*>(p) + (lane & 31) * stride + (lane >> 5) * 4;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = static_cast<T>(acc[t][g * 4 + j] * f);
+      *reinterpret_cast<x4*>(row + t * 32 + g * 8) = v;
+    }
+}
+
+// Registers 8 h .. 8 h + 7 of an accumulator, rounded: the second operand of the product
+// that sums over the accumulator's rows.
+template <class T> __device__ __forceinline__ typename El<T>::x8 operand(const f32x16& x, int h) {
+  typename El<T>::x8 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = static_cast<T>(x[h * 8 + j]);
+  return r;
+}
+
+// The row index that register r of a 32x32 accumulator holds in this lane.
+__device__ __forceinline__ int acc_row(int r, int lane) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
+
+template <class T, int D, bool CAUSAL>
+__global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention a) {
+  using E = El<T>;
+  using Tl = Tile<D>;
+  constexpr int kTile = kStep * Tl::kRow;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (a.S + kRows - 1) / kRows;
+  const int64_t total = static_cast<int64_t>(tiles) * a.B * a.H;
+  const int64_t item = xcd_item(blockIdx.x, total);
+  if ((blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
+  const int tile = tiles - 1 - static_cast<int>(item % tiles);  // causal: the long rows first
+  const int bh = static_cast<int>(item / tiles), h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk);
+  const int n = length_of(a, b);
+  const int q0 = tile * kRows, qw = q0 + wave * 32, row = qw + (lane & 31);
+
+  typename E::x8 q[D / 16];
+  const i32x4 dq = buffer(at<T>(a.q, a.q_st, b, qw, h), span<T, D>(n, qw, a.q_st[1]));
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    q[kk] = load16<typename E::x8>(dq, static_cast<int>((lane & 31) * a.q_st[1] * 2) + (kk * 2 + (lane >> 5)) * 16);
+
+  const int end = CAUSAL ? min(n, q0 + kRows) : n;          // keys any row of the workgroup sees
+  const int limit = CAUSAL ? min(row + 1, n) : n;           // keys this lane's row sees
+  const int open = CAUSAL ? min(qw + 1, n) : n;             // keys that all rows of the wave see
+  const int last = CAUSAL ? min(qw + 32, n) : n;            // keys that any row of the wave sees
+  const int steps = q0 < n ? (end + kStep - 1) / kStep : 0;
+
+  typename Tl::template Copy<kStep, kWaves> ck, cv;
+  ck.init(wave, lane, a.k_st[1] * 2);
+  cv.init(wave, lane, a.v_st[1] * 2);
+  const uint32_t lds = lds_address(smem);
+  auto fetch = [&](int j) {
+    const int s = j * kStep;
+    ck.go(buffer(at<T>(a.k, a.k_st, b, s, hk), span<T, D>(n, s, a.k_st[1])), lds + (j & 1) * 2 * kTile, wave);
+    cv.go(buffer(at<T>(a.v, a.v_st, b, s, hk), span<T, D>(n, s, a.v_st[1])), lds + (j & 1) * 2 * kTile + kTile, wave);
+  };
+
+  f32x16 o[D / 32] = {};
+  float top = -INFINITY, sum = 0.f;
+  const float c = a.scale * kLog2e;
+  if (steps > 0) fetch(0);
+  for (int j = 0; j < steps; ++j) {
+    copies_done();
+    barrier();  // step j has landed for every wave, and nobody reads the other buffer any more
+    if (j + 1 < steps) fetch(j + 1);
+    const int s0 = j * kStep;
+    if (s0 >= last) continue;
+    const char* kt = smem + (j & 1) * 2 * kTile;
+    const char* vt = kt + kTile;
+    f32x16 s[2] = {};
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[t] = E::mfma(Tl::template rows<T>(kt, t * 32, kk, lane), q[kk], s[t]);
+    if (s0 + kStep > open) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (s0 + t * 32 + acc_row(r, lane) >= limit) s[t][r] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+    mx = fmaxf(mx, other_half(mx)) * c;
+    // The subtracted maximum may lag by a factor of 2^8: the quotient is the same, and
+    // the accumulators are rescaled a few times a row instead of at every step.
+    if (__any(mx > top + 8.f)) {
+      const float now = fmaxf(top, mx), f = __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      sum *= f;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) o[t] *= f;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], c, -top));
+        sum += s[t][r];
+      }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const typename E::x8 p = operand<T>(s[t], hh);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e)
+          o[e] = E::mfma(Tl::template columns<T>(vt, t * 32 + hh * 16, e * 32, lane), p, o[e]);
+      }
+  }
+  sum += other_half(sum);
+  if (row >= n) sum = 0.f;
+  const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // a NaN stays one
+  if (row >= n)
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) o[t] = f32x16{};
+  store_rows<T, D>(o, inv, const_cast<char*>(at<T>(a.out, a.o_st, b, qw, h)), a.o_st[1], a.S - qw, lane);
+  if (a.lse && lane < 32 && row < a.S)
+    a.lse[(static_cast<int64_t>(b) * a.H + h) * a.S + row] = row < n ? top + __builtin_amdgcn_logf(sum) : -INFINITY;
+}
+
+// dq of 128 rows a workgroup, and delta of those rows for the kernel that follows.
+template <class T, int D, bool CAUSAL>
+__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention a) {
+  using E = El<T>;
+  using Tl = Tile<D>;
+  constexpr int kTile = kStep * Tl::kRow;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (a.S + kRows - 1) / kRows;
+  const int64_t total = static_cast<int64_t>(tiles) * a.B * a.H;
+  const int64_t item = xcd_item(blockIdx.x, total);
+  if ((blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
+  const int tile = tiles - 1 - static_cast<int>(item % tiles);
+  const int bh = static_cast<int>(item / tiles), h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk);
+  const int n = length_of(a, b);
+  const int q0 = tile * kRows, qw = q0 + wave * 32, row = qw + (lane & 31);
+
+  typename E::x8 q[D / 16], g[D / 16];
+  float delta = 0.f;
+  {
+    const i32x4 dq = buffer(at<T>(a.q, a.q_st, b, qw, h), span<T, D>(n, qw, a.q_st[1]));
+    const i32x4 dg = buffer(at<T>(a.dout, a.g_st, b, qw, h), span<T, D>(n, qw, a.g_st[1]));
+    const i32x4 dO = buffer(at<T>(a.out, a.o_st, b, qw, h), span<T, D>(n, qw, a.o_st[1]));
+    const int r = lane & 31, cb = (lane >> 5) * 16;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      q[kk] = load16<typename E::x8>(dq, static_cast<int>(r * a.q_st[1] * 2) + kk * 32 + cb);
+      g[kk] = load16<typename E::x8>(dg, static_cast<int>(r * a.g_st[1] * 2) + kk * 32 + cb);
+      const typename E::x8 o = load16<typename E::x8>(dO, static_cast<int>(r * a.o_st[1] * 2) + kk * 32 + cb);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = fmaf(static_cast<float>(g[kk][j]), static_cast<float>(o[j]), delta);
+    }
+    delta += other_half(delta);
+  }
+  const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.S + row;
+  if (lane < 32 && row < a.S) a.delta[stat] = delta;
+  const float lse = row < n ? a.lse[stat] : 0.f;
+
+  const int end = CAUSAL ? min(n, q0 + kRows) : n;
+  const int limit = CAUSAL ? min(row + 1, n) : n;
+  const int open = CAUSAL ? min(qw + 1, n) : n;
+  const int last = CAUSAL ? min(qw + 32, n) : n;
+  const int steps = q0 < n ? (end + kStep - 1) / kStep : 0;
+
+  typename Tl::template Copy<kStep, kWaves> ck, cv;
+  ck.init(wave, lane, a.k_st[1] * 2);
+  cv.init(wave, lane, a.v_st[1] * 2);
+  const uint32_t lds = lds_address(smem);
+  auto fetch = [&](int j) {
+    const int s = j * kStep;
+    ck.go(buffer(at<T>(a.k, a.k_st, b, s, hk), span<T, D>(n, s, a.k_st[1])), lds + (j & 1) * 2 * kTile, wave);
+    cv.go(buffer(at<T>(a.v, a.v_st, b, s, hk), span<T, D>(n, s, a.v_st[1])), lds + (j & 1) * 2 * kTile + kTile, wave);
+  };
+
+  f32x16 acc[D / 32] = {};
+  const float c = a.scale * kLog2e;
+  if (steps > 0) fetch(0);
+  for (int j = 0; j < steps; ++j) {
+    copies_done();
+    barrier();
+    if (j + 1 < steps) fetch(j + 1);
+    const int s0 = j * kStep;
+    if (s0 >= last) continue;
+    const char* kt = smem + (j & 1) * 2 * kTile;
+    const char* vt = kt + kTile;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        s = E::mfma(Tl::template rows<T>(kt, t * 32, kk, lane), q[kk], s);
+        dp = E::mfma(Tl::template rows<T>(vt, t * 32, kk, lane), g[kk], dp);
+      }
+      const bool edge = s0 + t * 32 + 32 > open;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
+        float ds = p * (dp[r] - delta);
+        s[r] = ds;
+      }
+      if (edge) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (s0 + t * 32 + acc_row(r, lane) >= limit) s[r] = 0.f;
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const typename E::x8 ds = operand<T>(s, hh);
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e)
+          acc[e] = E::mfma(Tl::template columns<T>(kt, t * 32 + hh * 16, e * 32, lane), ds, acc[e]);
+      }
+    }
+  }
+  if (row >= n)
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) acc[t] = f32x16{};
+  store_rows<T, D>(acc, a.scale, const_cast<char*>(at<T>(a.dq, a.dq_st, b, qw, h)), a.dq_st[1], a.S - qw, lane);
+}
+
+// dk and dv of 128 keys a workgroup: walks the query heads that share the key head, and
+// of each the rows that see the keys, 32 at a time.  No atomics: the order of the sums
+// is fixed.  v's fragments are read from LDS again at every step: with k's, both
+// accumulators and v's in registers a SIMD would hold one wave instead of two.
+// With splits > 1 a workgroup takes one part of the walk and leaves its sums, 32 bits,
+// in the workspace.
+template <class T, int D, bool CAUSAL>
+__global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention a) {
+  using E = El<T>;
+  using Tl = Tile<D>;
+  constexpr int kQ = 32, kTile = kQ * Tl::kRow, kV = kRows * Tl::kRow, kStage = 2 * kTile + 2 * 256;
+  __shared__ __attribute__((aligned(1024))) char smem[kV + 2 * kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (a.S + kRows - 1) / kRows;
+  const int64_t total = static_cast<int64_t>(tiles) * a.B * a.Hk * a.splits;
+  const int64_t item = xcd_item(blockIdx.x, total);
+  if ((blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
+  const int split = static_cast<int>(item % a.splits);
+  const int64_t rest = item / a.splits;
+  const int tile = static_cast<int>(rest % tiles);  // causal: the first keys have the most rows
+  const int bh = static_cast<int>(rest / tiles), hk = bh % a.Hk, b = bh / a.Hk, G = a.H / a.Hk;
+  const int n = length_of(a, b);
+  const int k0 = tile * kRows, kw = k0 + wave * 32, key = kw + (lane & 31);
+
+  // v's tile; rows past the end are zero
+  const uint32_t lds = lds_address(smem);
+  {
+    typename Tl::template Copy<kRows, kWaves> cv;
+    cv.init(wave, lane, a.v_st[1] * 2);
+    cv.go(buffer(at<T>(a.v, a.v_st, b, k0, hk), span<T, D>(n, k0, a.v_st[1])), lds, wave);
+  }
+  typename E::x8 k[D / 16];
+  const i32x4 dk = buffer(at<T>(a.k, a.k_st, b, kw, hk), span<T, D>(n, kw, a.k_st[1]));
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    k[kk] = load16<typename E::x8>(dk, static_cast<int>((lane & 31) * a.k_st[1] * 2) + (kk * 2 + (lane >> 5)) * 16);
+
+  const int first = CAUSAL ? k0 / kQ : 0;                                 // first step of rows
+  const int each = k0 < n ? (n + kQ - 1) / kQ - first : 0;                // steps a head
+  const int all = each * G;                                               // the whole walk
+  const int lo = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
+  const int hi = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits);
+
+  typename Tl::template Copy<kQ, kWaves> cq, cg;
+  cq.init(wave, lane, a.q_st[1] * 2);
+  cg.init(wave, lane, a.g_st[1] * 2);
+  // the walk's step that is fetched next: head of the group, step of that head
+  int fh = hi > lo ? lo / each : 0, fs = hi > lo ? lo % each : 0;
+  auto fetch = [&](int buf) {
+    const int h = hk * G + fh, s = (first + fs) * kQ;
+    const uint32_t to = lds + kV + buf * kStage;
+    cq.go(buffer(at<T>(a.q, a.q_st, b, s, h), span<T, D>(n, s, a.q_st[1])), to, wave);
+    cg.go(buffer(at<T>(a.dout, a.g_st, b, s, h), span<T, D>(n, s, a.g_st[1])), to + kTile, wave);
+    if (wave < 2) {  // lse or delta of the 32 rows (and of 32 more)
+      const float* p = (wave ? a.delta : a.lse) + (static_cast<int64_t>(b) * a.H + h) * a.S + s;
+      copy4(buffer(p, static_cast<int64_t>(n - s) * 4), lane * 4, to + 2 * kTile + wave * 256);
+    }
+    if (++fs == each) fs = 0, ++fh;
+  };
+
+  f32x16 dka[D / 32] = {}, dva[D / 32] = {};
+  const float c = a.scale * kLog2e;
+  int buf = 1;
+  if (lo < hi) fetch(0);
+  for (int i = lo; i < hi; ++i) {
+    buf ^= 1;
+    const int s0 = (first + (fs ? fs : each) - 1) * kQ;  // the step fetched last
+    copies_done();
+    barrier();
+    if (i + 1 < hi) fetch(buf ^ 1);
+    if (CAUSAL && s0 + kQ <= kw) continue;  // no row of the step sees the wave's keys
+    const char* qt = smem + kV + buf * kStage;
+    const char* gt = qt + kTile;
+    const float* lse = reinterpret_cast<const float*>(gt + kTile);
+    f32x16 s = {}, dp = {};
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      s = E::mfma(Tl::template rows<T>(qt, 0, kk, lane), k[kk], s);
+      dp = E::mfma(Tl::template rows<T>(gt, 0, kk, lane), Tl::template rows<T>(smem, wave * 32, kk, lane), dp);
+    }
+    // Rows past the end hold zeros for q, do, lse and delta: p = 1 there, times zero.
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const f32x4 l = *reinterpret_cast<const f32x4*>(lse + m * 8 + (lane >> 5) * 4);
+      const f32x4 d = *reinterpret_cast<const f32x4*>(lse + 64 + m * 8 + (lane >> 5) * 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = m * 4 + j;
+        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l[j]));
+        dp[r] = s[r] * (dp[r] - d[j]);
+      }
+    }
+    if (CAUSAL && s0 < kw + 31) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (s0 + acc_row(r, lane) < key) s[r] = dp[r] = 0.f;
+    }
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const typename E::x8 p = operand<T>(s, hh), ds = operand<T>(dp, hh);
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) {
+        dva[e] = E::mfma(Tl::template columns<T>(gt, hh * 16, e * 32, lane), p, dva[e]);
+        dka[e] = E::mfma(Tl::template columns<T>(qt, hh * 16, e * 32, lane), ds, dka[e]);
+      }
+    }
+  }
+  copies_done();  // v's tile, if the walk was empty
+  if (a.splits > 1) {
+    if (key < a.S) {
+      const int64_t part = static_cast<int64_t>(a.B) * a.S * a.Hk * D;
+      float* w = a.partial + split * 2 * part + ((static_cast<int64_t>(b) * a.S + key) * a.Hk + hk) * D;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4 x, y;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = dka[t][g * 4 + j], y[j] = dva[t][g * 4 + j];
+          const int e = t * 32 + g * 8 + (lane >> 5) * 4;
+          *reinterpret_cast<f32x4*>(w + e) = x;
+          *reinterpret_cast<f32x4*>(w + part + e) = y;
+        }
+    }
+    return;
+  }
+  if (key >= n)
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) dka[t] = dva[t] = f32x16{};
+  store_rows<T, D>(dka, a.scale, const_cast<char*>(at<T>(a.dk, a.dk_st, b, kw, hk)), a.dk_st[1], a.S - kw, lane);
+  store_rows<T, D>(dva, 1.f, const_cast<char*>(at<T>(a.dv, a.dv_st, b, kw, hk)), a.dv_st[1], a.S - kw, lane);
+}
+
+// Adds the parts of a split walk, in their order: 4 elements a thread of dk, then of dv.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attention_join_kernel(KgsAttention a) {
+  using x4 = typename El<T>::x4;
+  const int64_t part = static_cast<int64_t>(a.B) * a.S * a.Hk * D, i = (blockIdx.x * 256ll + threadIdx.x) * 4;
+  if (i >= 2 * part) return;
+  const bool v = i >= part;
+  const int64_t e = v ? i - part : i;
+  const int d = static_cast<int>(e % D), hk = static_cast<int>(e / D % a.Hk);
+  const int64_t bs = e / D / a.Hk;
+  const int s = static_cast<int>(bs % a.S), b = static_cast<int>(bs / a.S);
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  if (s < (a.lengths ? min(a.lengths[b], a.S) : a.S))
+    for (int p = 0; p < a.splits; ++p) sum += *reinterpret_cast<const f32x4*>(a.partial + p * 2 * part + i);
+  x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = static_cast<T>(v ? sum[j] : sum[j] * a.scale);
+  char* to = const_cast<char*>(v ? at<T>(a.dv, a.dv_st, b, s, hk) : at<T>(a.dk, a.dk_st, b, s, hk));
+  *reinterpret_cast<x4*>(to + d * 2) = r;
+}
+
+int check(const KgsAttention* a, bool backward) {
+  const char* w = "attention";
+  if (!a || !a->q || !a->k || !a->v || !a->out) return fail(w, "a tensor is missing");
+  if (a->B < 0 || a->S < 0 || a->H <= 0 || a->Hk <= 0 || a->H % a->Hk) return fail(w, "bad sizes");
+  if (a->D != 64 && a->D != 128) return fail(w, "head dimension must be 64 or 128");
+  if (a->type != 0 && a->type != 1) return fail(w, "type must be bfloat16 or float16");
+  if (backward && (!a->dout || !a->lse || !a->delta || !a->dq || !a->dk || !a->dv)) return fail(w, "a tensor is missing");
+  if (backward && (a->splits < 1 || (a->splits > 1 && !a->partial))) return fail(w, "bad split");
+  const int64_t* st[] = {a->q_st, a->k_st, a->v_st, a->o_st, a->g_st, a->dq_st, a->dk_st, a->dv_st};
+  for (int i = 0; i < (backward ? 8 : 4); ++i)
+    for (int j = 0; j < 3; ++j)
+      // rows behind the last lie past the descriptor's end; offsets inside a tile stay under 2^30
+      if (st[i][j] < 0 || st[i][j] % 8 || (j == 1 && (st[i][j] < a->D || st[i][j] > (1 << 22)))) return fail(w, "unsupported strides");
+  const int64_t tiles = (a->S + kRows - 1) / kRows;
+  if (tiles * a->B * a->H * (backward ? a->splits : 1) > 0x7FFFFF00ll) return fail(w, "too many workgroups");
+  return 0;
+}
+
+unsigned grid(int64_t total) { return static_cast<unsigned>((total + 7) / 8 * 8); }
+
+template <class T, int D, bool CAUSAL> int forward(const KgsAttention& a, hipStream_t s) {
+  const int64_t tiles = (a.S + kRows - 1) / kRows;
+  attention_fwd_kernel<T, D, CAUSAL><<<grid(tiles * a.B * a.H), kThreads, 0, s>>>(a);
+  return launched("attention forward");
+}
+
+template <class T, int D, bool CAUSAL> int backward(const KgsAttention& a, hipStream_t s) {
+  const int64_t tiles = (a.S + kRows - 1) / kRows;
+  attention_dq_kernel<T, D, CAUSAL><<<grid(tiles * a.B * a.H), kThreads, 0, s>>>(a);
+  if (launched("attention dq")) return -1;
+  attention_dkv_kernel<T, D, CAUSAL><<<grid(tiles * a.B * a.Hk * a.splits), kThreads, 0, s>>>(a);
+  if (launched("attention dk, dv")) return -1;
+  if (a.splits > 1) {
+    const int64_t n = 2 * static_cast<int64_t>(a.B) * a.S * a.Hk * D / 4;
+    attention_join_kernel<T, D><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(a);
+    return launched("attention join");
+  }
+  return 0;
+}
+
+template <class T, int D> int run(const KgsAttention& a, bool back, hipStream_t s) {
+  if (back) return a.causal ? backward<T, D, true>(a, s) : backward<T, D, false>(a, s);
+  return a.causal ? forward<T, D, true>(a, s) : forward<T, D, false>(a, s);
+}
+
+int dispatch(const KgsAttention* a, bool back, void* stream) {
+  if (check(a, back)) return -1;
+  if (a->B == 0 || a->S == 0) return 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a->type == 0) return a->D == 64 ? run<bf16, 64>(*a, back, s) : run<bf16, 128>(*a, back, s);
+  return a->D == 64 ? run<f16, 64>(*a, back, s) : run<f16, 128>(*a, back, s);
+}
+
+}  // namespace
+}  // namespace kgs
+
+extern "C" {
+int kgs_attention_fwd(const KgsAttention* a, void* stream) { return kgs::dispatch(a, false, stream); }
+int kgs_attention_bwd(const KgsAttention* a, void* stream) { return kgs::dispatch(a, true, stream); }
+}

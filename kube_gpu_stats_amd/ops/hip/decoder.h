@@ -1,0 +1,60 @@
+// C interface of libkgs_decoder.so (loaded with ctypes by kube_gpu_stats_amd/ops/decoder.py,
+// whose Structures repeat these layouts field by field).  Every entry launches on `stream`,
+// returns 0, or -1 with kgs_decoder_last_error() set.
+#pragma once
+#include <cstdint>
+
+extern "C" {
+
+// Tensors [B, S, heads, D]; strides in elements of (B, S, heads), D contiguous; pointers
+// 16-byte aligned, strides multiples of 8.  lse, delta: float [B, H, S].
+struct KgsAttention {
+  const void *q, *k, *v;
+  void* out;
+  const void* dout;
+  void *dq, *dk, *dv;
+  float *lse, *delta, *partial;  // partial: float [splits, 2, B, S, Hk, D]
+  const int32_t* lengths;        // [B] or null
+  int64_t q_st[3], k_st[3], v_st[3], o_st[3], g_st[3], dq_st[3], dk_st[3], dv_st[3];
+  int32_t B, S, H, Hk, D, type, causal, splits;  // type: 0 bfloat16, 1 float16
+  float scale;
+};
+
+// x [T, K] and w [2F, K] with row strides, h [T, F], saved [T, 2F] (null: not kept), dh [T, F]
+// with a row stride, dgu [T, 2F], dx [T, K], dw [2F, K] (either null: not wanted).  Pointers
+// 16-byte aligned; K, F and strides multiples of 8.  tile, splits: of the forward product,
+// of dx and of dw.  partial: float [splits, rows, columns] of the largest split product.
+struct KgsSwiglu {
+  const void *x, *w;
+  void *h, *saved;
+  const void* dh;
+  void *dgu, *dx, *dw;
+  float* partial;
+  int64_t x_ld, w_ld, dh_ld;
+  int32_t T, K, F, type;
+  int32_t tile[3], splits[3];
+};
+
+// Rows of `width` elements; row strides in elements.  rstd float [2, rows] (of the stream, of
+// the branch); dstream and dout may be null (zero).  post_weight and gate may be null.
+// partial: float [parts, 3, width].  dbranch may equal dresidual where they are the same.
+struct KgsAddNorm {
+  const void *residual, *branch, *weight, *post_weight, *gate;
+  void *stream, *out;
+  float* rstd;
+  const void *dstream, *dout;
+  void *dresidual, *dbranch, *dweight, *dpost_weight, *dgate;
+  float* partial;
+  int64_t residual_ld, branch_ld, stream_ld, dstream_ld, dout_ld;
+  int32_t rows, width, type, parts;  // type: 0 bfloat16, 1 float16, 2 float32
+  float scale, eps;
+};
+
+const char* kgs_decoder_last_error();
+int kgs_swiglu_fwd(const KgsSwiglu* a, void* stream);
+int kgs_swiglu_bwd(const KgsSwiglu* a, void* stream);
+int kgs_add_norm_fwd(const KgsAddNorm* a, void* stream);
+int kgs_add_norm_bwd(const KgsAddNorm* a, void* stream);
+int kgs_attention_fwd(const KgsAttention* a, void* stream);
+int kgs_attention_bwd(const KgsAttention* a, void* stream);
+}

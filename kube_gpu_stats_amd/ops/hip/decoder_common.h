@@ -1,0 +1,176 @@
+// What the decoder block's kernels share on gfx950: element types and their matrix
+// instruction, buffer descriptors whose range check keeps every load in bounds, copies
+// from memory straight into LDS, and the swizzled tile that both row-wise and
+// transposed fragment reads walk without bank conflicts.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace kgs {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using i32x4 = __attribute__((ext_vector_type(4))) int;
+using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
+
+constexpr int kWave = 64;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+template <class T> struct El;
+template <> struct El<bf16> {
+  using x2 = __attribute__((ext_vector_type(2))) bf16;
+  using x4 = __attribute__((ext_vector_type(4))) bf16;
+  using x8 = __attribute__((ext_vector_type(8))) bf16;
+  static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ x4 read_tr(const char* lds) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) x4*)lds);
+  }
+};
+template <> struct El<f16> {
+  using x2 = __attribute__((ext_vector_type(2))) f16;
+  using x4 = __attribute__((ext_vector_type(4))) f16;
+  using x8 = __attribute__((ext_vector_type(8))) f16;
+  static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ x4 read_tr(const char* lds) {
+    using i16x4 = __attribute__((ext_vector_type(4))) short;
+    return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)lds));
+  }
+};
+
+template <class T> __device__ __forceinline__ typename El<T>::x8 join(typename El<T>::x4 a, typename El<T>::x4 b) {
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// A raw buffer descriptor over [base, base + bytes): a lane's access past it reads 0 or
+// stores nothing, dword by dword.  Offsets are 32 bits, so callers move the base (64
+// bits) from tile to tile and keep offsets inside one tile (under 2^30); an offset of
+// kFar is past the end of any.
+constexpr uint32_t kFar = 0x7FFFFFE0u;
+__device__ __forceinline__ i32x4 buffer(const void* base, int64_t bytes) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  bytes = bytes < 0 ? 0 : bytes;
+  const uint32_t n = bytes > kFar ? kFar : static_cast<uint32_t>(bytes);
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(p));
+  r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>(p >> 32) & 0xFFFF);
+  r[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(n));
+  r[3] = 0x00027000;
+  return r;
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(i32x4 d) {
+  const uint64_t p = static_cast<uint32_t>(d[0]) | (static_cast<uint64_t>(static_cast<uint32_t>(d[1])) << 32);
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(p), 0, d[2], 0x00027000);
+}
+
+template <class V> __device__ __forceinline__ V load16(i32x4 d, int voff) {
+  return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(rsrc(d), voff, 0, 0));
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
+}
+
+// 16 (or 4) bytes a lane from memory to LDS at lds + lane * 16 (or 4); lds must be the
+// same in the whole wave.  Written as assembly because the compiler, which cannot tell
+// the buffer being filled from the one being read, would wait for the copy before the
+// next LDS read; there is no result register, and copies_done() is the wait.  The s_nop
+// covers what the compiler would: a scalar register written by a vector instruction (the
+// descriptor's readfirstlane) is not read by a memory instruction within 5 states.
+__device__ __forceinline__ void copy16(i32x4 d, int voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(d)
+               : "memory");
+}
+__device__ __forceinline__ void copy4(i32x4 d, int voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(d)
+               : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ void barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// A tile of rows of W elements (W = 64 or 128) in LDS, in 16-byte chunks, chunk c of a
+// row at c ^ swizzle(row).  256 bytes (all 64 banks) are one row of 128 or two of 64.
+// Row-wise reads take the same chunk of 32 rows: 16 rows in turn land on 16 places.
+// Transposed reads take 64 bytes of 4 rows in turn: the swizzle's high bits come from
+// the row's low ones, so that the four lie in different quarters of the 256 bytes.
+template <int W> struct Tile {
+  static constexpr int kRow = W * 2;
+  static __device__ __forceinline__ int swizzle(int row) {
+    if constexpr (W == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else return ((row & 2) << 1) | ((row >> 2) & 3);
+  }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * kRow + ((chunk ^ swizzle(row)) << 4); }
+
+  // Lane's fragment of rows r0..r0+31, elements 16 kk..16 kk + 15: row lane % 32,
+  // 8 elements from 16 kk + 8 (lane / 32).
+  template <class T> static __device__ __forceinline__ typename El<T>::x8 rows(const char* t, int r0, int kk, int lane) {
+    return *reinterpret_cast<const typename El<T>::x8*>(t + r0 * kRow + at(lane & 31, kk * 2 + (lane >> 5)));
+  }
+  // The transposed fragment in the order of rows(): lane holds element e0 + lane % 32 of
+  // rows r0 + 8 (lane / 32) + {0..7}.
+  template <class T> static __device__ __forceinline__ typename El<T>::x8 columns_in_order(const char* t, int r0, int e0,
+                                                                                           int lane) {
+    const int i = lane & 15, row = (lane >> 5) * 8 + (i >> 2);
+    const int chunk = (e0 >> 3) + ((lane >> 4) & 1) * 2 + ((i >> 1) & 1);
+    const char* p = t + r0 * kRow + (i & 1) * 8;
+    return join<T>(El<T>::read_tr(p + at(row, chunk)), El<T>::read_tr(p + at(row + 4, chunk)));
+  }
+  // The transposed fragment: lane holds element e0 + lane % 32 of 8 rows, the rows
+  // that an accumulator of the 32x32 product keeps in its registers 8 h .. 8 h + 7:
+  // r0 + 4 (lane / 32) + {0..3} and 8 more.  r0 a multiple of 16.
+  template <class T> static __device__ __forceinline__ typename El<T>::x8 columns(const char* t, int r0, int e0, int lane) {
+    const int i = lane & 15, row = (lane >> 5) * 4 + (i >> 2);
+    const int chunk = (e0 >> 3) + ((lane >> 4) & 1) * 2 + ((i >> 1) & 1);
+    const char* p = t + r0 * kRow + (i & 1) * 8;
+    return join<T>(El<T>::read_tr(p + at(row, chunk)), El<T>::read_tr(p + at(row + 8, chunk)));
+  }
+  // Wave w of NW copies its part of ROWS rows, stride bytes apart in memory, to LDS.
+  template <int ROWS, int NW> struct Copy {
+    static constexpr int kAll = ROWS * kRow / 1024, kN = (kAll + NW - 1) / NW;
+    int voff[kN];
+    __device__ __forceinline__ void init(int wave, int lane, int64_t stride) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        const int byte = (wave * kN + i) * 1024 + lane * 16, row = byte / kRow, pc = (byte >> 4) & (W / 8 - 1);
+        voff[i] = static_cast<int>(row * stride) + ((pc ^ swizzle(row)) << 4);
+      }
+    }
+    __device__ __forceinline__ void go(i32x4 d, uint32_t lds, int wave) const {
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        if (kAll % NW == 0 || wave * kN + i < kAll) copy16(d, voff[i], lds + (wave * kN + i) * 1024);
+    }
+  };
+};
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// Workgroup id -> work item so that neighbouring items run on one of the 8 XCDs (ids
+// go round them in turn) and share its L2.  Returns total or more for no work.
+__device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t total) {
+  const int64_t per = (total + 7) / 8;
+  return (id & 7) * per + (id >> 3);
+}
+
+// Error text of the calling thread's last failed entry, and its setter.
+extern thread_local char g_decoder_error[256];
+int fail(const char* what, const char* why);
+int launched(const char* what);
+
+}  // namespace kgs

@@ -1,0 +1,322 @@
+// The gated half of a feed-forward block, forward and backward, for gfx950.
+//
+//   g = x Wg^T, u = x Wu^T, h = silu(g) u            x [T, K], W = [Wg; Wu] [2F, K]
+//   dg = dh u silu'(g), du = dh silu(g)
+//   dx = dg Wg + du Wu = [dg du] W,   dW = [dg du]^T x
+//
+// One matrix product kernel serves the three products.  A workgroup's tile of the
+// forward product takes the same columns of Wg and Wu, so that a wave holds g and u of
+// the same elements and the activation and the product are its epilogue: h is written
+// once, and g and u only if a backward pass will want them.
+//
+// Tiles of both operands go from memory straight to LDS, two steps of 64 of the summed
+// index deep, as they lie in memory; an operand whose summed index is not the
+// contiguous one is transposed by the LDS read.  Accumulators are 32 bits.  Rounded to
+// the tensors' type: g and u as saved (the forward's own h uses them unrounded), dg and
+// du as operands of the two products, and the outputs.
+#include "decoder.h"
+#include "decoder_common.h"
+
+namespace kgs {
+namespace {
+
+constexpr int kK = 64;  // summed index a step
+
+struct Product {
+  const void *a, *b;   // a: [M, K] or, transposed, [K, M]; b: [N, K] or, transposed, [K, N]
+  int64_t a_ld, b_ld;  // elements
+  void *c, *saved;     // c [M, N] contiguous (pairs: [M, N / 2]); saved [M, N] or null
+  float* partial;      // splits > 1: [splits, M, N]
+  int M, N, K, splits;
+};
+
+// One operand's tile of ROWS indexes by kK of the sum, and its fragments.
+template <class T, int ROWS, bool TR, int NW> struct Operand;
+
+template <class T, int ROWS, int NW> struct Operand<T, ROWS, false, NW> {
+  using Tl = Tile<kK>;
+  using Cp = typename Tl::template Copy<ROWS, NW>;
+  static constexpr int kBytes = ROWS * kK * 2;
+  Cp copy;
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld) { copy.init(wave, lane, ld * 2); }
+  // rows r0.. (rows - r0 of them), sum indexes k0.. of K; chunks past K are read as zero
+  __device__ __forceinline__ void go(const void* p, int64_t ld, int r0, int rows, int k0, int K, uint32_t lds, int wave,
+                                     int lane) const {
+    const int64_t bytes = rows > r0 ? ((rows - 1 - r0) * ld + (K - k0)) * 2 : 0;
+    const i32x4 d = buffer(static_cast<const T*>(p) + r0 * ld + k0, bytes);
+    if (k0 + kK <= K) return copy.go(d, lds, wave);
+#pragma unroll
+    for (int i = 0; i < Cp::kN; ++i) {
+      const int byte = (wave * Cp::kN + i) * 1024 + lane * 16, row = byte / Tl::kRow;
+      const int chunk = ((byte >> 4) & 7) ^ Tl::swizzle(row);
+      if (Cp::kAll % NW == 0 || wave * Cp::kN + i < Cp::kAll)
+        copy16(d, k0 + chunk * 8 < K ? copy.voff[i] : static_cast<int>(kFar), lds + (wave * Cp::kN + i) * 1024);
+    }
+  }
+  static __device__ __forceinline__ typename El<T>::x8 read(const char* t, int r0, int kk, int lane) {
+    return Tl::template rows<T>(t, r0, kk, lane);
+  }
+};
+
+template <class T, int ROWS, int NW> struct Operand<T, ROWS, true, NW> {
+  static constexpr int W = ROWS >= 128 ? 128 : 64, kSub = ROWS / W, kSubBytes = kK * W * 2;
+  using Tl = Tile<W>;
+  using Cp = typename Tl::template Copy<kK, NW>;
+  static constexpr int kBytes = kSub * kSubBytes;
+  Cp copy;
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld) { copy.init(wave, lane, ld * 2); }
+  __device__ __forceinline__ void go(const void* p, int64_t ld, int r0, int rows, int k0, int K, uint32_t lds, int wave,
+                                     int) const {
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) {
+      const int r = r0 + s * W;
+      const int64_t bytes = rows > r ? ((K - 1 - k0) * ld + (rows - r)) * 2 : 0;
+      copy.go(buffer(static_cast<const T*>(p) + k0 * ld + r, bytes), lds + s * kSubBytes, wave);
+    }
+  }
+  static __device__ __forceinline__ typename El<T>::x8 read(const char* t, int r0, int kk, int lane) {
+    return Tl::template columns_in_order<T>(t + r0 / W * kSubBytes, kk * 16, r0 % W, lane);
+  }
+};
+
+// silu(g) = g / (1 + 2^(-g log2 e)): an overflowing power makes the quotient 0.
+__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + __builtin_amdgcn_exp2f(-g * kLog2e)); }
+
+// c = a b over tiles of BM x BN, WM x WN waves.  PAIR: the columns of a tile are BN / 2
+// of the first half of N and the same of the second.
+template <class T, int BM, int BN, int WM, int WN, bool TA, bool TB, bool PAIR>
+__global__ __launch_bounds__(WM * WN * 64, 2) void product_kernel(Product p) {
+  using E = El<T>;
+  constexpr int NW = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32, HALF = BN / 2;
+  using OA = Operand<T, BM, TA, NW>;
+  using OB = Operand<T, PAIR ? HALF : BN, TB, NW>;
+  constexpr int kB = PAIR ? 2 * OB::kBytes : OB::kBytes, kStage = OA::kBytes + kB;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int N = PAIR ? p.N / 2 : p.N;  // columns of c
+  const int tm = (p.M + BM - 1) / BM, tn = (N + (PAIR ? HALF : BN) - 1) / (PAIR ? HALF : BN);
+  const int64_t total = static_cast<int64_t>(tm) * tn * p.splits;
+  const int64_t item = xcd_item(blockIdx.x, total);
+  if ((blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
+  // Items in bands of 8 tiles of rows: an XCD's workgroups share 8 row tiles and few
+  // column tiles through their L2.
+  const int split = static_cast<int>(item / (static_cast<int64_t>(tm) * tn));
+  const int t = static_cast<int>(item % (static_cast<int64_t>(tm) * tn));
+  const int band = t / (8 * tn), high = min(8, tm - band * 8), in = t - band * 8 * tn;
+  const int m0 = (band * 8 + in % high) * BM, n0 = in / high * (PAIR ? HALF : BN);
+  const int steps_all = (p.K + kK - 1) / kK;
+  const int lo = static_cast<int>(static_cast<int64_t>(steps_all) * split / p.splits);
+  const int hi = static_cast<int>(static_cast<int64_t>(steps_all) * (split + 1) / p.splits);
+
+  OA oa;
+  OB ob;
+  oa.init(wave, lane, p.a_ld);
+  ob.init(wave, lane, p.b_ld);
+  const uint32_t lds = lds_address(smem);
+  auto fetch = [&](int j) {
+    const uint32_t to = lds + (j & 1) * kStage;
+    oa.go(p.a, p.a_ld, m0, p.M, j * kK, p.K, to, wave, lane);
+    ob.go(p.b, p.b_ld, n0, N, j * kK, p.K, to + OA::kBytes, wave, lane);
+    if (PAIR)
+      ob.go(static_cast<const T*>(p.b) + N * p.b_ld, p.b_ld, n0, N, j * kK, p.K, to + OA::kBytes + OB::kBytes, wave, lane);
+  };
+
+  f32x16 acc[MT][NT] = {};
+  if (lo < hi) fetch(lo);
+  for (int j = lo; j < hi; ++j) {
+    copies_done();
+    barrier();
+    if (j + 1 < hi) fetch(j + 1);
+    const char* at = smem + (j & 1) * kStage;
+    const char* bt = at + OA::kBytes;
+#pragma unroll
+    for (int kk = 0; kk < kK / 16; ++kk) {
+      typename E::x8 a[MT], b[NT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) a[i] = OA::read(at, wm * MT * 32 + i * 32, kk, lane);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        b[i] = PAIR ? OB::read(bt + (i < NT / 2 ? 0 : OB::kBytes), wn * NT * 16 + i % (NT / 2 ? NT / 2 : 1) * 32, kk, lane)
+                    : OB::read(bt, wn * NT * 32 + i * 32, kk, lane);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int k = 0; k < NT; ++k) acc[i][k] = E::mfma(b[k], a[i], acc[i][k]);
+    }
+  }
+
+  // lane % 32 = row of c, registers = columns, 4 in a row each
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int m = m0 + wm * MT * 32 + i * 32 + (lane & 31);
+    if (m >= p.M) continue;
+#pragma unroll
+    for (int k = 0; k < (PAIR ? NT / 2 : NT); ++k)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int n = n0 + wn * (PAIR ? NT * 16 : NT * 32) + k * 32 + g * 8 + (lane >> 5) * 4;
+        if (n >= N) continue;  // N is a multiple of 8
+        if (p.splits > 1) {
+          f32x4 x, y;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = acc[i][k][g * 4 + j], y[j] = PAIR ? acc[i][(NT / 2 + k) % NT][g * 4 + j] : 0.f;
+          float* to = p.partial + (static_cast<int64_t>(split) * p.M + m) * p.N + n;
+          *reinterpret_cast<f32x4*>(to) = x;
+          if (PAIR) *reinterpret_cast<f32x4*>(to + N) = y;
+        } else if (PAIR) {
+          typename E::x4 h, x, y;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float gate = acc[i][k][g * 4 + j], up = acc[i][(NT / 2 + k) % NT][g * 4 + j];
+            h[j] = static_cast<T>(gate * sigmoid(gate) * up);
+            x[j] = static_cast<T>(gate);
+            y[j] = static_cast<T>(up);
+          }
+          *reinterpret_cast<typename E::x4*>(static_cast<T*>(p.c) + static_cast<int64_t>(m) * N + n) = h;
+          if (p.saved) {
+            T* to = static_cast<T*>(p.saved) + static_cast<int64_t>(m) * p.N + n;
+            *reinterpret_cast<typename E::x4*>(to) = x;
+            *reinterpret_cast<typename E::x4*>(to + N) = y;
+          }
+        } else {
+          typename E::x4 x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = static_cast<T>(acc[i][k][g * 4 + j]);
+          *reinterpret_cast<typename E::x4*>(static_cast<T*>(p.c) + static_cast<int64_t>(m) * N + n) = x;
+        }
+      }
+  }
+}
+
+// The parts of a split product, added in their order, 4 columns a thread.
+template <class T, bool PAIR> __global__ __launch_bounds__(256) void join_kernel(Product p) {
+  using x4 = typename El<T>::x4;
+  const int N = PAIR ? p.N / 2 : p.N;
+  const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4;
+  if (i >= static_cast<int64_t>(p.M) * N) return;
+  const int64_t m = i / N, n = i % N, part = static_cast<int64_t>(p.M) * p.N;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+  const float* from = p.partial + m * p.N + n;
+  for (int s = 0; s < p.splits; ++s) {
+    x += *reinterpret_cast<const f32x4*>(from + s * part);
+    if (PAIR) y += *reinterpret_cast<const f32x4*>(from + s * part + N);
+  }
+  x4 h, g, u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    h[j] = static_cast<T>(PAIR ? x[j] * sigmoid(x[j]) * y[j] : x[j]);
+    g[j] = static_cast<T>(x[j]);
+    u[j] = static_cast<T>(y[j]);
+  }
+  *reinterpret_cast<x4*>(static_cast<T*>(p.c) + i) = h;
+  if (PAIR && p.saved) {
+    T* to = static_cast<T*>(p.saved) + m * p.N + n;
+    *reinterpret_cast<x4*>(to) = g;
+    *reinterpret_cast<x4*>(to + N) = u;
+  }
+}
+
+// [dg du] from dh and the saved [g u], 8 columns a thread.
+template <class T> __global__ __launch_bounds__(256) void gate_bwd_kernel(const T* dh, int64_t dh_ld, const T* saved, T* d,
+                                                                         int M, int F) {
+  using x8 = typename El<T>::x8;
+  const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 8;
+  if (i >= static_cast<int64_t>(M) * F) return;
+  const int64_t m = i / F, n = i % F;
+  const x8 a = *reinterpret_cast<const x8*>(dh + m * dh_ld + n);
+  const x8 g = *reinterpret_cast<const x8*>(saved + m * 2 * F + n);
+  const x8 u = *reinterpret_cast<const x8*>(saved + m * 2 * F + F + n);
+  x8 dg, du;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float gate = static_cast<float>(g[j]), grad = static_cast<float>(a[j]), s = sigmoid(gate);
+    dg[j] = static_cast<T>(grad * static_cast<float>(u[j]) * s * (1.f + gate * (1.f - s)));
+    du[j] = static_cast<T>(grad * gate * s);
+  }
+  *reinterpret_cast<x8*>(d + m * 2 * F + n) = dg;
+  *reinterpret_cast<x8*>(d + m * 2 * F + F + n) = du;
+}
+
+template <class T, int BM, int BN, int WM, int WN, bool TA, bool TB, bool PAIR>
+int product_tiled(const Product& p, hipStream_t s) {
+  constexpr int kLds = 2 * (BM + BN) * kK * 2;
+  const auto kernel = product_kernel<T, BM, BN, WM, WN, TA, TB, PAIR>;
+  // more than the default 64 KiB: once a device, and harmless when repeated
+  if (kLds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e != hipSuccess) return fail("swiglu LDS", hipGetErrorString(e));
+  }
+  const int N = PAIR ? p.N / 2 : p.N, bn = PAIR ? BN / 2 : BN;
+  const int64_t total = static_cast<int64_t>((p.M + BM - 1) / BM) * ((N + bn - 1) / bn) * p.splits;
+  if (total > 0x7FFFFF00ll) return fail("swiglu", "too many workgroups");
+  kernel<<<static_cast<unsigned>((total + 7) / 8 * 8), WM * WN * 64, kLds, s>>>(p);
+  if (launched("swiglu product")) return -1;
+  if (p.splits > 1) {
+    const int64_t n = static_cast<int64_t>(p.M) * N / 4;
+    join_kernel<T, PAIR><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p);
+    return launched("swiglu join");
+  }
+  return 0;
+}
+
+template <class T, bool TA, bool TB, bool PAIR> int product(const Product& p, int tile, hipStream_t s) {
+  switch (tile) {
+    case 0: return product_tiled<T, 128, 128, 2, 2, TA, TB, PAIR>(p, s);
+    case 1: return product_tiled<T, 256, 256, 2, 4, TA, TB, PAIR>(p, s);
+  }
+  return fail("swiglu", "unknown tile");
+}
+
+template <class T> int forward(const KgsSwiglu& a, hipStream_t s) {
+  const Product p{a.x, a.w, a.x_ld, a.w_ld, a.h, a.saved, a.partial, a.T, 2 * a.F, a.K, a.splits[0]};
+  return product<T, false, false, true>(p, a.tile[0], s);
+}
+
+template <class T> int backward(const KgsSwiglu& a, hipStream_t s) {
+  const int64_t n = static_cast<int64_t>(a.T) * a.F / 8;
+  gate_bwd_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(
+      static_cast<const T*>(a.dh), a.dh_ld, static_cast<const T*>(a.saved), static_cast<T*>(a.dgu), a.T, a.F);
+  if (launched("swiglu gate backward")) return -1;
+  if (a.dx) {
+    const Product p{a.dgu, a.w, 2ll * a.F, a.w_ld, a.dx, nullptr, a.partial, a.T, a.K, 2 * a.F, a.splits[1]};
+    if (product<T, false, true, false>(p, a.tile[1], s)) return -1;
+  }
+  if (a.dw) {
+    const Product p{a.dgu, a.x, 2ll * a.F, a.x_ld, a.dw, nullptr, a.partial, 2 * a.F, a.K, a.T, a.splits[2]};
+    if (product<T, true, true, false>(p, a.tile[2], s)) return -1;
+  }
+  return 0;
+}
+
+int check(const KgsSwiglu* a, bool back) {
+  const char* w = "swiglu";
+  if (!a || !a->x || !a->w || (!back && !a->h)) return fail(w, "a tensor is missing");
+  if (back && (!a->dh || !a->saved || !a->dgu)) return fail(w, "a tensor is missing");
+  if (a->T <= 0 || a->K <= 0 || a->F <= 0 || a->K % 8 || a->F % 8) return fail(w, "bad sizes");
+  // offsets inside a tile of 256 rows stay under 2^30
+  if (a->K > (1 << 20) || a->F > (1 << 20)) return fail(w, "too wide");
+  if (a->x_ld < a->K || a->w_ld < a->K || a->x_ld % 8 || a->w_ld % 8 || a->x_ld > (1 << 21) || a->w_ld > (1 << 21))
+    return fail(w, "unsupported strides");
+  if (back && (a->dh_ld < a->F || a->dh_ld % 8)) return fail(w, "unsupported strides");
+  if (a->type != 0 && a->type != 1) return fail(w, "type must be bfloat16 or float16");
+  for (int i = back ? 1 : 0; i < (back ? 3 : 1); ++i)
+    if (a->splits[i] < 1 || (a->splits[i] > 1 && !a->partial)) return fail(w, "bad split");
+  return 0;
+}
+
+}  // namespace
+}  // namespace kgs
+
+extern "C" {
+int kgs_swiglu_fwd(const KgsSwiglu* a, void* stream) {
+  if (kgs::check(a, false)) return -1;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return a->type == 0 ? kgs::forward<kgs::bf16>(*a, s) : kgs::forward<kgs::f16>(*a, s);
+}
+int kgs_swiglu_bwd(const KgsSwiglu* a, void* stream) {
+  if (kgs::check(a, true)) return -1;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return a->type == 0 ? kgs::backward<kgs::bf16>(*a, s) : kgs::backward<kgs::f16>(*a, s);
+}
+}
