@@ -53,7 +53,7 @@ def lib() -> ctypes.CDLL:
 
 
 # The C structures of ops/hip/decoder.h, field by field.
-_ATTENTION = struct.Struct("@12P24q8if")
+_ATTENTION = struct.Struct("@13P24q8if")
 _SWIGLU = struct.Struct("@9P3q4i3i3i")
 _ADD_NORM = struct.Struct("@16P5q4i2f")
 
@@ -144,7 +144,7 @@ def _attention_checks(q, k, v, scale, lengths, **more):
     B, S, H, D = q.shape
     Hk = k.shape[2]
     code = _type(q, "q", "bfloat16 or float16")
-    _same(q, "q", k=k, v=v, **{n: t for n, t in more.items() if n != "lse"})
+    _same(q, "q", k=k, v=v, **{n: t for n, t in more.items() if n not in ("lse", "low")})
     _shape(k, "k", (B, S, Hk, D))
     _shape(v, "v", (B, S, Hk, D))
     for name, t in more.items():
@@ -166,9 +166,9 @@ def _attention_checks(q, k, v, scale, lengths, **more):
             raise ValueError(f"lengths is on {lengths.device}, q is on {q.device}")
         lengths = lengths.contiguous()
     if "lse" in more:
-        lse = more["lse"]
-        if lse.dtype != torch.float32 or not lse.is_contiguous() or lse.device != q.device:
-            raise ValueError("lse must be the float32 tensor that attention_fwd returned")
+        for name, t in (("lse", torch.float32), ("low", torch.uint8)):
+            if more[name].dtype != t or not more[name].is_contiguous() or more[name].device != q.device:
+                raise ValueError(f"{name} must be the {t} tensor that attention_fwd returned")
     _on_gpu(q, "q")
     return B, S, H, Hk, D, code, scale, lengths
 
@@ -215,8 +215,9 @@ def _split_qkv(qkv, heads: int):
 
 
 def attention_fwd(q, k, v, *, causal: bool = True, scale: float | None = None, lengths=None, stream=None):
-    """``attention`` without autograd: (out, lse), lse [B, H, S] float32 the base-2 logarithm
-    of each row's sum (-inf behind a sequence's end), for ``attention_bwd``."""
+    """``attention`` without autograd: (out, saved), saved for ``attention_bwd``: (lse, low), lse
+    [B, H, S] float32 the base-2 logarithm of each row's sum (-inf behind a sequence's end),
+    low [B, S, H, D] uint8 what rounding took from out, in 254ths of its last place, plus 128."""
     return _attention_fwd(q, k, v, causal, scale, lengths, stream, True)
 
 
@@ -228,46 +229,55 @@ def _attention_fwd(q, k, v, causal, scale, lengths, stream, keep):
         (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
         out = torch.empty(B, S, H, D, dtype=q.dtype, device=q.device)
         lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device) if keep else None
-        args = _ATTENTION.pack(_ptr(q), _ptr(k), _ptr(v), _ptr(out), 0, 0, 0, 0, _ptr(lse), 0, 0, _ptr(lengths),
+        low = torch.empty(B, S, H, D, dtype=torch.uint8, device=q.device) if keep else None
+        args = _ATTENTION.pack(_ptr(q), _ptr(k), _ptr(v), _ptr(out), 0, 0, 0, 0, _ptr(lse), 0, 0, _ptr(low), _ptr(lengths),
                                *qs, *ks, *vs, S * H * D, H * D, D, *([0] * 12), B, S, H, Hk, D, code, int(causal), 1,
                                scale)
         if out.numel():
             _call("kgs_attention_fwd", args, q.device, stream)
-    return out, lse
+    return out, (lse, low) if keep else None
 
 
-def _dkv_splits(B: int, S: int, H: int, Hk: int) -> int:
+WIDE = (int(os.environ.get("W0", "0")), int(os.environ.get("W1", "0")))
+
+
+def _attention_wide(B: int, S: int, H: int, Hk: int) -> tuple[int, int]:
+    return WIDE
+
+
+def _dkv_splits(B: int, S: int, H: int, Hk: int, causal: bool) -> int:
     """Parts that the walk over query rows is cut into for dk and dv: with fewer workgroups
     (one per 128 keys and key head) than the chip holds at once, two per CU, it is cut, as
-    long as a part keeps 16 steps of 32 rows."""
+    long as a part keeps 16 steps of 32 rows.  Causal walks differ in length: twice as many
+    parts, so that the short ones fill up behind the long ones."""
     groups = max(1, B * Hk * -(-S // 128))
     steps = (H // Hk) * -(-S // 32)
-    return max(1, min(512 // groups, steps // 16, 8))
+    return max(1, min(-(-(1024 if causal else 512) // groups), steps // 16, 16))
 
 
-def attention_bwd(dout, q, k, v, out, lse, *, causal: bool = True, scale: float | None = None, lengths=None,
+def attention_bwd(dout, q, k, v, out, saved, *, causal: bool = True, scale: float | None = None, lengths=None,
                   stream=None):
-    """(dq, dk, dv) of ``attention`` from the gradient of its result, with ``out`` and ``lse``
+    """(dq, dk, dv) of ``attention`` from the gradient of its result, with ``out`` and ``saved``
     of ``attention_fwd`` and the same keywords; the probabilities are computed again."""
-    return _attention_bwd(dout, q, k, v, out, lse, causal, scale, lengths, stream, None)
+    return _attention_bwd(dout, q, k, v, out, *saved, causal, scale, lengths, stream, None)
 
 
-def _attention_bwd(dout, q, k, v, out, lse, causal, scale, lengths, stream, into):
+def _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, stream, into):
     import torch
 
-    B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths, dout=dout, out=out, lse=lse)
+    B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths, dout=dout, out=out, lse=lse, low=low)
     with _placed(q.device, stream):
         (q, qs), (k, ks), (v, vs), (out, os_), (dout, gs) = _heads(q), _heads(k), _heads(v), _heads(out), _heads(dout)
         if into is None:
             into = [torch.empty(B, S, n, D, dtype=q.dtype, device=q.device) for n in (H, Hk, Hk)]
-        splits = _dkv_splits(B, S, H, Hk)
+        splits = _dkv_splits(B, S, H, Hk, causal)
         # delta, then the parts of a split walk
         parts = splits * 2 * B * S * Hk * D if splits > 1 else 0
-        rows = (B * H * S + 3) // 4 * 4  # the parts are read 16 bytes at a time
+        rows = B * H * -(-S // 32) * 64
         work = torch.empty(rows + parts, dtype=torch.float32, device=q.device)
         st = [s for t in into for s in t.stride()[:3]]
         args = _ATTENTION.pack(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), *(_ptr(t) for t in into), _ptr(lse),
-                               _ptr(work), _ptr(work) + rows * 4 if parts else 0, _ptr(lengths), *qs, *ks, *vs, *os_,
+                               _ptr(work), _ptr(work) + rows * 4 if parts else 0, _ptr(low), _ptr(lengths), *qs, *ks, *vs, *os_,
                                *gs, *st, B, S, H, Hk, D, code, int(causal), splits, scale)
         if q.numel():
             _call("kgs_attention_bwd", args, q.device, stream)
@@ -290,16 +300,22 @@ def _matrix(t):
 
 
 def _swiglu_checks(x, w, **more):
+    import torch
+
     if x.dim() < 1 or w.dim() != 2:
         raise ValueError(f"x must be [..., width] and w [2 inner, width], not {tuple(x.shape)} and {tuple(w.shape)}")
     K, F = x.shape[-1], w.shape[0] // 2
     code = _type(x, "x", "bfloat16 or float16")
-    _same(x, "x", w=w, **more)
+    _same(x, "x", w=w, **{n: t for n, t in more.items() if n != "saved"})
     _shape(w, "w", (2 * F, K))
     if K == 0 or F == 0 or K % 8 or F % 8 or K > 1 << 20 or F > 1 << 20:
         raise ValueError(f"width and inner must be multiples of 8, at most {1 << 20}, not {K} and {F}")
     for name, t in more.items():
         _shape(t, name, (*x.shape[:-1], F if name == "dh" else 2 * F))
+    if "saved" in more:
+        saved = more["saved"]
+        if saved.dtype != torch.float32 or not saved.is_contiguous() or saved.device != x.device:
+            raise ValueError("saved must be the float32 tensor that swiglu_fwd returned")
     T = x.numel() // K
     if T >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} rows, not {T}")
@@ -325,8 +341,8 @@ def swiglu(x, w):
 
     x [..., width], w [2 inner, width] (the gate's rows first) of bfloat16 or float16, width
     and inner multiples of 8; any row strides with contiguous, 16-byte aligned rows are read
-    in place.  Returns [..., inner].  With a gradient wanted the two projections are kept,
-    rounded to the tensors' type, for the backward pass.
+    in place.  Returns [..., inner].  With a gradient wanted the two projections are kept
+    for the backward pass, in 32 bits.
     """
     import torch
 
@@ -336,7 +352,7 @@ def swiglu(x, w):
 
 
 def swiglu_fwd(x, w, *, stream=None):
-    """``swiglu`` without autograd: (h, saved), saved [..., 2 inner] for ``swiglu_bwd``."""
+    """``swiglu`` without autograd: (h, saved), saved [..., 2 inner] float32 for ``swiglu_bwd``."""
     return _swiglu_fwd(x, w, stream, True)
 
 
@@ -346,7 +362,7 @@ def _swiglu_fwd(x, w, stream, keep):
     T, K, F, code = _swiglu_checks(x, w)
     with _placed(x.device, stream):
         h = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
-        saved = torch.empty(*x.shape[:-1], 2 * F, dtype=x.dtype, device=x.device) if keep else None
+        saved = torch.empty(*x.shape[:-1], 2 * F, dtype=torch.float32, device=x.device) if keep else None
         if T:
             (x, x_ld), (w, w_ld) = _matrix(x), _matrix(w)
             tile, splits = _product_plan(T, 2 * F, K)
@@ -372,7 +388,6 @@ def _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, stream):
         dw = new(w.shape, dtype=x.dtype, device=x.device) if want_dw else None
         if T and (want_dx or want_dw):
             (x, x_ld), (w, w_ld), (dh, dh_ld) = _matrix(x), _matrix(w), _matrix(dh)
-            saved = saved.contiguous()
             if saved.data_ptr() % 16:
                 saved = saved.clone()
             tx, sx = _product_plan(T, K, 2 * F)
@@ -528,33 +543,33 @@ def _functions():
     class Attention(torch.autograd.Function):
         @staticmethod
         def forward(ctx, q, k, v, causal, scale, lengths):
-            out, lse = _attention_fwd(q, k, v, causal, scale, lengths, None, True)
-            ctx.save_for_backward(q, k, v, out, lse, lengths)
+            out, saved = _attention_fwd(q, k, v, causal, scale, lengths, None, True)
+            ctx.save_for_backward(q, k, v, out, *saved, lengths)
             ctx.options = causal, scale
             return out
 
         @staticmethod
         @once_differentiable
         def backward(ctx, dout):
-            q, k, v, out, lse, lengths = ctx.saved_tensors
-            grads = _attention_bwd(dout, q, k, v, out, lse, *ctx.options, lengths, None, None)
+            q, k, v, out, lse, low, lengths = ctx.saved_tensors
+            grads = _attention_bwd(dout, q, k, v, out, lse, low, *ctx.options, lengths, None, None)
             return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
 
     class AttentionQkv(torch.autograd.Function):
         @staticmethod
         def forward(ctx, qkv, heads, causal, scale, lengths):
-            out, lse = _attention_fwd(*_split_qkv(qkv, heads), causal, scale, lengths, None, True)
-            ctx.save_for_backward(qkv, out, lse, lengths)
+            out, saved = _attention_fwd(*_split_qkv(qkv, heads), causal, scale, lengths, None, True)
+            ctx.save_for_backward(qkv, out, *saved, lengths)
             ctx.options = heads, causal, scale
             return out
 
         @staticmethod
         @once_differentiable
         def backward(ctx, dout):
-            qkv, out, lse, lengths = ctx.saved_tensors
+            qkv, out, lse, low, lengths = ctx.saved_tensors
             heads, causal, scale = ctx.options
             grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-            _attention_bwd(dout, *_split_qkv(qkv, heads), out, lse, causal, scale, lengths, None,
+            _attention_bwd(dout, *_split_qkv(qkv, heads), out, lse, low, causal, scale, lengths, None,
                            _split_qkv(grad, heads))
             return grad, None, None, None, None
 

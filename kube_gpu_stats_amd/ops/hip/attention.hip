@@ -15,16 +15,22 @@
 //
 // Scores, statistics, sums and accumulators are 32 bits.  Rounded to the tensors' type:
 // p and ds, as operands of a matrix instruction (half a step each, independent from
-// term to term), and the outputs.
+// term to term), and the outputs.  The rounding of out would reach dq and dk through
+// delta (a third more error than theirs); so the forward pass that a backward follows
+// also keeps 8 bits of what it rounded off.
 #include "decoder.h"
 #include "decoder_common.h"
 
 namespace kgs {
 namespace {
 
-constexpr int kWaves = 4, kThreads = kWaves * kWave;
-constexpr int kRows = kWaves * 32;  // rows a workgroup holds
-constexpr int kStep = 64;           // keys a step of forward and dq
+// A workgroup holds 128 rows in four waves, and two share a CU.  One of 256 rows with four
+// or five steps under way instead of two was within 10 % either way (for forward and dq
+// best on few key heads, worse on many or short rows; for dk and dv always worse).
+constexpr int NW = 4, kThreads = NW * kWave, kRows = NW * 32;
+constexpr int NS = 2;       // slots of LDS: one step in work, one under way
+constexpr int kStep = 64;   // keys a step of forward and dq
+constexpr int kQStep = 32;  // rows a step of dk, dv
 
 __device__ __forceinline__ int length_of(const KgsAttention& a, int b) {
   if (!a.lengths) return a.S;
@@ -41,14 +47,15 @@ template <class T, int D> __device__ __forceinline__ int64_t span(int n, int s, 
   return n > s ? ((n - 1 - s) * stride + D) * static_cast<int64_t>(sizeof(T)) : 0;
 }
 
-// Stores a wave's accumulator (lane % 32 = row, registers = elements) times f to rows
-// of memory, the rows up to `rows` only.
+// Stores a wave's accumulator (lane % 32 = row, registers = elements) times f to rows of
+// memory, the rows up to `rows` only, by way of the wave's own 32 rows of LDS: as it lies
+// in the registers a store would write 8 bytes of each of 32 rows, from LDS it writes
+// whole rows.
 template <class T, int D>
-__device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float f, char* p, int64_t stride, int rows,
-                                           int lane) {
+__device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float f, char* lds, char* p, int64_t stride,
+                                           int rows, int lane) {
   using x4 = typename El<T>::x4;
-  if ((lane & 31) >= rows) return;
-  T* row = reinterpret_cast<T*>(p) + (lane & 31) * stride + (lane >> 5) * 4;
+  using Tl = Tile<D>;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
@@ -56,8 +63,53 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float f,
       x4 v;
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = static_cast<T>(acc[t][g * 4 + j] * f);
-      *reinterpret_cast<x4*>(row + t * 32 + g * 8) = v;
+      *reinterpret_cast<x4*>(lds + Tl::at(lane & 31, t * 4 + g) + (lane >> 5) * 8) = v;
     }
+  constexpr int kPer = 64 / (D / 8);  // rows a store
+#pragma unroll
+  for (int i = 0; i < 32 / kPer; ++i) {
+    const int row = i * kPer + lane / (D / 8), chunk = lane % (D / 8);
+    const i32x4 v = *reinterpret_cast<const i32x4*>(lds + Tl::at(row, chunk));
+    if (row < rows) *reinterpret_cast<i32x4*>(p + row * stride * 2 + chunk * 16) = v;
+  }
+}
+
+// The power of two below x, times 2^-7 or 2^-10: x's last place in T.  Tiny x: 0.
+template <class T> __device__ __forceinline__ float last_place(float x) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(int, x) & 0x7F800000) * (__is_same(T, bf16) ? 0x1p-7f : 0x1p-10f);
+}
+
+// What the rounding of acc f took, beside store_rows: 128 + 254 (acc f - rounded) / last
+// place, a byte each, 1 to 255 because half a last place is the most.  Where last_place
+// is 0, and for fp16 below its normal range, the byte is anything: it counts for less
+// than the smallest normal number's last place.
+template <class T, int D>
+__device__ __forceinline__ void store_low(const f32x16 (&acc)[D / 32], float f, char* lds, uint8_t* p, int64_t stride,
+                                          int rows, int lane) {
+  constexpr int kPer = 64 / (D / 16);
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint32_t q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = acc[t][g * 4 + j] * f, r = static_cast<float>(static_cast<T>(x));
+        // 1 / last place, by its exponent; 2^23 + 2^22 puts the rounded sum in the low bits
+        const float k = __builtin_bit_cast(
+            float, ((254 + (__is_same(T, bf16) ? 7 : 10)) << 23) - (__builtin_bit_cast(int, r) & 0x7F800000));
+        q[j] = __builtin_bit_cast(uint32_t, fmaf((x - r) * 254.f, k, 12582912.f + 128.f));
+      }
+      const uint32_t lo = __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0400), hi = __builtin_amdgcn_perm(q[3], q[2], 0x0C0C0400);
+      const int row = lane & 31, e = t * 32 + g * 8 + (lane >> 5) * 4;
+      *reinterpret_cast<uint32_t*>(lds + row * D + ((((e >> 4) ^ (row >> 1)) & (D / 16 - 1)) << 4) + (e & 15)) = lo | (hi << 16);
+    }
+#pragma unroll
+  for (int i = 0; i < 32 / kPer; ++i) {
+    const int row = i * kPer + lane / (D / 16), chunk = lane % (D / 16);
+    const i32x4 v = *reinterpret_cast<const i32x4*>(lds + row * D + (((chunk ^ (row >> 1)) & (D / 16 - 1)) << 4));
+    if (row < rows) *reinterpret_cast<i32x4*>(p + row * stride + chunk * 16) = v;
+  }
 }
 
 // Registers 8 h .. 8 h + 7 of an accumulator, rounded: the second operand of the product
@@ -77,14 +129,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
   using E = El<T>;
   using Tl = Tile<D>;
   constexpr int kTile = kStep * Tl::kRow;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];
+  __shared__ __attribute__((aligned(1024))) char smem[NS * 2 * kTile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.S + kRows - 1) / kRows;
-  const int64_t total = static_cast<int64_t>(tiles) * a.B * a.H;
-  const int64_t item = xcd_item(blockIdx.x, total);
-  if ((blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
-  const int tile = tiles - 1 - static_cast<int>(item % tiles);  // causal: the long rows first
-  const int bh = static_cast<int>(item / tiles), h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk);
+  int bh, rank;
+  if (!head_item(blockIdx.x, a.B * a.H, tiles, CAUSAL ? 16 : 1, bh, rank)) return;
+  const int tile = tiles - 1 - rank;  // causal: the long rows first
+  const int h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk);
   const int n = length_of(a, b);
   const int q0 = tile * kRows, qw = q0 + wave * 32, row = qw + (lane & 31);
 
@@ -100,28 +151,37 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
   const int last = CAUSAL ? min(qw + 32, n) : n;            // keys that any row of the wave sees
   const int steps = q0 < n ? (end + kStep - 1) / kStep : 0;
 
-  typename Tl::template Copy<kStep, kWaves> ck, cv;
+  // Steps NS - 1 ahead of the one in work are under way.  Past the last key the
+  // descriptors are empty: the copies count, so the wait is the same everywhere.
+  using Cp = typename Tl::template Copy<kStep, NW>;
+  Cp ck, cv;
   ck.init(wave, lane, a.k_st[1] * 2);
   cv.init(wave, lane, a.v_st[1] * 2);
   const uint32_t lds = lds_address(smem);
-  auto fetch = [&](int j) {
+  auto fetch = [&](int j, int slot) {
     const int s = j * kStep;
-    ck.go(buffer(at<T>(a.k, a.k_st, b, s, hk), span<T, D>(n, s, a.k_st[1])), lds + (j & 1) * 2 * kTile, wave);
-    cv.go(buffer(at<T>(a.v, a.v_st, b, s, hk), span<T, D>(n, s, a.v_st[1])), lds + (j & 1) * 2 * kTile + kTile, wave);
+    ck.go(buffer(at<T>(a.k, a.k_st, b, s, hk), span<T, D>(n, s, a.k_st[1])), lds + slot * 2 * kTile, wave);
+    cv.go(buffer(at<T>(a.v, a.v_st, b, s, hk), span<T, D>(n, s, a.v_st[1])), lds + slot * 2 * kTile + kTile, wave);
   };
 
   f32x16 o[D / 32] = {};
   float top = -INFINITY, sum = 0.f;
   const float c = a.scale * kLog2e;
-  if (steps > 0) fetch(0);
+  if (steps > 0) fetch(0, 0);
+  loads_done();
+  if (steps > 0)
+#pragma unroll
+    for (int j = 1; j < NS - 1; ++j) fetch(j, j);
+  int slot = 0;
   for (int j = 0; j < steps; ++j) {
-    copies_done();
-    barrier();  // step j has landed for every wave, and nobody reads the other buffer any more
-    if (j + 1 < steps) fetch(j + 1);
+    copies_left<(NS - 2) * 2 * Cp::kN>();
+    barrier();  // step j has landed for every wave, and nobody reads the slot before it any more
+    fetch(j + NS - 1, slot == 0 ? NS - 1 : slot - 1);
     const int s0 = j * kStep;
-    if (s0 >= last) continue;
-    const char* kt = smem + (j & 1) * 2 * kTile;
+    const char* kt = smem + slot * 2 * kTile;
     const char* vt = kt + kTile;
+    slot = slot == NS - 1 ? 0 : slot + 1;
+    if (s0 >= last) continue;
     f32x16 s[2] = {};
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk)
@@ -166,13 +226,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
           o[e] = E::mfma(Tl::template columns<T>(vt, t * 32 + hh * 16, e * 32, lane), p, o[e]);
       }
   }
+  copies_done();
+  barrier();  // the tiles are read; their place is used for the results' way out
+  char* const own = smem + wave * 32 * Tl::kRow;
   sum += other_half(sum);
   if (row >= n) sum = 0.f;
   const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // a NaN stays one
   if (row >= n)
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) o[t] = f32x16{};
-  store_rows<T, D>(o, inv, const_cast<char*>(at<T>(a.out, a.o_st, b, qw, h)), a.o_st[1], a.S - qw, lane);
+  store_rows<T, D>(o, inv, own, const_cast<char*>(at<T>(a.out, a.o_st, b, qw, h)), a.o_st[1], a.S - qw, lane);
+  if (a.low)
+    store_low<T, D>(o, inv, own, a.low + ((static_cast<int64_t>(b) * a.S + qw) * a.H + h) * D, static_cast<int64_t>(a.H) * D,
+                    a.S - qw, lane);
   if (a.lse && lane < 32 && row < a.S)
     a.lse[(static_cast<int64_t>(b) * a.H + h) * a.S + row] = row < n ? top + __builtin_amdgcn_logf(sum) : -INFINITY;
 }
@@ -183,14 +249,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   using E = El<T>;
   using Tl = Tile<D>;
   constexpr int kTile = kStep * Tl::kRow;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];
+  __shared__ __attribute__((aligned(1024))) char smem[NS * 2 * kTile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.S + kRows - 1) / kRows;
-  const int64_t total = static_cast<int64_t>(tiles) * a.B * a.H;
-  const int64_t item = xcd_item(blockIdx.x, total);
-  if ((blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
-  const int tile = tiles - 1 - static_cast<int>(item % tiles);
-  const int bh = static_cast<int>(item / tiles), h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk);
+  int bh, rank;
+  if (!head_item(blockIdx.x, a.B * a.H, tiles, CAUSAL ? 16 : 1, bh, rank)) return;
+  const int tile = tiles - 1 - rank;
+  const int h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk);
   const int n = length_of(a, b);
   const int q0 = tile * kRows, qw = q0 + wave * 32, row = qw + (lane & 31);
 
@@ -201,19 +266,31 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
     const i32x4 dg = buffer(at<T>(a.dout, a.g_st, b, qw, h), span<T, D>(n, qw, a.g_st[1]));
     const i32x4 dO = buffer(at<T>(a.out, a.o_st, b, qw, h), span<T, D>(n, qw, a.o_st[1]));
     const int r = lane & 31, cb = (lane >> 5) * 16;
+    const i32x4 dl = buffer(a.low + ((static_cast<int64_t>(b) * a.S + qw) * a.H + h) * D,
+                            n > qw ? (static_cast<int64_t>(n - 1 - qw) * a.H + 1) * D : 0);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       q[kk] = load16<typename E::x8>(dq, static_cast<int>(r * a.q_st[1] * 2) + kk * 32 + cb);
       g[kk] = load16<typename E::x8>(dg, static_cast<int>(r * a.g_st[1] * 2) + kk * 32 + cb);
       const typename E::x8 o = load16<typename E::x8>(dO, static_cast<int>(r * a.o_st[1] * 2) + kk * 32 + cb);
+      const u32x2 low = __builtin_bit_cast(
+          u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc(dl), r * a.H * D + kk * 16 + (lane >> 5) * 8, 0, 0));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta = fmaf(static_cast<float>(g[kk][j]), static_cast<float>(o[j]), delta);
+      for (int j = 0; j < 8; ++j) {
+        const float x = static_cast<float>(o[j]);
+        const float rest = static_cast<float>((low[j >> 2] >> (8 * (j & 3))) & 0xFF) - 128.f;
+        delta = fmaf(static_cast<float>(g[kk][j]), fmaf(rest, last_place<T>(x) * (1.f / 254.f), x), delta);
+      }
     }
     delta += other_half(delta);
   }
   const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.S + row;
-  if (lane < 32 && row < a.S) a.delta[stat] = delta;
   const float lse = row < n ? a.lse[stat] : 0.f;
+  // For dk, dv: the 32 rows' lse, then their delta, side by side.  Rows past the end get
+  // zeros: with zeros for q and do they are p = 1 times zero there.
+  const int groups = (a.S + 31) / 32, group = qw / 32;
+  if (group < groups)
+    a.delta[(static_cast<int64_t>(b * a.H + h) * groups + group) * 64 + lane] = lane < 32 ? lse : delta;
 
   const int end = CAUSAL ? min(n, q0 + kRows) : n;
   const int limit = CAUSAL ? min(row + 1, n) : n;
@@ -221,27 +298,36 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   const int last = CAUSAL ? min(qw + 32, n) : n;
   const int steps = q0 < n ? (end + kStep - 1) / kStep : 0;
 
-  typename Tl::template Copy<kStep, kWaves> ck, cv;
+  // Steps NS - 1 ahead of the one in work are under way.  Past the last key the
+  // descriptors are empty: the copies count, so the wait is the same everywhere.
+  using Cp = typename Tl::template Copy<kStep, NW>;
+  Cp ck, cv;
   ck.init(wave, lane, a.k_st[1] * 2);
   cv.init(wave, lane, a.v_st[1] * 2);
   const uint32_t lds = lds_address(smem);
-  auto fetch = [&](int j) {
+  auto fetch = [&](int j, int slot) {
     const int s = j * kStep;
-    ck.go(buffer(at<T>(a.k, a.k_st, b, s, hk), span<T, D>(n, s, a.k_st[1])), lds + (j & 1) * 2 * kTile, wave);
-    cv.go(buffer(at<T>(a.v, a.v_st, b, s, hk), span<T, D>(n, s, a.v_st[1])), lds + (j & 1) * 2 * kTile + kTile, wave);
+    ck.go(buffer(at<T>(a.k, a.k_st, b, s, hk), span<T, D>(n, s, a.k_st[1])), lds + slot * 2 * kTile, wave);
+    cv.go(buffer(at<T>(a.v, a.v_st, b, s, hk), span<T, D>(n, s, a.v_st[1])), lds + slot * 2 * kTile + kTile, wave);
   };
 
   f32x16 acc[D / 32] = {};
   const float c = a.scale * kLog2e;
-  if (steps > 0) fetch(0);
+  if (steps > 0) fetch(0, 0);
+  loads_done();
+  if (steps > 0)
+#pragma unroll
+    for (int j = 1; j < NS - 1; ++j) fetch(j, j);
+  int slot = 0;
   for (int j = 0; j < steps; ++j) {
-    copies_done();
+    copies_left<(NS - 2) * 2 * Cp::kN>();
     barrier();
-    if (j + 1 < steps) fetch(j + 1);
+    fetch(j + NS - 1, slot == 0 ? NS - 1 : slot - 1);
     const int s0 = j * kStep;
-    if (s0 >= last) continue;
-    const char* kt = smem + (j & 1) * 2 * kTile;
+    const char* kt = smem + slot * 2 * kTile;
     const char* vt = kt + kTile;
+    slot = slot == NS - 1 ? 0 : slot + 1;
+    if (s0 >= last) continue;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       f32x16 s = {}, dp = {};
@@ -271,10 +357,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
       }
     }
   }
+  copies_done();
+  barrier();
   if (row >= n)
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) acc[t] = f32x16{};
-  store_rows<T, D>(acc, a.scale, const_cast<char*>(at<T>(a.dq, a.dq_st, b, qw, h)), a.dq_st[1], a.S - qw, lane);
+  store_rows<T, D>(acc, a.scale, smem + wave * 32 * Tl::kRow, const_cast<char*>(at<T>(a.dq, a.dq_st, b, qw, h)), a.dq_st[1], a.S - qw, lane);
 }
 
 // dk and dv of 128 keys a workgroup: walks the query heads that share the key head, and
@@ -287,24 +375,21 @@ template <class T, int D, bool CAUSAL>
 __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention a) {
   using E = El<T>;
   using Tl = Tile<D>;
-  constexpr int kQ = 32, kTile = kQ * Tl::kRow, kV = kRows * Tl::kRow, kStage = 2 * kTile + 2 * 256;
-  __shared__ __attribute__((aligned(1024))) char smem[kV + 2 * kStage];
+  constexpr int kQ = kQStep, kTile = kQ * Tl::kRow, kV = kRows * Tl::kRow, kStage = 2 * kTile + 256;
+  __shared__ __attribute__((aligned(1024))) char smem[kV + NS * kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.S + kRows - 1) / kRows;
-  const int64_t total = static_cast<int64_t>(tiles) * a.B * a.Hk * a.splits;
-  const int64_t item = xcd_item(blockIdx.x, total);
-  if ((blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
-  const int split = static_cast<int>(item % a.splits);
-  const int64_t rest = item / a.splits;
-  const int tile = static_cast<int>(rest % tiles);  // causal: the first keys have the most rows
-  const int bh = static_cast<int>(rest / tiles), hk = bh % a.Hk, b = bh / a.Hk, G = a.H / a.Hk;
+  int bh, rank;
+  if (!head_item(blockIdx.x, a.B * a.Hk, tiles * a.splits, CAUSAL ? 16 : 1, bh, rank)) return;
+  const int split = rank % a.splits, tile = rank / a.splits;  // causal: the first keys have the most rows
+  const int hk = bh % a.Hk, b = bh / a.Hk, G = a.H / a.Hk;
   const int n = length_of(a, b);
   const int k0 = tile * kRows, kw = k0 + wave * 32, key = kw + (lane & 31);
 
   // v's tile; rows past the end are zero
   const uint32_t lds = lds_address(smem);
   {
-    typename Tl::template Copy<kRows, kWaves> cv;
+    typename Tl::template Copy<kRows, NW> cv;
     cv.init(wave, lane, a.v_st[1] * 2);
     cv.go(buffer(at<T>(a.v, a.v_st, b, k0, hk), span<T, D>(n, k0, a.v_st[1])), lds, wave);
   }
@@ -320,48 +405,56 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
   const int lo = static_cast<int>(static_cast<int64_t>(all) * split / a.splits);
   const int hi = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / a.splits);
 
-  typename Tl::template Copy<kQ, kWaves> cq, cg;
+  using Cp = typename Tl::template Copy<kQ, NW>;
+  Cp cq, cg;
   cq.init(wave, lane, a.q_st[1] * 2);
   cg.init(wave, lane, a.g_st[1] * 2);
-  // the walk's step that is fetched next: head of the group, step of that head
-  int fh = hi > lo ? lo / each : 0, fs = hi > lo ? lo % each : 0;
-  auto fetch = [&](int buf) {
-    const int h = hk * G + fh, s = (first + fs) * kQ;
-    const uint32_t to = lds + kV + buf * kStage;
-    cq.go(buffer(at<T>(a.q, a.q_st, b, s, h), span<T, D>(n, s, a.q_st[1])), to, wave);
-    cg.go(buffer(at<T>(a.dout, a.g_st, b, s, h), span<T, D>(n, s, a.g_st[1])), to + kTile, wave);
-    if (wave < 2) {  // lse or delta of the 32 rows (and of 32 more)
-      const float* p = (wave ? a.delta : a.lse) + (static_cast<int64_t>(b) * a.H + h) * a.S + s;
-      copy4(buffer(p, static_cast<int64_t>(n - s) * 4), lane * 4, to + 2 * kTile + wave * 256);
-    }
+  // The walk's step that is fetched next: head of the group, step of that head.  Past the
+  // end of the walk the descriptors are empty, as in the forward pass.
+  int fh = hi > lo ? lo / each : 0, fs = hi > lo ? lo % each : 0, fi = lo;
+  const int groups = (a.S + 31) / 32;
+  auto fetch = [&](int slot) {
+    const int h = hk * G + fh, s = (first + fs) * kQ, end = fi < hi ? n : 0;
+    const uint32_t to = lds + kV + slot * kStage;
+    cq.go(buffer(at<T>(a.q, a.q_st, b, s, h), span<T, D>(end, s, a.q_st[1])), to, wave);
+    cg.go(buffer(at<T>(a.dout, a.g_st, b, s, h), span<T, D>(end, s, a.g_st[1])), to + kTile, wave);
+    if (wave == 0)  // lse and delta of the rows
+      copy4(buffer(a.delta + (static_cast<int64_t>(b * a.H + h) * groups + first + fs) * 64, end ? 256 : 0), lane * 4,
+            to + 2 * kTile);
+    ++fi;
     if (++fs == each) fs = 0, ++fh;
   };
 
   f32x16 dka[D / 32] = {}, dva[D / 32] = {};
   const float c = a.scale * kLog2e;
-  int buf = 1;
   if (lo < hi) fetch(0);
+  loads_done();
+  if (lo < hi)
+#pragma unroll
+    for (int j = 1; j < NS - 1; ++j) fetch(j);
+  int slot = 0, ss = hi > lo ? lo % each : 0;
   for (int i = lo; i < hi; ++i) {
-    buf ^= 1;
-    const int s0 = (first + (fs ? fs : each) - 1) * kQ;  // the step fetched last
-    copies_done();
+    if (wave == 0) copies_left<(NS - 2) * (2 * Cp::kN + 1)>();
+    else copies_left<(NS - 2) * 2 * Cp::kN>();
     barrier();
-    if (i + 1 < hi) fetch(buf ^ 1);
-    if (CAUSAL && s0 + kQ <= kw) continue;  // no row of the step sees the wave's keys
-    const char* qt = smem + kV + buf * kStage;
+    fetch(slot == 0 ? NS - 1 : slot - 1);
+    const int s0 = (first + ss) * kQ;
+    const char* qt = smem + kV + slot * kStage;
     const char* gt = qt + kTile;
     const float* lse = reinterpret_cast<const float*>(gt + kTile);
+    slot = slot == NS - 1 ? 0 : slot + 1;
+    if (++ss == each) ss = 0;
+    if (CAUSAL && s0 + kQ <= kw) continue;  // no row of the step sees the wave's keys
     f32x16 s = {}, dp = {};
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       s = E::mfma(Tl::template rows<T>(qt, 0, kk, lane), k[kk], s);
       dp = E::mfma(Tl::template rows<T>(gt, 0, kk, lane), Tl::template rows<T>(smem, wave * 32, kk, lane), dp);
     }
-    // Rows past the end hold zeros for q, do, lse and delta: p = 1 there, times zero.
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
       const f32x4 l = *reinterpret_cast<const f32x4*>(lse + m * 8 + (lane >> 5) * 4);
-      const f32x4 d = *reinterpret_cast<const f32x4*>(lse + 64 + m * 8 + (lane >> 5) * 4);
+      const f32x4 d = *reinterpret_cast<const f32x4*>(lse + 32 + m * 8 + (lane >> 5) * 4);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = m * 4 + j;
@@ -384,7 +477,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
       }
     }
   }
-  copies_done();  // v's tile, if the walk was empty
+  copies_done();
   if (a.splits > 1) {
     if (key < a.S) {
       const int64_t part = static_cast<int64_t>(a.B) * a.S * a.Hk * D;
@@ -406,8 +499,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
   if (key >= n)
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) dka[t] = dva[t] = f32x16{};
-  store_rows<T, D>(dka, a.scale, const_cast<char*>(at<T>(a.dk, a.dk_st, b, kw, hk)), a.dk_st[1], a.S - kw, lane);
-  store_rows<T, D>(dva, 1.f, const_cast<char*>(at<T>(a.dv, a.dv_st, b, kw, hk)), a.dv_st[1], a.S - kw, lane);
+  char* const own = smem + wave * 32 * Tl::kRow;  // the wave's rows of v, which no other reads
+  store_rows<T, D>(dka, a.scale, own, const_cast<char*>(at<T>(a.dk, a.dk_st, b, kw, hk)), a.dk_st[1], a.S - kw, lane);
+  store_rows<T, D>(dva, 1.f, own, const_cast<char*>(at<T>(a.dv, a.dv_st, b, kw, hk)), a.dv_st[1], a.S - kw, lane);
 }
 
 // Adds the parts of a split walk, in their order: 4 elements a thread of dk, then of dv.
@@ -437,34 +531,35 @@ int check(const KgsAttention* a, bool backward) {
   if (a->B < 0 || a->S < 0 || a->H <= 0 || a->Hk <= 0 || a->H % a->Hk) return fail(w, "bad sizes");
   if (a->D != 64 && a->D != 128) return fail(w, "head dimension must be 64 or 128");
   if (a->type != 0 && a->type != 1) return fail(w, "type must be bfloat16 or float16");
-  if (backward && (!a->dout || !a->lse || !a->delta || !a->dq || !a->dk || !a->dv)) return fail(w, "a tensor is missing");
+  if (backward && (!a->dout || !a->lse || !a->low || !a->delta || !a->dq || !a->dk || !a->dv)) return fail(w, "a tensor is missing");
   if (backward && (a->splits < 1 || (a->splits > 1 && !a->partial))) return fail(w, "bad split");
   const int64_t* st[] = {a->q_st, a->k_st, a->v_st, a->o_st, a->g_st, a->dq_st, a->dk_st, a->dv_st};
   for (int i = 0; i < (backward ? 8 : 4); ++i)
     for (int j = 0; j < 3; ++j)
       // rows behind the last lie past the descriptor's end; offsets inside a tile stay under 2^30
       if (st[i][j] < 0 || st[i][j] % 8 || (j == 1 && (st[i][j] < a->D || st[i][j] > (1 << 22)))) return fail(w, "unsupported strides");
-  const int64_t tiles = (a->S + kRows - 1) / kRows;
-  if (tiles * a->B * a->H * (backward ? a->splits : 1) > 0x7FFFFF00ll) return fail(w, "too many workgroups");
+  if (a->H > (1 << 18)) return fail(w, "too many heads");  // offsets inside a tile of low
+  // workgroups, and the products of counts that head_item forms, stay under 2^31
+  const int64_t tiles = (a->S + 127) / 128;
+  if ((tiles + 16) * (static_cast<int64_t>(a->B) * a->H + 16) * (backward ? a->splits : 1) * 16 > 0x7FFFFFFFll)
+    return fail(w, "too many workgroups");
   return 0;
 }
 
-unsigned grid(int64_t total) { return static_cast<unsigned>((total + 7) / 8 * 8); }
-
 template <class T, int D, bool CAUSAL> int forward(const KgsAttention& a, hipStream_t s) {
   const int64_t tiles = (a.S + kRows - 1) / kRows;
-  attention_fwd_kernel<T, D, CAUSAL><<<grid(tiles * a.B * a.H), kThreads, 0, s>>>(a);
+  attention_fwd_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(a.B * static_cast<int64_t>(a.H), tiles)), kThreads, 0, s>>>(a);
   return launched("attention forward");
 }
 
 template <class T, int D, bool CAUSAL> int backward(const KgsAttention& a, hipStream_t s) {
-  const int64_t tiles = (a.S + kRows - 1) / kRows;
-  attention_dq_kernel<T, D, CAUSAL><<<grid(tiles * a.B * a.H), kThreads, 0, s>>>(a);
+  const int64_t tiles = (a.S + kRows - 1) / kRows, b = a.B;
+  attention_dq_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(b * a.H, tiles)), kThreads, 0, s>>>(a);
   if (launched("attention dq")) return -1;
-  attention_dkv_kernel<T, D, CAUSAL><<<grid(tiles * a.B * a.Hk * a.splits), kThreads, 0, s>>>(a);
+  attention_dkv_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(b * a.Hk, tiles * a.splits)), kThreads, 0, s>>>(a);
   if (launched("attention dk, dv")) return -1;
   if (a.splits > 1) {
-    const int64_t n = 2 * static_cast<int64_t>(a.B) * a.S * a.Hk * D / 4;
+    const int64_t n = 2 * b * a.S * a.Hk * D / 4;
     attention_join_kernel<T, D><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(a);
     return launched("attention join");
   }

@@ -7,20 +7,24 @@
 extern "C" {
 
 // Tensors [B, S, heads, D]; strides in elements of (B, S, heads), D contiguous; pointers
-// 16-byte aligned, strides multiples of 8.  lse, delta: float [B, H, S].
+// 16-byte aligned, strides multiples of 8.  lse: float [B, H, S],
+// delta: float [B, H, ceil(S / 32), 2, 32] (workspace).  low: [B, S, H, D], what rounding
+// took from out, in 254ths of its last place, plus 128.  The forward pass writes lse and low if they
+// are not null.
 struct KgsAttention {
   const void *q, *k, *v;
   void* out;
   const void* dout;
   void *dq, *dk, *dv;
   float *lse, *delta, *partial;  // partial: float [splits, 2, B, S, Hk, D]
+  uint8_t* low;
   const int32_t* lengths;        // [B] or null
   int64_t q_st[3], k_st[3], v_st[3], o_st[3], g_st[3], dq_st[3], dk_st[3], dv_st[3];
   int32_t B, S, H, Hk, D, type, causal, splits;  // type: 0 bfloat16, 1 float16
   float scale;
 };
 
-// x [T, K] and w [2F, K] with row strides, h [T, F], saved [T, 2F] (null: not kept), dh [T, F]
+// x [T, K] and w [2F, K] with row strides, h [T, F], saved float [T, 2F] (null: not kept), dh [T, F]
 // with a row stride, dgu [T, 2F], dx [T, K], dw [2F, K] (either null: not wanted).  Pointers
 // 16-byte aligned; K, F and strides multiples of 8.  tile, splits: of the forward product,
 // of dx and of dw.  partial: float [splits, rows, columns] of the largest split product.

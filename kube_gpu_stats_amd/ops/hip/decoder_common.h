@@ -96,7 +96,12 @@ __device__ __forceinline__ void copy4(i32x4 d, int voff, uint32_t lds) {
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(d)
                : "memory");
 }
-__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits until at most N of the wave's copies are under way.
+template <int N> __device__ __forceinline__ void copies_left() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_done() { copies_left<0>(); }
+// The same wait in a form the compiler knows: what it loaded before is there, and it puts
+// no wait of its own for that into the loop that follows.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }
 
 __device__ __forceinline__ void barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -166,6 +171,33 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 
 __device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t total) {
   const int64_t per = (total + 7) / 8;
   return (id & 7) * per + (id >> 3);
+}
+
+// The same for `heads` heads of `ranks` pieces each, the longest piece first (rank 0).
+// An XCD takes whole heads: their pieces read the same keys.  It goes through `group`
+// heads at a time rank by rank: where pieces differ in length (causal) the short ones of
+// 16 heads fill up the end (forward of 4 x 32 heads, 2048 positions: 192 us, 208 us head
+// by head); where they do not, head by head keeps fewer keys in the L2 in use (280 us,
+// 297 us by 16).  The heads that are left when 8 do not divide them are dealt to the
+// XCDs piece by piece, so that none has more than its share.
+__host__ __device__ __forceinline__ int64_t head_items(int64_t heads, int64_t ranks) {
+  return 8 * ((heads % 8 * ranks + 7) / 8 + heads / 8 * ranks);
+}
+__device__ __forceinline__ bool head_item(int id, int heads, int ranks, int group, int& head, int& rank) {
+  const int x = id & 7, left = heads & 7, own = heads >> 3, dealt = (left * ranks + 7) / 8;
+  int k = id >> 3;
+  if (k < dealt) {
+    const int i = k * 8 + x;
+    if (i >= left * ranks) return false;
+    rank = i / left;
+    head = heads - left + i % left;
+    return true;
+  }
+  k -= dealt;
+  const int g = k / (group * ranks), size = min(group, own - g * group), in = k - g * group * ranks;
+  rank = in / size;
+  head = x * own + g * group + in % size;
+  return true;
 }
 
 // Error text of the calling thread's last failed entry, and its setter.

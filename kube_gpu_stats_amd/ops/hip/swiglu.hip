@@ -11,9 +11,10 @@
 //
 // Tiles of both operands go from memory straight to LDS, two steps of 64 of the summed
 // index deep, as they lie in memory; an operand whose summed index is not the
-// contiguous one is transposed by the LDS read.  Accumulators are 32 bits.  Rounded to
-// the tensors' type: g and u as saved (the forward's own h uses them unrounded), dg and
-// du as operands of the two products, and the outputs.
+// contiguous one is transposed by the LDS read.  Accumulators are 32 bits, and so are g
+// and u as saved: rounded to 16 bits they would add as much error to dx and dw as the
+// rounding of dg and du, operands of the two products, which is not to be avoided.
+// Rounded besides those: the outputs.
 #include "decoder.h"
 #include "decoder_common.h"
 
@@ -25,7 +26,8 @@ constexpr int kK = 64;  // summed index a step
 struct Product {
   const void *a, *b;   // a: [M, K] or, transposed, [K, M]; b: [N, K] or, transposed, [K, N]
   int64_t a_ld, b_ld;  // elements
-  void *c, *saved;     // c [M, N] contiguous (pairs: [M, N / 2]); saved [M, N] or null
+  void* c;             // [M, N] contiguous (pairs: [M, N / 2])
+  float *saved;        // [M, N] or null
   float* partial;      // splits > 1: [splits, M, N]
   int M, N, K, splits;
 };
@@ -165,19 +167,19 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_kernel(Product p) {
           *reinterpret_cast<f32x4*>(to) = x;
           if (PAIR) *reinterpret_cast<f32x4*>(to + N) = y;
         } else if (PAIR) {
-          typename E::x4 h, x, y;
+          typename E::x4 h;
+          f32x4 x, y;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float gate = acc[i][k][g * 4 + j], up = acc[i][(NT / 2 + k) % NT][g * 4 + j];
-            h[j] = static_cast<T>(gate * sigmoid(gate) * up);
-            x[j] = static_cast<T>(gate);
-            y[j] = static_cast<T>(up);
+            x[j] = acc[i][k][g * 4 + j];
+            y[j] = acc[i][(NT / 2 + k) % NT][g * 4 + j];
+            h[j] = static_cast<T>(x[j] * sigmoid(x[j]) * y[j]);
           }
           *reinterpret_cast<typename E::x4*>(static_cast<T*>(p.c) + static_cast<int64_t>(m) * N + n) = h;
           if (p.saved) {
-            T* to = static_cast<T*>(p.saved) + static_cast<int64_t>(m) * p.N + n;
-            *reinterpret_cast<typename E::x4*>(to) = x;
-            *reinterpret_cast<typename E::x4*>(to + N) = y;
+            float* to = p.saved + static_cast<int64_t>(m) * p.N + n;
+            *reinterpret_cast<f32x4*>(to) = x;
+            *reinterpret_cast<f32x4*>(to + N) = y;
           }
         } else {
           typename E::x4 x;
@@ -202,40 +204,36 @@ template <class T, bool PAIR> __global__ __launch_bounds__(256) void join_kernel
     x += *reinterpret_cast<const f32x4*>(from + s * part);
     if (PAIR) y += *reinterpret_cast<const f32x4*>(from + s * part + N);
   }
-  x4 h, g, u;
+  x4 h;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    h[j] = static_cast<T>(PAIR ? x[j] * sigmoid(x[j]) * y[j] : x[j]);
-    g[j] = static_cast<T>(x[j]);
-    u[j] = static_cast<T>(y[j]);
-  }
+  for (int j = 0; j < 4; ++j) h[j] = static_cast<T>(PAIR ? x[j] * sigmoid(x[j]) * y[j] : x[j]);
   *reinterpret_cast<x4*>(static_cast<T*>(p.c) + i) = h;
   if (PAIR && p.saved) {
-    T* to = static_cast<T*>(p.saved) + m * p.N + n;
-    *reinterpret_cast<x4*>(to) = g;
-    *reinterpret_cast<x4*>(to + N) = u;
+    float* to = p.saved + m * p.N + n;
+    *reinterpret_cast<f32x4*>(to) = x;
+    *reinterpret_cast<f32x4*>(to + N) = y;
   }
 }
 
-// [dg du] from dh and the saved [g u], 8 columns a thread.
-template <class T> __global__ __launch_bounds__(256) void gate_bwd_kernel(const T* dh, int64_t dh_ld, const T* saved, T* d,
-                                                                         int M, int F) {
-  using x8 = typename El<T>::x8;
-  const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 8;
+// [dg du] from dh and the saved [g u], 4 columns a thread.
+template <class T> __global__ __launch_bounds__(256) void gate_bwd_kernel(const T* dh, int64_t dh_ld, const float* saved,
+                                                                         T* d, int M, int F) {
+  using x4 = typename El<T>::x4;
+  const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4;
   if (i >= static_cast<int64_t>(M) * F) return;
   const int64_t m = i / F, n = i % F;
-  const x8 a = *reinterpret_cast<const x8*>(dh + m * dh_ld + n);
-  const x8 g = *reinterpret_cast<const x8*>(saved + m * 2 * F + n);
-  const x8 u = *reinterpret_cast<const x8*>(saved + m * 2 * F + F + n);
-  x8 dg, du;
+  const x4 a = *reinterpret_cast<const x4*>(dh + m * dh_ld + n);
+  const f32x4 g = *reinterpret_cast<const f32x4*>(saved + m * 2 * F + n);
+  const f32x4 u = *reinterpret_cast<const f32x4*>(saved + m * 2 * F + F + n);
+  x4 dg, du;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float gate = static_cast<float>(g[j]), grad = static_cast<float>(a[j]), s = sigmoid(gate);
-    dg[j] = static_cast<T>(grad * static_cast<float>(u[j]) * s * (1.f + gate * (1.f - s)));
-    du[j] = static_cast<T>(grad * gate * s);
+  for (int j = 0; j < 4; ++j) {
+    const float grad = static_cast<float>(a[j]), s = sigmoid(g[j]);
+    dg[j] = static_cast<T>(grad * u[j] * s * (1.f + g[j] * (1.f - s)));
+    du[j] = static_cast<T>(grad * g[j] * s);
   }
-  *reinterpret_cast<x8*>(d + m * 2 * F + n) = dg;
-  *reinterpret_cast<x8*>(d + m * 2 * F + F + n) = du;
+  *reinterpret_cast<x4*>(d + m * 2 * F + n) = dg;
+  *reinterpret_cast<x4*>(d + m * 2 * F + F + n) = du;
 }
 
 template <class T, int BM, int BN, int WM, int WN, bool TA, bool TB, bool PAIR>
@@ -269,14 +267,14 @@ template <class T, bool TA, bool TB, bool PAIR> int product(const Product& p, in
 }
 
 template <class T> int forward(const KgsSwiglu& a, hipStream_t s) {
-  const Product p{a.x, a.w, a.x_ld, a.w_ld, a.h, a.saved, a.partial, a.T, 2 * a.F, a.K, a.splits[0]};
+  const Product p{a.x, a.w, a.x_ld, a.w_ld, a.h, static_cast<float*>(a.saved), a.partial, a.T, 2 * a.F, a.K, a.splits[0]};
   return product<T, false, false, true>(p, a.tile[0], s);
 }
 
 template <class T> int backward(const KgsSwiglu& a, hipStream_t s) {
-  const int64_t n = static_cast<int64_t>(a.T) * a.F / 8;
+  const int64_t n = static_cast<int64_t>(a.T) * a.F / 4;
   gate_bwd_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(
-      static_cast<const T*>(a.dh), a.dh_ld, static_cast<const T*>(a.saved), static_cast<T*>(a.dgu), a.T, a.F);
+      static_cast<const T*>(a.dh), a.dh_ld, static_cast<const float*>(a.saved), static_cast<T*>(a.dgu), a.T, a.F);
   if (launched("swiglu gate backward")) return -1;
   if (a.dx) {
     const Product p{a.dgu, a.w, 2ll * a.F, a.w_ld, a.dx, nullptr, a.partial, a.T, a.K, 2 * a.F, a.splits[1]};
