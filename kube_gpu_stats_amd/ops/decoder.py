@@ -311,11 +311,11 @@ def _swiglu_checks(x, w, **more):
     if K == 0 or F == 0 or K % 8 or F % 8 or K > 1 << 20 or F > 1 << 20:
         raise ValueError(f"width and inner must be multiples of 8, at most {1 << 20}, not {K} and {F}")
     for name, t in more.items():
-        _shape(t, name, (*x.shape[:-1], F if name == "dh" else 2 * F))
+        _shape(t, name, (*x.shape[:-1], F if name == "dh" else 6 * F))
     if "saved" in more:
         saved = more["saved"]
-        if saved.dtype != torch.float32 or not saved.is_contiguous() or saved.device != x.device:
-            raise ValueError("saved must be the float32 tensor that swiglu_fwd returned")
+        if saved.dtype != torch.uint8 or not saved.is_contiguous() or saved.device != x.device:
+            raise ValueError("saved must be the uint8 tensor that swiglu_fwd returned")
     T = x.numel() // K
     if T >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} rows, not {T}")
@@ -342,7 +342,7 @@ def swiglu(x, w):
     x [..., width], w [2 inner, width] (the gate's rows first) of bfloat16 or float16, width
     and inner multiples of 8; any row strides with contiguous, 16-byte aligned rows are read
     in place.  Returns [..., inner].  With a gradient wanted the two projections are kept
-    for the backward pass, in 32 bits.
+    for the backward pass, 24 bits of each value.
     """
     import torch
 
@@ -352,7 +352,8 @@ def swiglu(x, w):
 
 
 def swiglu_fwd(x, w, *, stream=None):
-    """``swiglu`` without autograd: (h, saved), saved [..., 2 inner] float32 for ``swiglu_bwd``."""
+    """``swiglu`` without autograd: (h, saved), saved [..., 6 inner] uint8 for ``swiglu_bwd``: of
+    each row the upper 16 bits of the two projections, then the 8 bits below."""
     return _swiglu_fwd(x, w, stream, True)
 
 
@@ -362,7 +363,7 @@ def _swiglu_fwd(x, w, stream, keep):
     T, K, F, code = _swiglu_checks(x, w)
     with _placed(x.device, stream):
         h = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
-        saved = torch.empty(*x.shape[:-1], 2 * F, dtype=torch.float32, device=x.device) if keep else None
+        saved = torch.empty(*x.shape[:-1], 6 * F, dtype=torch.uint8, device=x.device) if keep else None
         if T:
             (x, x_ld), (w, w_ld) = _matrix(x), _matrix(w)
             tile, splits = _product_plan(T, 2 * F, K)

@@ -24,7 +24,7 @@ struct KgsAttention {
   float scale;
 };
 
-// x [T, K] and w [2F, K] with row strides, h [T, F], saved float [T, 2F] (null: not kept), dh [T, F]
+// x [T, K] and w [2F, K] with row strides, h [T, F], saved [T, 6F] bytes (null: not kept), dh [T, F]
 // with a row stride, dgu [T, 2F], dx [T, K], dw [2F, K] (either null: not wanted).  Pointers
 // 16-byte aligned; K, F and strides multiples of 8.  tile, splits: of the forward product,
 // of dx and of dw.  partial: float [splits, rows, columns] of the largest split product.

@@ -11,10 +11,10 @@
 //
 // Tiles of both operands go from memory straight to LDS, two steps of 64 of the summed
 // index deep, as they lie in memory; an operand whose summed index is not the
-// contiguous one is transposed by the LDS read.  Accumulators are 32 bits, and so are g
-// and u as saved: rounded to 16 bits they would add as much error to dx and dw as the
-// rounding of dg and du, operands of the two products, which is not to be avoided.
-// Rounded besides those: the outputs.
+// contiguous one is transposed by the LDS read.  Accumulators are 32 bits; g and u are
+// saved with 24 of them: rounded to 16 they would add as much error to dx and dw as the
+// rounding of dg and du, operands of the two products, which is not to be avoided, and
+// 32 cost a third more traffic.  Rounded besides those: the outputs.
 #include "decoder.h"
 #include "decoder_common.h"
 
@@ -27,7 +27,7 @@ struct Product {
   const void *a, *b;   // a: [M, K] or, transposed, [K, M]; b: [N, K] or, transposed, [K, N]
   int64_t a_ld, b_ld;  // elements
   void* c;             // [M, N] contiguous (pairs: [M, N / 2])
-  float *saved;        // [M, N] or null
+  uint8_t* saved;      // [M, 3 N] (Saved) or null
   float* partial;      // splits > 1: [splits, M, N]
   int M, N, K, splits;
 };
@@ -81,8 +81,51 @@ template <class T, int ROWS, int NW> struct Operand<T, ROWS, true, NW> {
   }
 };
 
+// A row of n saved values: their upper 16 bits, then the 8 below, rounded.
+struct Saved {
+  uint8_t* row;
+  int n;
+  __device__ __forceinline__ Saved(uint8_t* base, int64_t m, int n) : row(base + m * 3 * n), n(n) {}
+  __device__ __forceinline__ uint16_t* high(int i) const { return reinterpret_cast<uint16_t*>(row) + i; }
+  __device__ __forceinline__ uint8_t* low(int i) const { return row + 2 * static_cast<int64_t>(n) + i; }
+  // 4 values from i, a multiple of 4
+  __device__ __forceinline__ f32x4 load(int i) const {
+    const u32x2 h = *reinterpret_cast<const u32x2*>(high(i));
+    const uint32_t l = *reinterpret_cast<const uint32_t*>(low(i));
+    f32x4 x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x[j] = __builtin_bit_cast(float, ((h[j >> 1] >> (16 * (j & 1))) << 16) | (((l >> (8 * j)) & 0xFF) << 8));
+    return x;
+  }
+  static __device__ __forceinline__ void split(f32x4 x, u32x2& h, uint32_t& l) {
+    uint32_t b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float e = x[j];  // (of an element itself, bit_cast takes the first)
+      const uint32_t v = __builtin_bit_cast(uint32_t, e);
+      // half a step up; not across the exponent of infinities and NaNs, whose payload stays above
+      b[j] = (v & 0x7F800000u) == 0x7F800000u ? v : v + 0x80u;
+    }
+    h[0] = __builtin_amdgcn_perm(b[1], b[0], 0x07060302);
+    h[1] = __builtin_amdgcn_perm(b[3], b[2], 0x07060302);
+    l = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0501) | (__builtin_amdgcn_perm(b[3], b[2], 0x0C0C0501) << 16);
+  }
+  __device__ __forceinline__ void store(int i, f32x4 x) const {
+    u32x2 h;
+    uint32_t l;
+    split(x, h, l);
+    *reinterpret_cast<u32x2*>(high(i)) = h;
+    *reinterpret_cast<uint32_t*>(low(i)) = l;
+  }
+};
+
 // silu(g) = g / (1 + 2^(-g log2 e)): an overflowing power makes the quotient 0.
 __device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + __builtin_amdgcn_exp2f(-g * kLog2e)); }
+
+__device__ __forceinline__ f32x4 quarter(const f32x16& x, int g) {
+  return f32x4{x[g * 4], x[g * 4 + 1], x[g * 4 + 2], x[g * 4 + 3]};
+}
 
 // c = a b over tiles of BM x BN, WM x WN waves.  PAIR: the columns of a tile are BN / 2
 // of the first half of N and the same of the second.
@@ -124,70 +167,136 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_kernel(Product p) {
       ob.go(static_cast<const T*>(p.b) + N * p.b_ld, p.b_ld, n0, N, j * kK, p.K, to + OA::kBytes + OB::kBytes, wave, lane);
   };
 
-  f32x16 acc[MT][NT] = {};
-  if (lo < hi) fetch(lo);
-  for (int j = lo; j < hi; ++j) {
-    copies_done();
-    barrier();
-    if (j + 1 < hi) fetch(j + 1);
+  // The fragments of a sixteenth of the sum, read while the products of the one before
+  // run: without that order, which the compiler would undo, a wave waits for LDS before
+  // every other product.
+  typename E::x8 fa[2][MT], fb[2][NT];
+  auto read = [&](int j, int kk, int into) {
     const char* at = smem + (j & 1) * kStage;
     const char* bt = at + OA::kBytes;
 #pragma unroll
-    for (int kk = 0; kk < kK / 16; ++kk) {
-      typename E::x8 a[MT], b[NT];
+    for (int i = 0; i < NT; ++i)
+      fb[into][i] = PAIR ? OB::read(bt + (i < NT / 2 ? 0 : OB::kBytes), wn * NT * 16 + i % (NT / 2 ? NT / 2 : 1) * 32, kk, lane)
+                         : OB::read(bt, wn * NT * 32 + i * 32, kk, lane);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) a[i] = OA::read(at, wm * MT * 32 + i * 32, kk, lane);
+    for (int i = 0; i < MT; ++i) fa[into][i] = OA::read(at, wm * MT * 32 + i * 32, kk, lane);
+  };
+  f32x16 acc[MT][NT] = {};
+  auto multiply = [&](int from) {
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-        b[i] = PAIR ? OB::read(bt + (i < NT / 2 ? 0 : OB::kBytes), wn * NT * 16 + i % (NT / 2 ? NT / 2 : 1) * 32, kk, lane)
-                    : OB::read(bt, wn * NT * 32 + i * 32, kk, lane);
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int k = 0; k < NT; ++k) acc[i][k] = E::mfma(fb[from][k], fa[from][i], acc[i][k]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (lo < hi) {
+    fetch(lo);
+    copies_done();
+    barrier();
+    if (lo + 1 < hi) fetch(lo + 1);
+    read(lo, 0, 0);
+    for (int j = lo; j < hi; ++j) {
 #pragma unroll
-        for (int k = 0; k < NT; ++k) acc[i][k] = E::mfma(b[k], a[i], acc[i][k]);
+      for (int kk = 0; kk + 1 < kK / 16; ++kk) {
+        read(j, kk + 1, (kk + 1) & 1);
+        multiply(kk & 1);
+      }
+      if (j + 1 < hi) {
+        copies_done();
+        barrier();  // step j + 1 has landed for every wave, and everyone has read step j
+        if (j + 2 < hi) fetch(j + 2);
+        read(j + 1, 0, 0);
+      }
+      multiply(1);
     }
   }
 
-  // lane % 32 = row of c, registers = columns, 4 in a row each
+  // Lane % 32 = row of c, registers = columns, 4 in a row each.  A split's parts go out as
+  // they lie; results by way of LDS, which the wave leaves in whole stretches of rows.
+  constexpr int CT = PAIR ? NT / 2 : NT, W = CT * 32;  // a wave's columns of c
+  const int nw = n0 + wn * W;
+  if (p.splits > 1) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = m0 + wm * MT * 32 + i * 32 + (lane & 31);
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int k = 0; k < CT; ++k)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int n = nw + k * 32 + g * 8 + (lane >> 5) * 4;
+          if (n >= N) continue;  // N is a multiple of 8
+          float* to = p.partial + (static_cast<int64_t>(split) * p.M + m) * p.N + n;
+          *reinterpret_cast<f32x4*>(to) = quarter(acc[i][k], g);
+          if (PAIR) *reinterpret_cast<f32x4*>(to + N) = quarter(acc[i][(CT + k) % NT], g);
+        }
+    }
+    return;
+  }
+  barrier();  // everyone has read the last step
+  constexpr int kRow = W * 2, kRows = 64 * 16 / kRow, kArea = 32 * kRow;  // bytes a row, rows a store
+  char* const own = smem + wave * (PAIR ? 4 : 1) * kArea;
+  const int row = lane & 31, half = lane >> 5;
+  // 16-byte chunk c of row r; 8 (or 4) rows lie side by side in the banks
+  const auto place = [](int r, int c) { return r * kRow + ((c ^ ((r >> (W == 64 ? 1 : 2)) & (W / 8 - 1))) << 4); };
+  const auto out = [&](const char* from, char* base, int64_t stride, int m, int n) {
+#pragma unroll
+    for (int i = 0; i < 32 / kRows; ++i) {
+      const int r = i * kRows + lane / (W / 8), c = lane % (W / 8);
+      const i32x4 v = *reinterpret_cast<const i32x4*>(from + place(r, c));
+      if (m + r < p.M && n + c * 8 < N) *reinterpret_cast<i32x4*>(base + (m + r) * stride + (n + c * 8) * 2) = v;
+    }
+  };
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int m = m0 + wm * MT * 32 + i * 32 + (lane & 31);
-    if (m >= p.M) continue;
+    const int m = m0 + wm * MT * 32 + i * 32;
 #pragma unroll
-    for (int k = 0; k < (PAIR ? NT / 2 : NT); ++k)
+    for (int k = 0; k < CT; ++k)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const int n = n0 + wn * (PAIR ? NT * 16 : NT * 32) + k * 32 + g * 8 + (lane >> 5) * 4;
-        if (n >= N) continue;  // N is a multiple of 8
-        if (p.splits > 1) {
-          f32x4 x, y;
+        const f32x4 x = quarter(acc[i][k], g);
+        f32x4 c = x;
+        const int at = place(row, k * 4 + g) + half * 8;
+        if constexpr (PAIR) {
+          const f32x4 y = quarter(acc[i][(CT + k) % NT], g);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = acc[i][k][g * 4 + j], y[j] = PAIR ? acc[i][(NT / 2 + k) % NT][g * 4 + j] : 0.f;
-          float* to = p.partial + (static_cast<int64_t>(split) * p.M + m) * p.N + n;
-          *reinterpret_cast<f32x4*>(to) = x;
-          if (PAIR) *reinterpret_cast<f32x4*>(to + N) = y;
-        } else if (PAIR) {
-          typename E::x4 h;
-          f32x4 x, y;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j] = acc[i][k][g * 4 + j];
-            y[j] = acc[i][(NT / 2 + k) % NT][g * 4 + j];
-            h[j] = static_cast<T>(x[j] * sigmoid(x[j]) * y[j]);
-          }
-          *reinterpret_cast<typename E::x4*>(static_cast<T*>(p.c) + static_cast<int64_t>(m) * N + n) = h;
+          for (int j = 0; j < 4; ++j) c[j] = x[j] * sigmoid(x[j]) * y[j];
           if (p.saved) {
-            float* to = p.saved + static_cast<int64_t>(m) * p.N + n;
-            *reinterpret_cast<f32x4*>(to) = x;
-            *reinterpret_cast<f32x4*>(to + N) = y;
+            u32x2 h;
+            uint32_t l;
+            Saved::split(x, h, l);
+            *reinterpret_cast<u32x2*>(own + kArea + at) = h;
+            *reinterpret_cast<uint32_t*>(own + 3 * kArea + at / 2) = l;
+            Saved::split(y, h, l);
+            *reinterpret_cast<u32x2*>(own + 2 * kArea + at) = h;
+            *reinterpret_cast<uint32_t*>(own + 3 * kArea + kArea / 2 + at / 2) = l;
           }
-        } else {
-          typename E::x4 x;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = static_cast<T>(acc[i][k][g * 4 + j]);
-          *reinterpret_cast<typename E::x4*>(static_cast<T*>(p.c) + static_cast<int64_t>(m) * N + n) = x;
         }
+        typename E::x4 r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] = static_cast<T>(c[j]);
+        *reinterpret_cast<typename E::x4*>(own + at) = r;
       }
+    out(own, static_cast<char*>(p.c), static_cast<int64_t>(N) * 2, m, nw);
+    if constexpr (PAIR) {
+      if (p.saved) {
+        const int64_t stride = 3ll * p.N;
+        char* const base = reinterpret_cast<char*>(p.saved);
+        out(own + kArea, base, stride, m, nw);
+        out(own + 2 * kArea, base + 2 * N, stride, m, nw);
+        // the low bytes, 8 a lane
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+          for (int s = 0; s < 32 / kRows; ++s) {
+            const int r = s * kRows + lane / (W / 8), c = lane % (W / 8);
+            const u32x2 x = *reinterpret_cast<const u32x2*>(own + 3 * kArea + v * (kArea / 2) + place(r, c) / 2);
+            if (m + r < p.M && nw + c * 8 < N)
+              *reinterpret_cast<u32x2*>(base + (m + r) * stride + 2 * p.N + v * N + nw + c * 8) = x;
+          }
+      }
+    }
   }
 }
 
@@ -209,22 +318,22 @@ template <class T, bool PAIR> __global__ __launch_bounds__(256) void join_kernel
   for (int j = 0; j < 4; ++j) h[j] = static_cast<T>(PAIR ? x[j] * sigmoid(x[j]) * y[j] : x[j]);
   *reinterpret_cast<x4*>(static_cast<T*>(p.c) + i) = h;
   if (PAIR && p.saved) {
-    float* to = p.saved + m * p.N + n;
-    *reinterpret_cast<f32x4*>(to) = x;
-    *reinterpret_cast<f32x4*>(to + N) = y;
+    const Saved to(p.saved, m, p.N);
+    to.store(n, x);
+    to.store(N + n, y);
   }
 }
 
 // [dg du] from dh and the saved [g u], 4 columns a thread.
-template <class T> __global__ __launch_bounds__(256) void gate_bwd_kernel(const T* dh, int64_t dh_ld, const float* saved,
-                                                                         T* d, int M, int F) {
+template <class T> __global__ __launch_bounds__(256) void gate_bwd_kernel(const T* dh, int64_t dh_ld, uint8_t* saved, T* d,
+                                                                         int M, int F) {
   using x4 = typename El<T>::x4;
   const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4;
   if (i >= static_cast<int64_t>(M) * F) return;
   const int64_t m = i / F, n = i % F;
   const x4 a = *reinterpret_cast<const x4*>(dh + m * dh_ld + n);
-  const f32x4 g = *reinterpret_cast<const f32x4*>(saved + m * 2 * F + n);
-  const f32x4 u = *reinterpret_cast<const f32x4*>(saved + m * 2 * F + F + n);
+  const Saved from(saved, m, 2 * F);
+  const f32x4 g = from.load(n), u = from.load(F + n);
   x4 dg, du;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -267,14 +376,14 @@ template <class T, bool TA, bool TB, bool PAIR> int product(const Product& p, in
 }
 
 template <class T> int forward(const KgsSwiglu& a, hipStream_t s) {
-  const Product p{a.x, a.w, a.x_ld, a.w_ld, a.h, static_cast<float*>(a.saved), a.partial, a.T, 2 * a.F, a.K, a.splits[0]};
+  const Product p{a.x, a.w, a.x_ld, a.w_ld, a.h, static_cast<uint8_t*>(a.saved), a.partial, a.T, 2 * a.F, a.K, a.splits[0]};
   return product<T, false, false, true>(p, a.tile[0], s);
 }
 
 template <class T> int backward(const KgsSwiglu& a, hipStream_t s) {
   const int64_t n = static_cast<int64_t>(a.T) * a.F / 4;
   gate_bwd_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(
-      static_cast<const T*>(a.dh), a.dh_ld, static_cast<const float*>(a.saved), static_cast<T*>(a.dgu), a.T, a.F);
+      static_cast<const T*>(a.dh), a.dh_ld, static_cast<uint8_t*>(a.saved), static_cast<T*>(a.dgu), a.T, a.F);
   if (launched("swiglu gate backward")) return -1;
   if (a.dx) {
     const Product p{a.dgu, a.w, 2ll * a.F, a.w_ld, a.dx, nullptr, a.partial, a.T, a.K, 2 * a.F, a.splits[1]};
@@ -299,7 +408,8 @@ int check(const KgsSwiglu* a, bool back) {
   if (back && (a->dh_ld < a->F || a->dh_ld % 8)) return fail(w, "unsupported strides");
   if (a->type != 0 && a->type != 1) return fail(w, "type must be bfloat16 or float16");
   for (int i = back ? 1 : 0; i < (back ? 3 : 1); ++i)
-    if (a->splits[i] < 1 || (a->splits[i] > 1 && !a->partial)) return fail(w, "bad split");
+    if ((i == 1 && !a->dx) || (i == 2 && !a->dw)) continue;
+    else if (a->splits[i] < 1 || (a->splits[i] > 1 && !a->partial)) return fail(w, "bad split");
   return 0;
 }
 

@@ -299,9 +299,9 @@ def swiglu_oracle(x, w, dh):
     # |silu'| <= 1.1, |silu''| <= 0.5
     r = {"h": h, "saved": gu}
     tol = {"h": u * h.abs() + 1.01 * (1.1 * up.abs() * eg + act.abs() * eu) + 16 * E32 * h.abs() + sub,
-           "saved": e}
+           "saved": e + 2.0 ** -16 * gu.abs()}  # 24 of 32 bits: 23 - 8 = 15 of the fraction, half a step is 2^-16
     dg, du = G * up * slope, G * act
-    # the backward sees g and u as saved (32 bits), rounds dg and du
+    # the backward sees g and u as saved, rounds dg and du
     rg, ru = tol["saved"][:, :F], tol["saved"][:, F:]
     e_dg = 1.02 * G.abs() * (up.abs() * 0.5 * rg + 1.1 * ru) + (u + 16 * E32) * dg.abs() + sub
     e_du = 1.02 * G.abs() * 1.1 * rg + (u + 16 * E32) * du.abs() + sub
@@ -318,11 +318,18 @@ def swiglu_inputs(T, K, F, t, dev, seed=0):
     return mk(T, K), mk(2 * F, K, std=K ** -0.5), mk(T, F)
 
 
+def projections(saved):
+    """The 32-bit values of a ``saved`` of swiglu_fwd, [..., 2 inner]."""
+    n = saved.shape[-1] // 3
+    high = saved[..., :2 * n].contiguous().view(torch.int16).int() << 16
+    return (high | (saved[..., 2 * n:].int() << 8)).view(F32)
+
+
 def swiglu_check(x, w, dh):
     h, saved = decoder.swiglu_fwd(x, w)
     dx, dw = decoder.swiglu_bwd(dh, x, w, saved)
     ref, tol = swiglu_oracle(x.reshape(-1, x.shape[-1]), w, dh.reshape(-1, dh.shape[-1]))
-    for n, got in (("h", h), ("saved", saved), ("dx", dx), ("dw", dw)):
+    for n, got in (("h", h), ("saved", projections(saved)), ("dx", dx), ("dw", dw)):
         close(got.reshape(ref[n].shape), ref[n], tol[n], n)
     assert torch.equal(decoder.swiglu(x, w), h)
     return h, saved, dx, dw
@@ -418,6 +425,14 @@ def test_swiglu_autograd(dev):
     a2 = x.clone().requires_grad_()
     decoder.swiglu(a2, w).backward(dh)
     assert torch.equal(a2.grad, want[2])
+    # one gradient wanted where both products' sums are cut into parts
+    x, w, dh = swiglu_inputs(1100, 72, 1032, BF16, dev)
+    assert decoder._product_plan(1100, 72, 2064)[1] > 1 and decoder._product_plan(2064, 72, 1100)[1] > 1
+    want = swiglu_check(x, w, dh)
+    a2, b2 = x.clone().requires_grad_(), w.clone().requires_grad_()
+    decoder.swiglu(a2, w).backward(dh)
+    decoder.swiglu(x, b2).backward(dh)
+    assert torch.equal(a2.grad, want[2]) and torch.equal(b2.grad, want[3])
 
 
 @gpu
@@ -794,8 +809,8 @@ SWIGLU_REFUSED = [
     ("no inner", lambda: decoder.swiglu(z(4, 64), z(0, 64)), ValueError),
     ("device", lambda: decoder.swiglu(z(4, 64), z(16, 64)), ValueError),
     ("dh shape", lambda: decoder.swiglu_bwd(z(4, 16), z(4, 64), z(16, 64), z(4, 16)), ValueError),
-    ("saved shape", lambda: decoder.swiglu_bwd(z(4, 8), z(4, 64), z(16, 64), z(4, 8, t=F32)), ValueError),
-    ("saved type", lambda: decoder.swiglu_bwd(z(4, 8), z(4, 64), z(16, 64), z(4, 16)), ValueError),
+    ("saved shape", lambda: decoder.swiglu_bwd(z(4, 8), z(4, 64), z(16, 64), z(4, 24, t=torch.uint8)), ValueError),
+    ("saved type", lambda: decoder.swiglu_bwd(z(4, 8), z(4, 64), z(16, 64), z(4, 48)), ValueError),
 ]
 NORM_REFUSED = [
     ("type", lambda: decoder.add_norm(*[z(4, 64, t=torch.float64)] * 2, z(64, t=torch.float64)), TypeError),
