@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 import os
 import struct
@@ -326,14 +327,30 @@ def _swiglu_checks(x, w, **more):
 PRODUCT_TILES = (0, 1)  # the tiles of swiglu.hip's product: 128 x 128, 256 x 256
 
 
+@functools.lru_cache(maxsize=4096)
 def _product_plan(M: int, N: int, K: int) -> tuple[int, int]:
-    """(tile, splits) of an [M, N] product over K: the 256 x 256 tile where its workgroups fill
-    the CUs, else 128 x 128, with the sum cut into parts while the CUs have room for two
-    workgroups each and a part keeps 8 steps of 64."""
-    if -(-M // 256) * -(-N // 256) >= 200:
-        return 1, 1
-    tiles = -(-M // 128) * -(-N // 128)
-    return 0, max(1, min(512 // tiles, K // 512, 16))
+    """(tile, splits) of an [M, N] product over K: the least of the times expected, from what
+    the tiles were measured at.  A step of 64 of the sum takes all workgroups that run at
+    once 1.83 us with the 256 x 256 tile (one a CU), 1.10 us with 128 x 128 (two a CU; 0.74
+    us if there is no more than one); a round of workgroups has a start and an end of its
+    own; the parts of a split sum are written and read as 32-bit numbers, at 4 TB/s, by
+    one more launch.  (2048 x 10752 over 2048: 115 us with 256 x 256, two rounds of which
+    the second is a third full, and 103 us with 128 x 128; 8192 x 22016 over 4096: 1290 us
+    and 1550 us.)"""
+    best = None
+    for tile, size, at_once in ((0, 128, 512), (1, 256, 256)):
+        blocks = -(-M // size) * -(-N // size)
+        for splits in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16):
+            steps = -(-K // 64 // splits)
+            if splits > 1 and steps < 8:
+                break
+            step = 1.83 if tile else 1.10 if blocks * splits > 256 else 0.74
+            time = -(-blocks * splits // at_once) * (steps * step + (8 if tile else 3.5))
+            if splits > 1:
+                time += 4 + 2 * splits * M * N * 4 / 4e6
+            if best is None or time < best[0]:
+                best = time, tile, splits
+    return best[1:]
 
 
 def swiglu(x, w):

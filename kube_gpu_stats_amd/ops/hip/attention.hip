@@ -31,6 +31,11 @@ constexpr int NW = 4, kThreads = NW * kWave, kRows = NW * 32;
 constexpr int NS = 2;       // slots of LDS: one step in work, one under way
 constexpr int kStep = 64;   // keys a step of forward and dq
 constexpr int kQStep = 32;  // rows a step of dk, dv
+constexpr int kAhead = 1;   // fragments of k read ahead of the products, forward
+
+// Matrix products and LDS reads stay on their side of this; arithmetic may cross.  The
+// compiler would place each read right before its product, with a wait between them.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0x406); }
 
 __device__ __forceinline__ int length_of(const KgsAttention& a, int b) {
   if (!a.lengths) return a.S;
@@ -183,10 +188,23 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
     slot = slot == NS - 1 ? 0 : slot + 1;
     if (s0 >= last) continue;
     f32x16 s[2] = {};
+    {
+      typename E::x8 f[kAhead + 1][2];
+      auto read = [&](int kk) {
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk)
+        for (int t = 0; t < 2; ++t) f[kk % (kAhead + 1)][t] = Tl::template rows<T>(kt, t * 32, kk, lane);
+      };
 #pragma unroll
-      for (int t = 0; t < 2; ++t) s[t] = E::mfma(Tl::template rows<T>(kt, t * 32, kk, lane), q[kk], s[t]);
+      for (int kk = 0; kk < kAhead; ++kk) read(kk);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        if (kk + kAhead < D / 16) read(kk + kAhead);
+        in_order();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t] = E::mfma(f[kk % (kAhead + 1)][t], q[kk], s[t]);
+        in_order();
+      }
+    }
     if (s0 + kStep > open) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -331,10 +349,21 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       f32x16 s = {}, dp = {};
+      {
+        typename E::x8 f[2][2];
+        auto read = [&](int kk) {
+          f[kk & 1][0] = Tl::template rows<T>(kt, t * 32, kk, lane);
+          f[kk & 1][1] = Tl::template rows<T>(vt, t * 32, kk, lane);
+        };
+        read(0);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        s = E::mfma(Tl::template rows<T>(kt, t * 32, kk, lane), q[kk], s);
-        dp = E::mfma(Tl::template rows<T>(vt, t * 32, kk, lane), g[kk], dp);
+        for (int kk = 0; kk < D / 16; ++kk) {
+          if (kk + 1 < D / 16) read(kk + 1);
+          in_order();
+          s = E::mfma(f[kk & 1][0], q[kk], s);
+          dp = E::mfma(f[kk & 1][1], g[kk], dp);
+          in_order();
+        }
       }
       const bool edge = s0 + t * 32 + 32 > open;
 #pragma unroll
@@ -446,10 +475,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
     if (++ss == each) ss = 0;
     if (CAUSAL && s0 + kQ <= kw) continue;  // no row of the step sees the wave's keys
     f32x16 s = {}, dp = {};
+    {
+      typename E::x8 f[2][3];
+      auto read = [&](int kk) {
+        f[kk & 1][0] = Tl::template rows<T>(qt, 0, kk, lane);
+        f[kk & 1][1] = Tl::template rows<T>(gt, 0, kk, lane);
+        f[kk & 1][2] = Tl::template rows<T>(smem, wave * 32, kk, lane);
+      };
+      read(0);
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      s = E::mfma(Tl::template rows<T>(qt, 0, kk, lane), k[kk], s);
-      dp = E::mfma(Tl::template rows<T>(gt, 0, kk, lane), Tl::template rows<T>(smem, wave * 32, kk, lane), dp);
+      for (int kk = 0; kk < D / 16; ++kk) {
+        if (kk + 1 < D / 16) read(kk + 1);
+        in_order();
+        s = E::mfma(f[kk & 1][0], k[kk], s);
+        dp = E::mfma(f[kk & 1][1], f[kk & 1][2], dp);
+        in_order();
+      }
     }
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
@@ -467,13 +508,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
       for (int r = 0; r < 16; ++r)
         if (s0 + acc_row(r, lane) < key) s[r] = dp[r] = 0.f;
     }
+    {
+      const typename E::x8 p[2] = {operand<T>(s, 0), operand<T>(s, 1)}, ds[2] = {operand<T>(dp, 0), operand<T>(dp, 1)};
+      typename E::x8 f[2][2];
+      auto read = [&](int i) {
+        f[i & 1][0] = Tl::template columns<T>(gt, i / (D / 32) * 16, i % (D / 32) * 32, lane);
+        f[i & 1][1] = Tl::template columns<T>(qt, i / (D / 32) * 16, i % (D / 32) * 32, lane);
+      };
+      read(0);
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const typename E::x8 p = operand<T>(s, hh), ds = operand<T>(dp, hh);
-#pragma unroll
-      for (int e = 0; e < D / 32; ++e) {
-        dva[e] = E::mfma(Tl::template columns<T>(gt, hh * 16, e * 32, lane), p, dva[e]);
-        dka[e] = E::mfma(Tl::template columns<T>(qt, hh * 16, e * 32, lane), ds, dka[e]);
+      for (int i = 0; i < D / 16; ++i) {
+        const int hh = i / (D / 32), e = i % (D / 32);
+        if (i + 1 < D / 16) read(i + 1);
+        in_order();
+        dva[e] = E::mfma(f[i & 1][0], p[hh], dva[e]);
+        dka[e] = E::mfma(f[i & 1][1], ds[hh], dka[e]);
+        in_order();
       }
     }
   }

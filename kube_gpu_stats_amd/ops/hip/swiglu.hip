@@ -144,12 +144,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_kernel(Product p) {
   const int64_t total = static_cast<int64_t>(tm) * tn * p.splits;
   const int64_t item = xcd_item(blockIdx.x, total);
   if ((blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
-  // Items in bands of 8 tiles of rows: an XCD's workgroups share 8 row tiles and few
+  // Items in bands of 4 tiles of rows: the workgroups of an XCD share 4 row tiles and few
   // column tiles through their L2.
   const int split = static_cast<int>(item / (static_cast<int64_t>(tm) * tn));
   const int t = static_cast<int>(item % (static_cast<int64_t>(tm) * tn));
-  const int band = t / (8 * tn), high = min(8, tm - band * 8), in = t - band * 8 * tn;
-  const int m0 = (band * 8 + in % high) * BM, n0 = in / high * (PAIR ? HALF : BN);
+  const int band = t / (4 * tn), high = min(4, tm - band * 4), in = t - band * 4 * tn;
+  const int m0 = (band * 4 + in % high) * BM, n0 = in / high * (PAIR ? HALF : BN);
   const int steps_all = (p.K + kK - 1) / kK;
   const int lo = static_cast<int>(static_cast<int64_t>(steps_all) * split / p.splits);
   const int hi = static_cast<int>(static_cast<int64_t>(steps_all) * (split + 1) / p.splits);
