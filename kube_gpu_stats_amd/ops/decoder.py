@@ -501,11 +501,14 @@ def _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, strea
 
 
 def _norm_parts(T: int, C: int) -> int:
-    """Parts that the backward's column sums come in: one a workgroup (of rows up to 512
-    wide, four rows a workgroup and a part a row), a workgroup taking rows in turn."""
-    rows = 4 if C <= 512 else 1
-    threads = 256 if C <= 4096 else 512 if C <= 8192 else 1024
-    return rows * min(-(-T // rows), 256 * 1024 // threads)
+    """Workgroups of the backward, each of which leaves a part of the column sums: as many as
+    run at once, 16 waves a CU.  Rows up to 512 wide share a workgroup of four waves, a
+    power of two of lanes with 8 elements each to a row."""
+    if C <= 512:
+        lanes = 1 << (-(-C // 8) - 1).bit_length()
+        return min(-(-T // (256 // lanes)), 1024)
+    waves = -(-C // 512) if C <= 8192 else -(-C // 1024)
+    return min(T, 256 * (16 // waves))
 
 
 def add_norm_bwd(dstream, dout, stream_, branch, weight, saved, *, post_weight=None, gate=None, scale: float = 1.0,
@@ -537,7 +540,7 @@ def add_norm_bwd(dstream, dout, stream_, branch, weight, saved, *, post_weight=N
             (ds, ds_ld), (dy, dy_ld) = (_lines(t) if t is not None else (None, 0) for t in (dstream, dout))
             w, pw, g = (None if t is None else t.contiguous() for t in (weight, post_weight, gate))
             parts = _norm_parts(T, C)
-            work = torch.empty(parts * 3 * C, dtype=torch.float32, device=s.device)
+            work = torch.empty(parts * 2 * C, dtype=torch.float32, device=s.device)
             args = _ADD_NORM.pack(0, _ptr(b), _ptr(w), _ptr(pw), _ptr(g), _ptr(s), 0, _ptr(saved), _ptr(ds), _ptr(dy),
                                   _ptr(dr), _ptr(db), *(_ptr(t) for t in grads), _ptr(work), 0, b_ld, s_ld, ds_ld, dy_ld,
                                   T, C, code, parts, scale, eps)

@@ -4,13 +4,15 @@
 //   s = r + scale gate n,   y = weight s rs  (rs = 1 / sqrt(mean s^2 + eps))
 //   ds = dS + rs (w dy - s rs^2 mean(w dy s)),   dr = ds,   t = scale ds
 //   dn = gate t,   db = rb (pw dn - b rb^2 mean(pw dn b))  (db = dn without post_weight)
-//   dweight = sum dy s rs,  dpost_weight = sum dn b rb,  dgate = sum t n   over the rows
+//   dweight = sum dy s rs,  with A = sum ds b rb over the rows:
+//   dpost_weight = scale gate A,  dgate = scale post_weight A
 //
 // Bound by memory: each row is read once and stays in its threads' registers between
-// the two means; the weights stay there from row to row.  A workgroup takes rows in
-// turn; for the backward's column sums each thread adds its columns in registers over
-// its rows, the workgroups' sums are joined by a second kernel in a fixed order (no
-// atomics, so equal calls give equal bits).
+// the two means; the weights stay there from row to row.  Rows up to 512 wide take a
+// power of two of lanes, 8 elements each, so that a wave works on several; wider ones a
+// workgroup.  Workgroups take rows in turn; for the backward's column sums each thread
+// adds its columns in registers over its rows, the workgroups' sums are joined by a
+// second kernel in a fixed order (no atomics, so equal calls give equal bits).
 //
 // Everything is computed in 32 bits and rounded once, as an output.  The forward
 // normalises the unrounded stream; the backward sees it as it was stored.
@@ -37,6 +39,16 @@ template <class T> __device__ __forceinline__ void load(float (&x)[kV], const T*
   }
 }
 
+// The same as it lies in memory.
+template <class T> __device__ __forceinline__ void load_raw(Loose<T>& r, const T* p, int c, int left) {
+  if (left >= kV) {
+    r = *reinterpret_cast<const Loose<T>*>(p + c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) r.v[i] = i < left ? p[c + i] : static_cast<T>(0.f);
+  }
+}
+
 template <class T> __device__ __forceinline__ void store(const float (&x)[kV], T* p, int left) {
   if (left >= kV) {
     Loose<T> r;
@@ -50,54 +62,75 @@ template <class T> __device__ __forceinline__ void store(const float (&x)[kV], T
   }
 }
 
-// Sum over a row's threads.  One wave a row: no LDS.  More: one slot a wave, and two
-// sets of slots in turn so that one barrier a sum is enough.
-template <int TPR> __device__ __forceinline__ float row_sum(float x, float* slots, int& turn) {
+// Sum over the threads of a row: `lanes` of a wave (a power of two), or the workgroup,
+// by way of one slot a wave in two sets used in turn, so that one barrier is enough.
+template <bool WAVES> __device__ __forceinline__ float row_sum(float x, int lanes, float* slots, int& turn) {
+  if constexpr (WAVES) {
+    for (int m = 1; m < lanes; m <<= 1) x += __shfl_xor(x, m, 64);
+  } else {
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, 64);
-  if constexpr (TPR > 64) {
-    float* s = slots + turn * (TPR / 64);
+    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m, 64);
+    float* s = slots + turn * 16;
     turn ^= 1;
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = x;
     __syncthreads();
     x = 0.f;
-#pragma unroll
-    for (int i = 0; i < TPR / 64; ++i) x += s[i];
+    for (unsigned i = 0; i < blockDim.x / 64; ++i) x += s[i];
   }
   return x;
 }
 
-template <int TPR> struct Shape {
-  static constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
+__host__ __device__ __forceinline__ int lanes_of_row(int width) {
+  int n = 1;
+  while (n * kV < width) n *= 2;
+  return n;
+}
+
+// Where a thread stands: the first column chunk of its row, the row of its workgroup's
+// turn, and the rows a turn.  WAVES: widths up to 512.
+template <bool WAVES> struct Place {
+  int lanes, t, row, rows;
+  __device__ __forceinline__ explicit Place(int width) {
+    lanes = WAVES ? lanes_of_row(width) : blockDim.x;
+    t = WAVES ? threadIdx.x & (lanes - 1) : threadIdx.x;
+    row = WAVES ? threadIdx.x / lanes : 0;
+    rows = WAVES ? 256 / lanes : 1;
+  }
 };
 
-// FULL: with post_weight or gate (or a scale).  NV: chunks of 8 a thread.
-template <class T, int TPR, int NV, bool FULL>
-__global__ __launch_bounds__(Shape<TPR>::kThreads) void add_norm_fwd_kernel(KgsAddNorm a) {
-  __shared__ float slots[2 * (TPR > 64 ? TPR / 64 : 1)];
+// FULL: with post_weight, gate or a scale.  NV: chunks of 8 a thread.
+template <class T, bool WAVES, int NV, bool FULL>
+__global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_fwd_kernel(KgsAddNorm a) {
+  __shared__ float slots[2 * 16];
   int turn = 0;
-  const int t = threadIdx.x % TPR, C = a.width;
+  const Place<WAVES> at(a.width);
+  const int C = a.width;
   const T *residual = static_cast<const T*>(a.residual), *branch = static_cast<const T*>(a.branch);
-  float w[NV][kV], pw[FULL ? NV : 1][kV], gate[FULL ? NV : 1][kV];
+  float w[NV][kV], pw[FULL ? NV : 1][kV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (t + i * TPR) * kV;
+    const int c = (at.t + i * at.lanes) * kV;
     load(w[i], static_cast<const T*>(a.weight) + c, C - c);
-    if constexpr (FULL) {
-      if (a.post_weight) load(pw[i], static_cast<const T*>(a.post_weight) + c, C - c);
-      else for (float& x : pw[i]) x = 1.f;
-      if (a.gate) load(gate[i], static_cast<const T*>(a.gate) + c, C - c);
-      else for (float& x : gate[i]) x = 1.f;
-      for (float& x : gate[i]) x *= a.scale;
+    if constexpr (FULL) {  // what the normalised branch is multiplied by
+      for (float& x : pw[i]) x = a.scale;
+      float f[kV];
+      if (a.post_weight) {
+        load(f, static_cast<const T*>(a.post_weight) + c, C - c);
+        for (int j = 0; j < kV; ++j) pw[i][j] *= f[j];
+      }
+      if (a.gate) {
+        load(f, static_cast<const T*>(a.gate) + c, C - c);
+        for (int j = 0; j < kV; ++j) pw[i][j] *= f[j];
+      }
     }
   }
-  const int step = gridDim.x * Shape<TPR>::kRows;
-  for (int row = blockIdx.x * Shape<TPR>::kRows + threadIdx.x / TPR; row < a.rows; row += step) {
+  const int step = gridDim.x * at.rows;
+  for (int row = blockIdx.x * at.rows + at.row; row < a.rows; row += step) {
     float s[NV][kV], b[NV][kV];
     float sq = 0.f, rb = 1.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * TPR) * kV;
+      const int c = (at.t + i * at.lanes) * kV;
       load(b[i], branch + row * a.branch_ld + c, C - c);
       load(s[i], residual + row * a.residual_ld + c, C - c);
     }
@@ -107,171 +140,248 @@ __global__ __launch_bounds__(Shape<TPR>::kThreads) void add_norm_fwd_kernel(KgsA
         for (int i = 0; i < NV; ++i)
 #pragma unroll
           for (int j = 0; j < kV; ++j) sq = fmaf(b[i][j], b[i][j], sq);
-        rb = 1.f / sqrtf(row_sum<TPR>(sq, slots, turn) / C + a.eps);
+        rb = 1.f / sqrtf(row_sum<WAVES>(sq, at.lanes, slots, turn) / C + a.eps);
         sq = 0.f;
       }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * TPR) * kV;
+      const int c = (at.t + i * at.lanes) * kV;
 #pragma unroll
       for (int j = 0; j < kV; ++j) {
-        if constexpr (FULL) s[i][j] = fmaf(gate[i][j], b[i][j] * rb * pw[i][j], s[i][j]);
+        if constexpr (FULL) s[i][j] = fmaf(pw[i][j], b[i][j] * rb, s[i][j]);
         else s[i][j] += b[i][j];
         sq = fmaf(s[i][j], s[i][j], sq);
       }
       store(s[i], static_cast<T*>(a.stream) + row * a.stream_ld + c, C - c);
     }
-    const float rs = 1.f / sqrtf(row_sum<TPR>(sq, slots, turn) / C + a.eps);
+    const float rs = 1.f / sqrtf(row_sum<WAVES>(sq, at.lanes, slots, turn) / C + a.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * TPR) * kV;
+      const int c = (at.t + i * at.lanes) * kV;
 #pragma unroll
       for (int j = 0; j < kV; ++j) s[i][j] *= rs * w[i][j];
       store(s[i], static_cast<T*>(a.out) + static_cast<int64_t>(row) * C + c, C - c);
     }
-    if (a.rstd && t == 0) {
+    if (a.rstd && at.t == 0) {
       a.rstd[row] = rs;
       a.rstd[a.rows + row] = rb;
     }
   }
 }
 
-template <class T, int TPR, int NV, bool FULL>
-__global__ __launch_bounds__(Shape<TPR>::kThreads) void add_norm_bwd_kernel(KgsAddNorm a) {
-  constexpr int kRows = Shape<TPR>::kRows;
-  __shared__ float slots[2 * (TPR > 64 ? TPR / 64 : 1)];
+// The next row's loads are under way while this one is reduced; with one chunk a thread
+// that fits the registers of 16 waves a CU.  Two chunks (rows over 8192 wide) do without,
+// and read the weights again for every row.  WHOLE: the width is a multiple of 8, so that
+// a chunk is there or not: a thread past the end reads the row's first chunk, without a
+// branch, and its zero weights keep it out of the sums.
+template <class T, bool WAVES, int NV, bool FULL, bool WHOLE>
+__global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_bwd_kernel(KgsAddNorm a) {
+  __shared__ float slots[2 * 16];
+  __shared__ float sums[WAVES ? (FULL ? 2 : 1) * 4 * 512 : 1];
+  constexpr bool kAhead = NV == 1;
   int turn = 0;
-  const int t = threadIdx.x % TPR, C = a.width;
-  float w[NV][kV], pw[FULL ? NV : 1][kV], gate[FULL ? NV : 1][kV];
-  float dw[NV][kV] = {}, dpw[FULL ? NV : 1][kV] = {}, dgate[FULL ? NV : 1][kV] = {};
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (t + i * TPR) * kV;
-    load(w[i], static_cast<const T*>(a.weight) + c, C - c);
-    if constexpr (FULL) {
-      if (a.post_weight) load(pw[i], static_cast<const T*>(a.post_weight) + c, C - c);
-      else for (float& x : pw[i]) x = 1.f;
-      if (a.gate) load(gate[i], static_cast<const T*>(a.gate) + c, C - c);
-      else for (float& x : gate[i]) x = 1.f;
-    }
-  }
-  const int step = gridDim.x * kRows;
-  for (int row = blockIdx.x * kRows + threadIdx.x / TPR; row < a.rows; row += step) {
-    const float rs = a.rstd[row];
-    float s[NV][kV], dy[NV][kV], ds[NV][kV], b[FULL ? NV : 1][kV];
-    float dot = 0.f;
+  const Place<WAVES> at(a.width);
+  const int C = a.width;
+  const auto column = [&](int i) { return (at.t + i * at.lanes) * kV; };
+  const auto get = [&](Loose<T>& r, const void* p, int64_t start, int c) {
+    const T* from = static_cast<const T*>(p) + start;
+    if constexpr (WHOLE) r = *reinterpret_cast<const Loose<T>*>(from + (c < C ? c : 0));
+    else load_raw(r, from, c, C - c);
+  };
+  // weight, and scale post_weight gate; zero past the end
+  float w[NV][kV], full[FULL ? NV : 1][kV];
+  const auto weights = [&] {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * TPR) * kV;
-      load(s[i], static_cast<const T*>(a.stream) + row * a.stream_ld + c, C - c);
-      if (a.dout) load(dy[i], static_cast<const T*>(a.dout) + row * a.dout_ld + c, C - c);
-      else for (float& x : dy[i]) x = 0.f;
-      if (a.dstream) load(ds[i], static_cast<const T*>(a.dstream) + row * a.dstream_ld + c, C - c);
-      else for (float& x : ds[i]) x = 0.f;
-      if constexpr (FULL) load(b[i], static_cast<const T*>(a.branch) + row * a.branch_ld + c, C - c);
+      const int c = column(i);
+      load(w[i], static_cast<const T*>(a.weight) + c, C - c);
+      if constexpr (FULL) {
+        float f[kV];
+#pragma unroll
+        for (int j = 0; j < kV; ++j) full[i][j] = c + j < C ? a.scale : 0.f;
+        if (a.post_weight) {
+          load(f, static_cast<const T*>(a.post_weight) + c, C - c);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) full[i][j] *= f[j];
+        }
+        if (a.gate) {
+          load(f, static_cast<const T*>(a.gate) + c, C - c);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) full[i][j] *= f[j];
+        }
+      }
     }
+  };
+  if (kAhead) weights();
+  struct Row {
+    Loose<T> s[NV], dy[NV], ds[NV], b[FULL ? NV : 1];
+    float rs, rb;
+  } next;
+  const auto fetch = [&](int row) {
+    next.rs = a.rstd[row];
+    next.rb = FULL ? a.rstd[a.rows + row] : 1.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      get(next.s[i], a.stream, row * a.stream_ld, column(i));
+      if (a.dout) get(next.dy[i], a.dout, row * a.dout_ld, column(i));
+      if (a.dstream) get(next.ds[i], a.dstream, row * a.dstream_ld, column(i));
+      if constexpr (FULL) get(next.b[i], a.branch, row * a.branch_ld, column(i));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < kV; ++j) next.dy[i].v[j] = next.ds[i].v[j] = static_cast<T>(0.f);  // absent
+  float dw[NV][kV] = {}, sum[FULL ? NV : 1][kV] = {};  // column sums: dweight, A
+  const int step = gridDim.x * at.rows;
+  int row = blockIdx.x * at.rows + at.row;
+  if (kAhead && row < a.rows) fetch(row);
+  for (; row < a.rows; row += step) {
+    if (!kAhead) {
+      fetch(row);
+      weights();
+    }
+    float s[NV][kV], dy[NV][kV], ds[NV][kV], b[FULL ? NV : 1][kV];
+    const float rs = next.rs, rb = next.rb;
+    float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < kV; ++j) {
-        s[i][j] *= rs;
-        dw[i][j] = fmaf(dy[i][j], s[i][j], dw[i][j]);
-        dy[i][j] *= w[i][j];
+        const float g = static_cast<float>(next.dy[i].v[j]);
+        s[i][j] = static_cast<float>(next.s[i].v[j]) * rs;
+        ds[i][j] = static_cast<float>(next.ds[i].v[j]);
+        if constexpr (FULL) b[i][j] = static_cast<float>(next.b[i].v[j]) * rb;
+        dw[i][j] = fmaf(g, s[i][j], dw[i][j]);
+        dy[i][j] = g * w[i][j];
         dot = fmaf(dy[i][j], s[i][j], dot);
       }
-    const float mean = row_sum<TPR>(dot, slots, turn) / C;
+    if (kAhead && row + step < a.rows) fetch(row + step);
+    const float mean = row_sum<WAVES>(dot, at.lanes, slots, turn) / C;
+    float dot2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (t + i * TPR) * kV;
+      const int c = column(i);
 #pragma unroll
       for (int j = 0; j < kV; ++j) ds[i][j] = fmaf(rs, dy[i][j] - s[i][j] * mean, ds[i][j]);
       store(ds[i], static_cast<T*>(a.dresidual) + static_cast<int64_t>(row) * C + c, C - c);
-    }
-    if constexpr (FULL) {
-      const float rb = a.rstd[a.rows + row];
-      float dot2 = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
+      if constexpr (FULL) {
 #pragma unroll
         for (int j = 0; j < kV; ++j) {
-          const float bh = b[i][j] * rb, g = ds[i][j] * a.scale, dn = g * gate[i][j];
-          dgate[i][j] = fmaf(g, bh * pw[i][j], dgate[i][j]);
-          dpw[i][j] = fmaf(dn, bh, dpw[i][j]);
-          b[i][j] = bh;
-          ds[i][j] = dn * pw[i][j];
-          dot2 = fmaf(ds[i][j], bh, dot2);
+          sum[i][j] = fmaf(ds[i][j], b[i][j], sum[i][j]);
+          ds[i][j] *= full[i][j];
+          dot2 = fmaf(ds[i][j], b[i][j], dot2);
         }
-      const float mean2 = a.post_weight ? row_sum<TPR>(dot2, slots, turn) / C : 0.f;
+      }
+    }
+    if constexpr (FULL) {
+      const float mean2 = a.post_weight ? row_sum<WAVES>(dot2, at.lanes, slots, turn) / C : 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (t + i * TPR) * kV;
+        const int c = column(i);
 #pragma unroll
         for (int j = 0; j < kV; ++j) ds[i][j] = rb * (ds[i][j] - b[i][j] * mean2);
         store(ds[i], static_cast<T*>(a.dbranch) + static_cast<int64_t>(row) * C + c, C - c);
       }
     }
   }
-  // this workgroup's column sums; with several rows in flight, one part a row of them
-  float* part = a.partial + (static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR) * 3 * C;
+  // this workgroup's column sums
+  float* part = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * C;
+  if constexpr (WAVES) {
+    // over the wave's rows, then over the four waves
+    const int n = at.lanes * kV, wave = threadIdx.x >> 6;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (t + i * TPR) * kV;
-    store(dw[i], part + c, C - c);
-    if constexpr (FULL) {
-      store(dpw[i], part + C + c, C - c);
-      store(dgate[i], part + 2 * C + c, C - c);
+    for (int j = 0; j < kV; ++j) {
+      for (int m = at.lanes; m < 64; m <<= 1) {
+        dw[0][j] += __shfl_xor(dw[0][j], m, 64);
+        if constexpr (FULL) sum[0][j] += __shfl_xor(sum[0][j], m, 64);
+      }
+      if ((threadIdx.x & 63) < at.lanes) {
+        sums[wave * 512 + at.t * kV + j] = dw[0][j];
+        if constexpr (FULL) sums[(4 + wave) * 512 + at.t * kV + j] = sum[0][j];
+      }
+    }
+    __syncthreads();
+    for (int v = 0; v < (FULL ? 2 : 1); ++v)
+      for (int c = threadIdx.x; c < n && c < C; c += 256) {
+        const float* x = sums + v * 4 * 512 + c;
+        part[v * C + c] = (x[0] + x[512]) + (x[1024] + x[1536]);
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = column(i);
+      store(dw[i], part + c, C - c);
+      if constexpr (FULL) store(sum[i], part + C + c, C - c);
     }
   }
 }
 
-// Column sums of the parts: 64 columns a workgroup, 16 threads a column.
+// Column sums of the parts: 16 columns a workgroup, 64 threads a column.
 template <class T> __global__ __launch_bounds__(1024) void add_norm_join_kernel(KgsAddNorm a) {
-  __shared__ float sums[16][64];
-  const int C = a.width, col = threadIdx.x & 63, group = threadIdx.x >> 6, c = blockIdx.x * 64 + col;
-  T* const to = static_cast<T*>(blockIdx.y == 0 ? a.dweight : blockIdx.y == 1 ? a.dpost_weight : a.dgate);
-  if (!to) return;
+  __shared__ float sums[64][16];
+  const int C = a.width, col = threadIdx.x & 15, group = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
   float sum = 0.f;
   if (c < C) {
     const float* p = a.partial + static_cast<int64_t>(blockIdx.y) * C + c;
 #pragma unroll 8
-    for (int i = group; i < a.parts; i += 16) sum += p[static_cast<int64_t>(i) * 3 * C];
+    for (int i = group; i < a.parts; i += 64) sum += p[static_cast<int64_t>(i) * 2 * C];
   }
   sums[group][col] = sum;
   __syncthreads();
   if (group == 0 && c < C) {
-    for (int i = 1; i < 16; ++i) sum += sums[i][col];
-    to[c] = static_cast<T>(sum);
+    sum = 0.f;
+    for (int i = 0; i < 64; ++i) sum += sums[i][col];
+    if (blockIdx.y == 0) {
+      static_cast<T*>(a.dweight)[c] = static_cast<T>(sum);
+    } else {
+      sum *= a.scale;
+      const float pw = a.post_weight ? static_cast<float>(static_cast<const T*>(a.post_weight)[c]) : 1.f;
+      const float gate = a.gate ? static_cast<float>(static_cast<const T*>(a.gate)[c]) : 1.f;
+      if (a.dpost_weight) static_cast<T*>(a.dpost_weight)[c] = static_cast<T>(sum * gate);
+      if (a.dgate) static_cast<T*>(a.dgate)[c] = static_cast<T>(sum * pw);
+    }
   }
 }
 
-template <class T, int TPR, int NV> int launch(const KgsAddNorm& a, bool back, hipStream_t s) {
-  constexpr int kRows = Shape<TPR>::kRows, kThreads = Shape<TPR>::kThreads;
-  const bool full = a.post_weight || a.gate || a.scale != 1.f;
-  if (!back) {
-    const int want = (a.rows + kRows - 1) / kRows, grid = want < 8192 ? want : 8192;
-    if (full) add_norm_fwd_kernel<T, TPR, NV, true><<<grid, kThreads, 0, s>>>(a);
-    else add_norm_fwd_kernel<T, TPR, NV, false><<<grid, kThreads, 0, s>>>(a);
-    return launched("add_norm forward");
-  }
-  // one part of the column sums a row of threads; the caller's partial has room for that
-  const int grid = a.parts / kRows;
-  if (grid < 1 || grid * kRows != a.parts) return fail("add_norm", "parts do not fit the rows of a workgroup");
-  if (full) add_norm_bwd_kernel<T, TPR, NV, true><<<grid, kThreads, 0, s>>>(a);
-  else add_norm_bwd_kernel<T, TPR, NV, false><<<grid, kThreads, 0, s>>>(a);
+bool is_full(const KgsAddNorm& a) { return a.post_weight || a.gate || a.scale != 1.f; }
+
+// Threads and rows a turn of a workgroup.
+template <bool WAVES, int NV> void shape(const KgsAddNorm& a, int& threads, int& rows) {
+  threads = WAVES ? 256 : (a.width + 64 * kV * NV - 1) / (64 * kV * NV) * 64;
+  rows = WAVES ? 256 / lanes_of_row(a.width) : 1;
+}
+
+template <class T, bool WAVES, int NV> int forward(const KgsAddNorm& a, hipStream_t s) {
+  int threads, rows;
+  shape<WAVES, NV>(a, threads, rows);
+  const int want = (a.rows + rows - 1) / rows, grid = want < 8192 ? want : 8192;
+  if (is_full(a)) add_norm_fwd_kernel<T, WAVES, NV, true><<<grid, threads, 0, s>>>(a);
+  else add_norm_fwd_kernel<T, WAVES, NV, false><<<grid, threads, 0, s>>>(a);
+  return launched("add_norm forward");
+}
+
+template <class T, bool WAVES, int NV, bool WHOLE> int backward(const KgsAddNorm& a, hipStream_t s) {
+  int threads, rows;
+  shape<WAVES, NV>(a, threads, rows);
+  if (is_full(a)) add_norm_bwd_kernel<T, WAVES, NV, true, WHOLE><<<a.parts, threads, 0, s>>>(a);
+  else add_norm_bwd_kernel<T, WAVES, NV, false, WHOLE><<<a.parts, threads, 0, s>>>(a);
   if (launched("add_norm backward")) return -1;
-  add_norm_join_kernel<T><<<dim3((a.width + 63) / 64, full ? 3 : 1), 1024, 0, s>>>(a);
+  const bool second = a.dpost_weight || a.dgate;
+  add_norm_join_kernel<T><<<dim3((a.width + 15) / 16, second ? 2 : 1), 1024, 0, s>>>(a);
   return launched("add_norm join");
 }
 
+template <class T, bool WAVES, int NV> int backward(const KgsAddNorm& a, hipStream_t s) {
+  return a.width % kV ? backward<T, WAVES, NV, false>(a, s) : backward<T, WAVES, NV, true>(a, s);
+}
+
 template <class T> int run(const KgsAddNorm& a, bool back, hipStream_t s) {
-  // At most 16 elements of a row a thread: the three column sums and the row fit the
-  // registers of four waves a SIMD.
-  if (a.width <= 512) return launch<T, 64, 1>(a, back, s);
-  if (a.width <= 2048) return launch<T, 256, 1>(a, back, s);
-  if (a.width <= 4096) return launch<T, 256, 2>(a, back, s);
-  if (a.width <= 8192) return launch<T, 512, 2>(a, back, s);
-  return launch<T, 1024, 2>(a, back, s);
+  if (a.width <= 512) return back ? backward<T, true, 1>(a, s) : forward<T, true, 1>(a, s);
+  if (a.width <= 8192 && back) return backward<T, false, 1>(a, s);
+  if (a.width <= 2048) return forward<T, false, 1>(a, s);
+  return back ? backward<T, false, 2>(a, s) : forward<T, false, 2>(a, s);
 }
 
 int dispatch(const KgsAddNorm* a, bool back, void* stream) {
@@ -280,7 +390,8 @@ int dispatch(const KgsAddNorm* a, bool back, void* stream) {
   if (!back && (!a->residual || !a->out)) return fail(w, "a tensor is missing");
   if (back && (!a->rstd || !a->dresidual || !a->dbranch || !a->dweight || !a->partial)) return fail(w, "a tensor is missing");
   if (back && ((a->post_weight && !a->dpost_weight) || (a->gate && !a->dgate))) return fail(w, "a tensor is missing");
-  if (a->rows <= 0 || a->width <= 0 || a->width > 16384) return fail(w, "bad sizes");
+  if (a->rows <= 0 || a->rows >= 1 << 30 || a->width <= 0 || a->width > 16384) return fail(w, "bad sizes");
+  if (back && (a->parts < 1 || a->parts > 65536)) return fail(w, "bad parts");
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->type) {
     case 0: return run<bf16>(*a, back, s);
