@@ -26,12 +26,14 @@ is launched.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import math
 import os
 import struct
+
+import torch
+from torch.autograd.function import once_differentiable
 
 from ..native import build as _build
 
@@ -59,42 +61,34 @@ _SWIGLU = struct.Struct("@9P3q4i3i3i")
 _ADD_NORM = struct.Struct("@16P5q4i2f")
 
 
-def _call(entry: str, args: bytes, device, stream) -> None:
-    import torch
-
-    s = stream if stream is not None else torch.cuda.current_stream(device)
-    if getattr(lib(), entry)(args, s.cuda_stream) != 0:
+def _call(entry: str, args: bytes, index: int) -> None:
+    # (the raw handle: a Stream object of torch.cuda.current_stream costs 2 us)
+    if getattr(_LIB or lib(), entry)(args, torch._C._cuda_getCurrentRawStream(index)) != 0:
         raise RuntimeError(lib().kgs_decoder_last_error().decode())
 
 
-@contextlib.contextmanager
-def _on(device, stream):
-    """Allocations and launches on the tensors' device and on ``stream``."""
-    import torch
-
-    with torch.cuda.device(device), torch.cuda.stream(stream):
-        yield
+def _here(t, stream) -> bool:
+    """Whether ``t``'s device and the wanted stream are the current ones."""
+    return stream is None and t.get_device() == torch.cuda.current_device()
 
 
-def _placed(device, stream):
-    import torch
-
-    if stream is None and device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    if stream is not None and stream.device != device:
-        raise ValueError(f"the stream is on {stream.device}, the tensors are on {device}")
-    return _on(device, stream)
+def _there(t, stream, call):
+    """``call()`` with ``t``'s device and ``stream`` current: allocations and launches belong there."""
+    if stream is not None and stream.device != t.device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors are on {t.device}")
+    with torch.cuda.device(t.device), torch.cuda.stream(stream):
+        return call()
 
 
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _type(t, name: str, allowed: str) -> int:
-    import torch
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
-    types = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-    code = types.get(t.dtype)
+
+def _type(t, name: str, allowed: str) -> int:
+    code = _TYPES.get(t.dtype)
     if code is None or code >= (3 if "float32" in allowed else 2):
         raise TypeError(f"{name} must be {allowed}, not {t.dtype}")
     return code
@@ -116,7 +110,7 @@ def _on_gpu(t, name: str) -> None:
 
 
 def _shape(t, name: str, want) -> None:
-    if tuple(t.shape) != tuple(want):
+    if t.shape != want:
         raise ValueError(f"{name} must have shape {tuple(want)}, not {tuple(t.shape)}")
 
 
@@ -125,50 +119,53 @@ def _shape(t, name: str, want) -> None:
 def _heads(t):
     """``t`` [B, S, heads, D] as the kernels read it, and its strides of (B, S, heads):
     D contiguous, positions apart, 16-byte rows.  Other layouts are copied."""
-    import torch
-
+    B, S, H, D = t.shape
+    b, s, h, d = t.stride()
     # A dimension of one may come with any stride; rows behind the last have to lie past it.
-    st = [t.shape[3] if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
-    if (t.stride(3) == 1 and t.shape[3] <= st[1] <= 1 << 22 and t.data_ptr() % 16 == 0
-            and not any(s % 8 for s in st)):
+    st = (b if B > 1 else D, s if S > 1 else D, h if H > 1 else D)
+    if d == 1 and D <= st[1] <= 1 << 22 and not (t.data_ptr() % 16 or (st[0] | st[1] | st[2]) % 8):
         return t, st
     t = t.clone(memory_format=torch.contiguous_format)
-    return t, list(t.stride()[:3])
+    return t, t.stride()[:3]
 
 
 def _attention_checks(q, k, v, scale, lengths, **more):
-    import torch
-
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         if t.dim() != 4:
             raise ValueError(f"{name} must be [batch, positions, heads, head dimension], not {tuple(t.shape)}")
     B, S, H, D = q.shape
     Hk = k.shape[2]
     code = _type(q, "q", "bfloat16 or float16")
-    _same(q, "q", k=k, v=v, **{n: t for n, t in more.items() if n not in ("lse", "low")})
-    _shape(k, "k", (B, S, Hk, D))
-    _shape(v, "v", (B, S, Hk, D))
-    for name, t in more.items():
-        _shape(t, name, (B, H, S) if name == "lse" else (B, S, H, D))
-    if D not in (64, 128):
+    dtype, device = q.dtype, q.device
+    if not (k.dtype == v.dtype == dtype and k.device == v.device == device):
+        _same(q, "q", k=k, v=v)
+    want = (B, S, Hk, D)
+    if k.shape != want or v.shape != want:
+        _shape(k, "k", want)
+        _shape(v, "v", want)
+    if more:
+        _same(q, "q", **{n: t for n, t in more.items() if n not in ("lse", "low")})
+        for name, t in more.items():
+            _shape(t, name, (B, H, S) if name == "lse" else (B, S, H, D))
+    if D != 128 and D != 64:
         raise ValueError(f"the head dimension must be 64 or 128, not {D}")
     if H == 0 or Hk == 0 or H % Hk:
         raise ValueError(f"{H} query heads cannot share {Hk} key heads")
     if S >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} positions, not {S}")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not (math.isfinite(scale) and scale > 0):
+    if not 0 < scale < math.inf:
         raise ValueError(f"scale must be finite and positive, not {scale}")
     if lengths is not None:
         if lengths.dtype != torch.int32:
             raise TypeError(f"lengths must be int32, not {lengths.dtype}")
         _shape(lengths, "lengths", (B,))
-        if lengths.device != q.device:
-            raise ValueError(f"lengths is on {lengths.device}, q is on {q.device}")
+        if lengths.device != device:
+            raise ValueError(f"lengths is on {lengths.device}, q is on {device}")
         lengths = lengths.contiguous()
-    if "lse" in more:
+    if more:
         for name, t in (("lse", torch.float32), ("low", torch.uint8)):
-            if more[name].dtype != t or not more[name].is_contiguous() or more[name].device != q.device:
+            if more[name].dtype != t or not more[name].is_contiguous() or more[name].device != device:
                 raise ValueError(f"{name} must be the {t} tensor that attention_fwd returned")
     _on_gpu(q, "q")
     return B, S, H, Hk, D, code, scale, lengths
@@ -188,10 +185,8 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, lengt
     A position that is masked by ``causal`` alone is multiplied by a zero probability, as in
     a plain matrix product: its v must be finite.
     """
-    import torch
-
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _functions()[0].apply(q, k, v, causal, scale, lengths)
+        return _Attention.apply(q, k, v, causal, scale, lengths)
     return _attention_fwd(q, k, v, causal, scale, lengths, None, False)[0]
 
 
@@ -199,11 +194,9 @@ def attention_qkv(qkv, heads: int, *, causal: bool = True, scale: float | None =
     """``attention`` of one projection's output [B, S, heads + 2 Hk, D], the query heads
     first, then the key heads, then the value heads; differentiable, with one gradient of
     the same layout (no gradients of views to be put together)."""
-    import torch
-
     q, k, v = _split_qkv(qkv, heads)
     if torch.is_grad_enabled() and qkv.requires_grad:
-        return _functions()[1].apply(qkv, heads, causal, scale, lengths)
+        return _AttentionQkv.apply(qkv, heads, causal, scale, lengths)
     return _attention_fwd(q, k, v, causal, scale, lengths, None, False)[0]
 
 
@@ -223,29 +216,24 @@ def attention_fwd(q, k, v, *, causal: bool = True, scale: float | None = None, l
 
 
 def _attention_fwd(q, k, v, causal, scale, lengths, stream, keep):
-    import torch
-
     B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths)
-    with _placed(q.device, stream):
-        (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
-        out = torch.empty(B, S, H, D, dtype=q.dtype, device=q.device)
-        lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device) if keep else None
-        low = torch.empty(B, S, H, D, dtype=torch.uint8, device=q.device) if keep else None
-        args = _ATTENTION.pack(_ptr(q), _ptr(k), _ptr(v), _ptr(out), 0, 0, 0, 0, _ptr(lse), 0, 0, _ptr(low), _ptr(lengths),
-                               *qs, *ks, *vs, S * H * D, H * D, D, *([0] * 12), B, S, H, Hk, D, code, int(causal), 1,
-                               scale)
-        if out.numel():
-            _call("kgs_attention_fwd", args, q.device, stream)
+    if not _here(q, stream):
+        return _there(q, stream, lambda: _attention_fwd(q, k, v, causal, scale, lengths, None, keep))
+    (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
+    out = q.new_empty((B, S, H, D))
+    lse = low = None
+    if keep:
+        lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device)
+        low = torch.empty(B, S, H, D, dtype=torch.uint8, device=q.device)
+    if B and S:
+        _call("kgs_attention_fwd",
+              _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, 0, 0, 0, _ptr(lse), 0, 0,
+                              _ptr(low), _ptr(lengths), *qs, *ks, *vs, S * H * D, H * D, D, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                              0, 0, B, S, H, Hk, D, code, bool(causal), 1, scale), q.get_device())
     return out, (lse, low) if keep else None
 
 
-WIDE = (int(os.environ.get("W0", "0")), int(os.environ.get("W1", "0")))
-
-
-def _attention_wide(B: int, S: int, H: int, Hk: int) -> tuple[int, int]:
-    return WIDE
-
-
+@functools.lru_cache(maxsize=4096)
 def _dkv_splits(B: int, S: int, H: int, Hk: int, causal: bool) -> int:
     """Parts that the walk over query rows is cut into for dk and dv: with fewer workgroups
     (one per 128 keys and key head) than the chip holds at once, two per CU, it is cut, as
@@ -264,24 +252,25 @@ def attention_bwd(dout, q, k, v, out, saved, *, causal: bool = True, scale: floa
 
 
 def _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, stream, into):
-    import torch
-
     B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths, dout=dout, out=out, lse=lse, low=low)
-    with _placed(q.device, stream):
-        (q, qs), (k, ks), (v, vs), (out, os_), (dout, gs) = _heads(q), _heads(k), _heads(v), _heads(out), _heads(dout)
-        if into is None:
-            into = [torch.empty(B, S, n, D, dtype=q.dtype, device=q.device) for n in (H, Hk, Hk)]
-        splits = _dkv_splits(B, S, H, Hk, causal)
-        # delta, then the parts of a split walk
-        parts = splits * 2 * B * S * Hk * D if splits > 1 else 0
-        rows = B * H * -(-S // 32) * 64
+    if not _here(q, stream):
+        return _there(q, stream, lambda: _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, None, into))
+    (q, qs), (k, ks), (v, vs), (out, os_), (dout, gs) = _heads(q), _heads(k), _heads(v), _heads(out), _heads(dout)
+    if into is None:
+        into = q.new_empty((B, S, H, D)), q.new_empty((B, S, Hk, D)), q.new_empty((B, S, Hk, D))
+    splits = _dkv_splits(B, S, H, Hk, bool(causal))
+    # delta, then the parts of a split walk
+    parts = splits * 2 * B * S * Hk * D if splits > 1 else 0
+    rows = B * H * -(-S // 32) * 64
+    if B and S:
         work = torch.empty(rows + parts, dtype=torch.float32, device=q.device)
-        st = [s for t in into for s in t.stride()[:3]]
-        args = _ATTENTION.pack(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(dout), *(_ptr(t) for t in into), _ptr(lse),
-                               _ptr(work), _ptr(work) + rows * 4 if parts else 0, _ptr(low), _ptr(lengths), *qs, *ks, *vs, *os_,
-                               *gs, *st, B, S, H, Hk, D, code, int(causal), splits, scale)
-        if q.numel():
-            _call("kgs_attention_bwd", args, q.device, stream)
+        at = work.data_ptr()
+        _call("kgs_attention_bwd",
+              _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(),
+                              *(t.data_ptr() for t in into), lse.data_ptr(), at, at + rows * 4 if parts else 0,
+                              low.data_ptr(), _ptr(lengths), *qs, *ks, *vs, *os_, *gs, *into[0].stride()[:3],
+                              *into[1].stride()[:3], *into[2].stride()[:3], B, S, H, Hk, D, code, bool(causal), splits,
+                              scale), q.get_device())
     return tuple(into)
 
 
@@ -290,30 +279,28 @@ def _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, stream,
 def _matrix(t):
     """``t`` [..., n] as rows the kernels read, and their stride: rows contiguous, apart, 16-byte
     aligned.  Other layouts are copied."""
-    import torch
-
     n = t.shape[-1]
-    m = t.reshape(-1, n)
-    ld = n if m.shape[0] == 1 else m.stride(0)
-    if m.stride(1) == 1 and n <= ld <= 1 << 21 and ld % 8 == 0 and m.data_ptr() % 16 == 0:
+    m = t if t.dim() == 2 else t.reshape(-1, n)
+    ld = m.stride(0) if m.shape[0] > 1 else n
+    if m.stride(1) == 1 and n <= ld <= 1 << 21 and not (ld % 8 or m.data_ptr() % 16):
         return m, ld
     return m.clone(memory_format=torch.contiguous_format), n
 
 
 def _swiglu_checks(x, w, **more):
-    import torch
-
     if x.dim() < 1 or w.dim() != 2:
         raise ValueError(f"x must be [..., width] and w [2 inner, width], not {tuple(x.shape)} and {tuple(w.shape)}")
     K, F = x.shape[-1], w.shape[0] // 2
     code = _type(x, "x", "bfloat16 or float16")
-    _same(x, "x", w=w, **{n: t for n, t in more.items() if n != "saved"})
-    _shape(w, "w", (2 * F, K))
+    if w.dtype != x.dtype or w.device != x.device or w.shape != (2 * F, K):
+        _same(x, "x", w=w)
+        _shape(w, "w", (2 * F, K))
     if K == 0 or F == 0 or K % 8 or F % 8 or K > 1 << 20 or F > 1 << 20:
         raise ValueError(f"width and inner must be multiples of 8, at most {1 << 20}, not {K} and {F}")
-    for name, t in more.items():
-        _shape(t, name, (*x.shape[:-1], F if name == "dh" else 6 * F))
-    if "saved" in more:
+    if more:
+        _same(x, "x", dh=more["dh"])
+        for name, t in more.items():
+            _shape(t, name, (*x.shape[:-1], F if name == "dh" else 6 * F))
         saved = more["saved"]
         if saved.dtype != torch.uint8 or not saved.is_contiguous() or saved.device != x.device:
             raise ValueError("saved must be the uint8 tensor that swiglu_fwd returned")
@@ -361,10 +348,8 @@ def swiglu(x, w):
     in place.  Returns [..., inner].  With a gradient wanted the two projections are kept
     for the backward pass, 24 bits of each value.
     """
-    import torch
-
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
-        return _functions()[2].apply(x, w)
+        return _Swiglu.apply(x, w)
     return _swiglu_fwd(x, w, None, False)[0]
 
 
@@ -375,19 +360,19 @@ def swiglu_fwd(x, w, *, stream=None):
 
 
 def _swiglu_fwd(x, w, stream, keep):
-    import torch
-
     T, K, F, code = _swiglu_checks(x, w)
-    with _placed(x.device, stream):
-        h = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
-        saved = torch.empty(*x.shape[:-1], 6 * F, dtype=torch.uint8, device=x.device) if keep else None
-        if T:
-            (x, x_ld), (w, w_ld) = _matrix(x), _matrix(w)
-            tile, splits = _product_plan(T, 2 * F, K)
-            part = torch.empty(splits * T * 2 * F, dtype=torch.float32, device=x.device) if splits > 1 else None
-            args = _SWIGLU.pack(_ptr(x), _ptr(w), _ptr(h), _ptr(saved), 0, 0, 0, 0, _ptr(part), x_ld, w_ld, 0, T, K, F,
-                                code, tile, 0, 0, splits, 1, 1)
-            _call("kgs_swiglu_fwd", args, x.device, stream)
+    if not _here(x, stream):
+        return _there(x, stream, lambda: _swiglu_fwd(x, w, None, keep))
+    lead = x.shape[:-1]
+    h = x.new_empty((*lead, F))
+    saved = torch.empty((*lead, 6 * F), dtype=torch.uint8, device=x.device) if keep else None
+    if T:
+        (x, x_ld), (w, w_ld) = _matrix(x), _matrix(w)
+        tile, splits = _product_plan(T, 2 * F, K)
+        part = torch.empty(splits * T * 2 * F, dtype=torch.float32, device=x.device) if splits > 1 else None
+        _call("kgs_swiglu_fwd",
+              _SWIGLU.pack(x.data_ptr(), w.data_ptr(), h.data_ptr(), _ptr(saved), 0, 0, 0, 0, _ptr(part), x_ld, w_ld, 0,
+                           T, K, F, code, tile, 0, 0, splits, 1, 1), x.get_device())
     return h, saved
 
 
@@ -397,25 +382,24 @@ def swiglu_bwd(dh, x, w, saved, *, stream=None):
 
 
 def _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, stream):
-    import torch
-
     T, K, F, code = _swiglu_checks(x, w, dh=dh, saved=saved)
-    with _placed(x.device, stream):
-        new = torch.empty if T else torch.zeros
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_dx else None
-        dw = new(w.shape, dtype=x.dtype, device=x.device) if want_dw else None
-        if T and (want_dx or want_dw):
-            (x, x_ld), (w, w_ld), (dh, dh_ld) = _matrix(x), _matrix(w), _matrix(dh)
-            if saved.data_ptr() % 16:
-                saved = saved.clone()
-            tx, sx = _product_plan(T, K, 2 * F)
-            tw, sw = _product_plan(2 * F, K, T)
-            size = max(sx * T * K if sx > 1 and want_dx else 0, sw * 2 * F * K if sw > 1 and want_dw else 0)
-            part = torch.empty(size, dtype=torch.float32, device=x.device) if size else None
-            dgu = torch.empty(T, 2 * F, dtype=x.dtype, device=x.device)
-            args = _SWIGLU.pack(_ptr(x), _ptr(w), 0, _ptr(saved), _ptr(dh), _ptr(dgu), _ptr(dx), _ptr(dw), _ptr(part),
-                                x_ld, w_ld, dh_ld, T, K, F, code, 0, tx, tw, 1, sx, sw)
-            _call("kgs_swiglu_bwd", args, x.device, stream)
+    if not _here(x, stream):
+        return _there(x, stream, lambda: _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, None))
+    dx = x.new_empty(x.shape) if want_dx else None
+    dw = (w.new_empty if T else w.new_zeros)(w.shape) if want_dw else None
+    if T and (want_dx or want_dw):
+        (x, x_ld), (w, w_ld), (dh, dh_ld) = _matrix(x), _matrix(w), _matrix(dh)
+        if saved.data_ptr() % 16:
+            saved = saved.clone()
+        tx, sx = _product_plan(T, K, 2 * F) if want_dx else (0, 1)
+        tw, sw = _product_plan(2 * F, K, T) if want_dw else (0, 1)
+        # one workspace for the parts: the products follow one another on the stream
+        size = max(sx * T * K if sx > 1 else 0, sw * 2 * F * K if sw > 1 else 0)
+        part = torch.empty(size, dtype=torch.float32, device=x.device) if size else None
+        dgu = x.new_empty((T, 2 * F))
+        _call("kgs_swiglu_bwd",
+              _SWIGLU.pack(x.data_ptr(), w.data_ptr(), 0, saved.data_ptr(), dh.data_ptr(), dgu.data_ptr(), _ptr(dx),
+                           _ptr(dw), _ptr(part), x_ld, w_ld, dh_ld, T, K, F, code, 0, tx, tw, 1, sx, sw), x.get_device())
     return dx, dw
 
 
@@ -426,9 +410,7 @@ MAX_NORM_WIDTH = 16384
 
 def _lines(t):
     """``t`` [..., C] as rows and their stride; rows that are not contiguous are copied."""
-    import torch
-
-    m = t.reshape(-1, t.shape[-1])
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
     if m.stride(1) != 1 and m.shape[1] > 1:
         m = m.clone(memory_format=torch.contiguous_format)
     return m, m.stride(0)
@@ -437,26 +419,32 @@ def _lines(t):
 def _add_norm_checks(first, name, weight, post_weight, gate, scale, eps, **rows):
     if first.dim() < 1:
         raise ValueError(f"{name} must be [..., width], not a single value")
-    C = first.shape[-1]
+    shape, dtype, device = first.shape, first.dtype, first.device
+    C = shape[-1]
     code = _type(first, name, "bfloat16, float16 or float32")
     for other, t in rows.items():
-        if t is not None:
-            _shape(t, other, first.shape)
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device):
+            _shape(t, other, shape)
+            _same(first, name, **{other: t})
     for other, t in (("weight", weight), ("post_weight", post_weight), ("gate", gate)):
-        if t is not None:
+        if t is not None and (t.shape != (C,) or t.dtype != dtype or t.device != device):
             _shape(t, other, (C,))
-    _same(first, name, weight=weight, post_weight=post_weight, gate=gate, **rows)
+            _same(first, name, **{other: t})
     if not 0 < C <= MAX_NORM_WIDTH:
         raise ValueError(f"the width must be 1 to {MAX_NORM_WIDTH}, not {C}")
     T = first.numel() // C
     if T >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} rows, not {T}")
-    if not math.isfinite(scale):
+    if not -math.inf < scale < math.inf:
         raise ValueError(f"scale must be finite, not {scale}")
-    if not (math.isfinite(eps) and eps >= 0):
+    if not 0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and not negative, not {eps}")
     _on_gpu(first, name)
     return T, C, code
+
+
+def _vector(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def add_norm(residual, branch, weight, *, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-6):
@@ -469,11 +457,9 @@ def add_norm(residual, branch, weight, *, post_weight=None, gate=None, scale: fl
     [..., C], weight, post_weight, gate [C], all of one type (bfloat16, float16, float32),
     C up to 16384, of any row stride.  Differentiable in all five tensors.
     """
-    import torch
-
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (residual, branch, weight, post_weight, gate)):
-        return _functions()[3].apply(residual, branch, weight, post_weight, gate, scale, eps)
+        return _AddNorm.apply(residual, branch, weight, post_weight, gate, scale, eps)
     return _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, False)[:2]
 
 
@@ -484,19 +470,19 @@ def add_norm_fwd(residual, branch, weight, *, post_weight=None, gate=None, scale
 
 
 def _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, keep):
-    import torch
-
     T, C, code = _add_norm_checks(residual, "residual", weight, post_weight, gate, scale, eps, branch=branch)
-    with _placed(residual.device, stream):
-        s = torch.empty(residual.shape, dtype=residual.dtype, device=residual.device)
-        out = torch.empty_like(s)
-        saved = torch.empty(2, T, dtype=torch.float32, device=residual.device) if keep else None
-        if T:
-            (r, r_ld), (b, b_ld) = _lines(residual), _lines(branch)
-            w, pw, g = (None if t is None else t.contiguous() for t in (weight, post_weight, gate))
-            args = _ADD_NORM.pack(_ptr(r), _ptr(b), _ptr(w), _ptr(pw), _ptr(g), _ptr(s), _ptr(out), _ptr(saved),
-                                  *([0] * 8), r_ld, b_ld, C, 0, 0, T, C, code, 0, scale, eps)
-            _call("kgs_add_norm_fwd", args, residual.device, stream)
+    if not _here(residual, stream):
+        return _there(residual, stream,
+                      lambda: _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, keep))
+    s, out = residual.new_empty(residual.shape), residual.new_empty(residual.shape)
+    saved = torch.empty(2, T, dtype=torch.float32, device=residual.device) if keep else None
+    if T:
+        (r, r_ld), (b, b_ld) = _lines(residual), _lines(branch)
+        w, pw, g = _vector(weight), _vector(post_weight), _vector(gate)
+        _call("kgs_add_norm_fwd",
+              _ADD_NORM.pack(r.data_ptr(), b.data_ptr(), w.data_ptr(), _ptr(pw), _ptr(g), s.data_ptr(), out.data_ptr(),
+                             _ptr(saved), 0, 0, 0, 0, 0, 0, 0, 0, r_ld, b_ld, C, 0, 0, T, C, code, 0, scale, eps),
+              r.get_device())
     return s, out, saved
 
 
@@ -517,113 +503,100 @@ def add_norm_bwd(dstream, dout, stream_, branch, weight, saved, *, post_weight=N
     its two results (either may be None: zero), its stream ``stream_``, and ``saved`` of
     ``add_norm_fwd`` with the same keywords.  Without post_weight, gate and scale dbranch is
     dresidual, the same tensor; gradients of absent weights are None."""
-    import torch
-
     if dstream is None and dout is None:
         raise ValueError("one of dstream and dout must be given")
     T, C, code = _add_norm_checks(stream_, "stream_", weight, post_weight, gate, scale, eps, dstream=dstream, dout=dout,
                                   branch=branch)
-    if saved.dtype != torch.float32 or tuple(saved.shape) != (2, T) or not saved.is_contiguous():
+    if saved.dtype != torch.float32 or saved.shape != (2, T) or not saved.is_contiguous():
         raise ValueError("saved must be the float32 tensor that add_norm_fwd returned")
     if saved.device != stream_.device:
         raise ValueError(f"saved is on {saved.device}, stream_ is on {stream_.device}")
-    with _placed(stream_.device, stream):
-        def new(like, zero=False):
-            return (torch.zeros if zero else torch.empty)(like.shape, dtype=like.dtype, device=like.device)
-
-        full = post_weight is not None or gate is not None or scale != 1.0
-        dr = new(stream_)
-        db = new(stream_) if full else dr
-        grads = [None if t is None else new(t, zero=not T) for t in (weight, post_weight, gate)]
-        if T:
-            (s, s_ld), (b, b_ld) = _lines(stream_), _lines(branch)
-            (ds, ds_ld), (dy, dy_ld) = (_lines(t) if t is not None else (None, 0) for t in (dstream, dout))
-            w, pw, g = (None if t is None else t.contiguous() for t in (weight, post_weight, gate))
-            parts = _norm_parts(T, C)
-            work = torch.empty(parts * 2 * C, dtype=torch.float32, device=s.device)
-            args = _ADD_NORM.pack(0, _ptr(b), _ptr(w), _ptr(pw), _ptr(g), _ptr(s), 0, _ptr(saved), _ptr(ds), _ptr(dy),
-                                  _ptr(dr), _ptr(db), *(_ptr(t) for t in grads), _ptr(work), 0, b_ld, s_ld, ds_ld, dy_ld,
-                                  T, C, code, parts, scale, eps)
-            _call("kgs_add_norm_bwd", args, s.device, stream)
-    return dr, db, *grads
+    if not _here(stream_, stream):
+        return _there(stream_, stream, lambda: add_norm_bwd(dstream, dout, stream_, branch, weight, saved, eps=eps,
+                                                            post_weight=post_weight, gate=gate, scale=scale))
+    dr = stream_.new_empty(stream_.shape)
+    db = stream_.new_empty(stream_.shape) if post_weight is not None or gate is not None or scale != 1.0 else dr
+    new = weight.new_empty if T else weight.new_zeros
+    dw, dpw, dg = new((C,)), new((C,)) if post_weight is not None else None, new((C,)) if gate is not None else None
+    if T:
+        (s, s_ld), (b, b_ld) = _lines(stream_), _lines(branch)
+        ds, ds_ld = _lines(dstream) if dstream is not None else (None, 0)
+        dy, dy_ld = _lines(dout) if dout is not None else (None, 0)
+        w, pw, g = _vector(weight), _vector(post_weight), _vector(gate)
+        parts = _norm_parts(T, C)
+        work = torch.empty(parts * 2 * C, dtype=torch.float32, device=s.device)
+        _call("kgs_add_norm_bwd",
+              _ADD_NORM.pack(0, b.data_ptr(), w.data_ptr(), _ptr(pw), _ptr(g), s.data_ptr(), 0, saved.data_ptr(),
+                             _ptr(ds), _ptr(dy), dr.data_ptr(), db.data_ptr(), dw.data_ptr(), _ptr(dpw), _ptr(dg),
+                             work.data_ptr(), 0, b_ld, s_ld, ds_ld, dy_ld, T, C, code, parts, scale, eps), s.get_device())
+    return dr, db, dw, dpw, dg
 
 
 # ---------------------------------------------------------------------------- autograd
 
-_FUNCTIONS = None
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, causal, scale, lengths):
+        out, saved = _attention_fwd(q, k, v, causal, scale, lengths, None, True)
+        ctx.save_for_backward(q, k, v, out, *saved, lengths)
+        ctx.options = causal, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, low, lengths = ctx.saved_tensors
+        grads = _attention_bwd(dout, q, k, v, out, lse, low, *ctx.options, lengths, None, None)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
 
 
-def _functions():
-    """The autograd functions, made on first use (importing this module needs no torch)."""
-    global _FUNCTIONS
-    if _FUNCTIONS is not None:
-        return _FUNCTIONS
-    import torch
-    from torch.autograd.function import once_differentiable
+class _AttentionQkv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, heads, causal, scale, lengths):
+        out, saved = _attention_fwd(*_split_qkv(qkv, heads), causal, scale, lengths, None, True)
+        ctx.save_for_backward(qkv, out, *saved, lengths)
+        ctx.options = heads, causal, scale
+        return out
 
-    class Attention(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, q, k, v, causal, scale, lengths):
-            out, saved = _attention_fwd(q, k, v, causal, scale, lengths, None, True)
-            ctx.save_for_backward(q, k, v, out, *saved, lengths)
-            ctx.options = causal, scale
-            return out
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        qkv, out, lse, low, lengths = ctx.saved_tensors
+        heads, causal, scale = ctx.options
+        grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _attention_bwd(dout, *_split_qkv(qkv, heads), out, lse, low, causal, scale, lengths, None,
+                       _split_qkv(grad, heads))
+        return grad, None, None, None, None
 
-        @staticmethod
-        @once_differentiable
-        def backward(ctx, dout):
-            q, k, v, out, lse, low, lengths = ctx.saved_tensors
-            grads = _attention_bwd(dout, q, k, v, out, lse, low, *ctx.options, lengths, None, None)
-            return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None, None)
 
-    class AttentionQkv(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, qkv, heads, causal, scale, lengths):
-            out, saved = _attention_fwd(*_split_qkv(qkv, heads), causal, scale, lengths, None, True)
-            ctx.save_for_backward(qkv, out, *saved, lengths)
-            ctx.options = heads, causal, scale
-            return out
+class _Swiglu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w):
+        h, saved = _swiglu_fwd(x, w, None, True)
+        ctx.save_for_backward(x, w, saved)
+        return h
 
-        @staticmethod
-        @once_differentiable
-        def backward(ctx, dout):
-            qkv, out, lse, low, lengths = ctx.saved_tensors
-            heads, causal, scale = ctx.options
-            grad = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-            _attention_bwd(dout, *_split_qkv(qkv, heads), out, lse, low, causal, scale, lengths, None,
-                           _split_qkv(grad, heads))
-            return grad, None, None, None, None
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        return _swiglu_bwd(dh, *ctx.saved_tensors, *ctx.needs_input_grad, None)
 
-    class Swiglu(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, x, w):
-            h, saved = _swiglu_fwd(x, w, None, True)
-            ctx.save_for_backward(x, w, saved)
-            return h
 
-        @staticmethod
-        @once_differentiable
-        def backward(ctx, dh):
-            return _swiglu_bwd(dh, *ctx.saved_tensors, *ctx.needs_input_grad, None)
+class _AddNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, residual, branch, weight, post_weight, gate, scale, eps):
+        stream, out, saved = _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, True)
+        ctx.save_for_backward(stream, branch, weight, saved, post_weight, gate)
+        ctx.options = scale, eps
+        ctx.set_materialize_grads(False)
+        return stream, out
 
-    class AddNorm(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, residual, branch, weight, post_weight, gate, scale, eps):
-            stream, out, saved = _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, True)
-            ctx.save_for_backward(stream, branch, weight, saved, post_weight, gate)
-            ctx.options = scale, eps
-            ctx.set_materialize_grads(False)
-            return stream, out
-
-        @staticmethod
-        @once_differentiable
-        def backward(ctx, dstream, dout):
-            if dstream is None and dout is None:
-                return (None,) * 7
-            stream, branch, weight, saved, post_weight, gate = ctx.saved_tensors
-            grads = add_norm_bwd(dstream, dout, stream, branch, weight, saved, post_weight=post_weight, gate=gate,
-                                 scale=ctx.options[0], eps=ctx.options[1])
-            return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)
-
-    _FUNCTIONS = Attention, AttentionQkv, Swiglu, AddNorm
-    return _FUNCTIONS
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dstream, dout):
+        if dstream is None and dout is None:
+            return (None,) * 7
+        stream, branch, weight, saved, post_weight, gate = ctx.saved_tensors
+        grads = add_norm_bwd(dstream, dout, stream, branch, weight, saved, post_weight=post_weight, gate=gate,
+                             scale=ctx.options[0], eps=ctx.options[1])
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)
