@@ -311,28 +311,37 @@ def _swiglu_checks(x, w, **more):
     return T, K, F, code
 
 
-PRODUCT_TILES = (0, 1)  # the tiles of swiglu.hip's product: 128 x 128, 256 x 256
+# The tiles of swiglu.hip's product, rows by columns: 128 x 128, 256 x 256, and for the
+# forward pass of up to 32 rows 32 x 256.
+PRODUCT_TILES = (0, 1, 2)
 
 
 @functools.lru_cache(maxsize=4096)
-def _product_plan(M: int, N: int, K: int) -> tuple[int, int]:
+def _product_plan(M: int, N: int, K: int, forward: bool = False) -> tuple[int, int]:
     """(tile, splits) of an [M, N] product over K: the least of the times expected, from what
     the tiles were measured at.  A step of 64 of the sum takes all workgroups that run at
     once 1.83 us with the 256 x 256 tile (one a CU), 1.10 us with 128 x 128 (two a CU; 0.74
-    us if there is no more than one); a round of workgroups has a start and an end of its
-    own; the parts of a split sum are written and read as 32-bit numbers, at 4 TB/s, by
-    one more launch.  (2048 x 10752 over 2048: 115 us with 256 x 256, two rounds of which
-    the second is a third full, and 103 us with 128 x 128; 8192 x 22016 over 4096: 1290 us
-    and 1550 us.)"""
+    us if there is no more than one); with 32 x 256 it is the time of reading the weights,
+    5.2 TB/s.  A round of workgroups has a start and an end of its own; the parts of a
+    split sum are written and read as 32-bit numbers, at 4 TB/s, by one more launch; no
+    plan is faster than reading and writing the operands once.  (2048 x 10752 over 2048:
+    115 us with 256 x 256, two rounds of which the second is a third full, and 103 us with
+    128 x 128; 8192 x 22016 over 4096: 1290 us and 1550 us; 5 x 22016 over 4096, weights
+    from memory: 37 us with 32 x 256 in 4 parts, 44 us with 128 x 128.)"""
+    floor = 2 * (M * K + N * K + M * N) / 5.2e6
     best = None
-    for tile, size, at_once in ((0, 128, 512), (1, 256, 256)):
-        blocks = -(-M // size) * -(-N // size)
+    for tile, rows, columns, at_once, around in ((0, 128, 128, 512, 3.5), (1, 256, 256, 256, 8.0), (2, 32, 256, 512, 3.5)):
+        if tile == 2 and not (forward and M <= 32):
+            continue
+        blocks = -(-M // rows) * -(-N // columns)
         for splits in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16):
             steps = -(-K // 64 // splits)
-            if splits > 1 and steps < 8:
+            if splits > 1 and steps < 4:
                 break
-            step = 1.83 if tile else 1.10 if blocks * splits > 256 else 0.74
-            time = -(-blocks * splits // at_once) * (steps * step + (8 if tile else 3.5))
+            step = (1.10 if blocks * splits > 256 else 0.74, 1.83, 1.5)[tile]
+            # a step's columns come from memory once, however many row tiles share them
+            step = max(step, min(blocks * splits, at_once) / -(-M // rows) * columns * 128 / 5.2e6)
+            time = max(floor, -(-blocks * splits // at_once) * (steps * step + around))
             if splits > 1:
                 time += 4 + 2 * splits * M * N * 4 / 4e6
             if best is None or time < best[0]:
@@ -368,7 +377,7 @@ def _swiglu_fwd(x, w, stream, keep):
     saved = torch.empty((*lead, 6 * F), dtype=torch.uint8, device=x.device) if keep else None
     if T:
         (x, x_ld), (w, w_ld) = _matrix(x), _matrix(w)
-        tile, splits = _product_plan(T, 2 * F, K)
+        tile, splits = _product_plan(T, 2 * F, K, True)
         part = torch.empty(splits * T * 2 * F, dtype=torch.float32, device=x.device) if splits > 1 else None
         _call("kgs_swiglu_fwd",
               _SWIGLU.pack(x.data_ptr(), w.data_ptr(), h.data_ptr(), _ptr(saved), 0, 0, 0, 0, _ptr(part), x_ld, w_ld, 0,
@@ -497,38 +506,37 @@ def _norm_parts(T: int, C: int) -> int:
     return min(T, 256 * (16 // waves))
 
 
-def add_norm_bwd(dstream, dout, stream_, branch, weight, saved, *, post_weight=None, gate=None, scale: float = 1.0,
+def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=None, gate=None, scale: float = 1.0,
                  eps: float = 1e-6, stream=None):
     """(dresidual, dbranch, dweight, dpost_weight, dgate) of ``add_norm`` from the gradients of
-    its two results (either may be None: zero), its stream ``stream_``, and ``saved`` of
-    ``add_norm_fwd`` with the same keywords.  Without post_weight, gate and scale dbranch is
+    its two results (either may be None: zero), its arguments, and ``saved`` of ``add_norm_fwd``.  Without post_weight, gate and scale dbranch is
     dresidual, the same tensor; gradients of absent weights are None."""
     if dstream is None and dout is None:
         raise ValueError("one of dstream and dout must be given")
-    T, C, code = _add_norm_checks(stream_, "stream_", weight, post_weight, gate, scale, eps, dstream=dstream, dout=dout,
+    T, C, code = _add_norm_checks(residual, "residual", weight, post_weight, gate, scale, eps, dstream=dstream, dout=dout,
                                   branch=branch)
     if saved.dtype != torch.float32 or saved.shape != (2, T) or not saved.is_contiguous():
         raise ValueError("saved must be the float32 tensor that add_norm_fwd returned")
-    if saved.device != stream_.device:
-        raise ValueError(f"saved is on {saved.device}, stream_ is on {stream_.device}")
-    if not _here(stream_, stream):
-        return _there(stream_, stream, lambda: add_norm_bwd(dstream, dout, stream_, branch, weight, saved, eps=eps,
+    if saved.device != residual.device:
+        raise ValueError(f"saved is on {saved.device}, residual is on {residual.device}")
+    if not _here(residual, stream):
+        return _there(residual, stream, lambda: add_norm_bwd(dstream, dout, residual, branch, weight, saved, eps=eps,
                                                             post_weight=post_weight, gate=gate, scale=scale))
-    dr = stream_.new_empty(stream_.shape)
-    db = stream_.new_empty(stream_.shape) if post_weight is not None or gate is not None or scale != 1.0 else dr
+    dr = residual.new_empty(residual.shape)
+    db = residual.new_empty(residual.shape) if post_weight is not None or gate is not None or scale != 1.0 else dr
     new = weight.new_empty if T else weight.new_zeros
     dw, dpw, dg = new((C,)), new((C,)) if post_weight is not None else None, new((C,)) if gate is not None else None
     if T:
-        (s, s_ld), (b, b_ld) = _lines(stream_), _lines(branch)
+        (r, r_ld), (b, b_ld) = _lines(residual), _lines(branch)
         ds, ds_ld = _lines(dstream) if dstream is not None else (None, 0)
         dy, dy_ld = _lines(dout) if dout is not None else (None, 0)
         w, pw, g = _vector(weight), _vector(post_weight), _vector(gate)
         parts = _norm_parts(T, C)
-        work = torch.empty(parts * 2 * C, dtype=torch.float32, device=s.device)
+        work = torch.empty(parts * 2 * C, dtype=torch.float32, device=r.device)
         _call("kgs_add_norm_bwd",
-              _ADD_NORM.pack(0, b.data_ptr(), w.data_ptr(), _ptr(pw), _ptr(g), s.data_ptr(), 0, saved.data_ptr(),
+              _ADD_NORM.pack(r.data_ptr(), b.data_ptr(), w.data_ptr(), _ptr(pw), _ptr(g), 0, 0, saved.data_ptr(),
                              _ptr(ds), _ptr(dy), dr.data_ptr(), db.data_ptr(), dw.data_ptr(), _ptr(dpw), _ptr(dg),
-                             work.data_ptr(), 0, b_ld, s_ld, ds_ld, dy_ld, T, C, code, parts, scale, eps), s.get_device())
+                             work.data_ptr(), r_ld, b_ld, 0, ds_ld, dy_ld, T, C, code, parts, scale, eps), r.get_device())
     return dr, db, dw, dpw, dg
 
 
@@ -586,7 +594,7 @@ class _AddNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, residual, branch, weight, post_weight, gate, scale, eps):
         stream, out, saved = _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, True)
-        ctx.save_for_backward(stream, branch, weight, saved, post_weight, gate)
+        ctx.save_for_backward(residual, branch, weight, saved, post_weight, gate)
         ctx.options = scale, eps
         ctx.set_materialize_grads(False)
         return stream, out
@@ -596,7 +604,7 @@ class _AddNorm(torch.autograd.Function):
     def backward(ctx, dstream, dout):
         if dstream is None and dout is None:
             return (None,) * 7
-        stream, branch, weight, saved, post_weight, gate = ctx.saved_tensors
-        grads = add_norm_bwd(dstream, dout, stream, branch, weight, saved, post_weight=post_weight, gate=gate,
+        residual, branch, weight, saved, post_weight, gate = ctx.saved_tensors
+        grads = add_norm_bwd(dstream, dout, residual, branch, weight, saved, post_weight=post_weight, gate=gate,
                              scale=ctx.options[0], eps=ctx.options[1])
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), None, None)

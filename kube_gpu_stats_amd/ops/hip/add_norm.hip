@@ -14,8 +14,10 @@
 // adds its columns in registers over its rows, the workgroups' sums are joined by a
 // second kernel in a fixed order (no atomics, so equal calls give equal bits).
 //
-// Everything is computed in 32 bits and rounded once, as an output.  The forward
-// normalises the unrounded stream; the backward sees it as it was stored.
+// Everything is computed in 32 bits and rounded once, as an output.  Both passes use the
+// unrounded stream: the backward adds it up again from residual and branch.  (The stored
+// one would save it a read where there are no post_weight, gate and scale, but add half
+// as much error again to dweight.)
 #include "decoder.h"
 #include "decoder_common.h"
 
@@ -175,8 +177,8 @@ __global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_fwd_kernel(KgsAdd
 // and read the weights again for every row.  WHOLE: the width is a multiple of 8, so that
 // a chunk is there or not: a thread past the end reads the row's first chunk, without a
 // branch, and its zero weights keep it out of the sums.
-template <class T, bool WAVES, int NV, bool FULL, bool WHOLE>
-__global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_bwd_kernel(KgsAddNorm a) {
+template <class T, bool WAVES, int NV, bool FULL, bool WHOLE, int THREADS>
+__global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
   __shared__ float slots[2 * 16];
   __shared__ float sums[WAVES ? (FULL ? 2 : 1) * 4 * 512 : 1];
   constexpr bool kAhead = NV == 1;
@@ -188,6 +190,20 @@ __global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_bwd_kernel(KgsAdd
     const T* from = static_cast<const T*>(p) + start;
     if constexpr (WHOLE) r = *reinterpret_cast<const Loose<T>*>(from + (c < C ? c : 0));
     else load_raw(r, from, c, C - c);
+  };
+  // For residual and branch: last read by the forward pass, they are not in a cache, and
+  // are not kept in one (8192 x 4096: 69 us to 61 us, all weights 88 us to 75 us; with the
+  // gradients read so too, which the pass before has just written, 47 us for 45 us at a
+  // size that the caches hold).
+  const auto get_once = [&](Loose<T>& r, const void* p, int64_t start, int c) {
+    if constexpr (WHOLE) {
+      typedef T V8 __attribute__((ext_vector_type(kV), aligned(sizeof(T))));
+      const V8 x = __builtin_nontemporal_load(reinterpret_cast<const V8*>(static_cast<const T*>(p) + start + (c < C ? c : 0)));
+#pragma unroll
+      for (int j = 0; j < kV; ++j) r.v[j] = x[j];
+    } else {
+      get(r, p, start, c);
+    }
   };
   // weight, and scale post_weight gate; zero past the end
   float w[NV][kV], full[FULL ? NV : 1][kV];
@@ -215,7 +231,7 @@ __global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_bwd_kernel(KgsAdd
   };
   if (kAhead) weights();
   struct Row {
-    Loose<T> s[NV], dy[NV], ds[NV], b[FULL ? NV : 1];
+    Loose<T> s[NV], dy[NV], ds[NV], b[NV];
     float rs, rb;
   } next;
   const auto fetch = [&](int row) {
@@ -223,10 +239,10 @@ __global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_bwd_kernel(KgsAdd
     next.rb = FULL ? a.rstd[a.rows + row] : 1.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      get(next.s[i], a.stream, row * a.stream_ld, column(i));
+      get_once(next.s[i], a.residual, row * a.residual_ld, column(i));
+      get_once(next.b[i], a.branch, row * a.branch_ld, column(i));
       if (a.dout) get(next.dy[i], a.dout, row * a.dout_ld, column(i));
       if (a.dstream) get(next.ds[i], a.dstream, row * a.dstream_ld, column(i));
-      if constexpr (FULL) get(next.b[i], a.branch, row * a.branch_ld, column(i));
     }
   };
 #pragma unroll
@@ -250,9 +266,14 @@ __global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_bwd_kernel(KgsAdd
 #pragma unroll
       for (int j = 0; j < kV; ++j) {
         const float g = static_cast<float>(next.dy[i].v[j]);
-        s[i][j] = static_cast<float>(next.s[i].v[j]) * rs;
         ds[i][j] = static_cast<float>(next.ds[i].v[j]);
-        if constexpr (FULL) b[i][j] = static_cast<float>(next.b[i].v[j]) * rb;
+        const float r = static_cast<float>(next.s[i].v[j]), x = static_cast<float>(next.b[i].v[j]);
+        if constexpr (FULL) {
+          b[i][j] = x * rb;
+          s[i][j] = fmaf(full[i][j], b[i][j], r) * rs;
+        } else {
+          s[i][j] = (r + x) * rs;
+        }
         dw[i][j] = fmaf(g, s[i][j], dw[i][j]);
         dy[i][j] = g * w[i][j];
         dot = fmaf(dy[i][j], s[i][j], dot);
@@ -362,32 +383,35 @@ template <class T, bool WAVES, int NV> int forward(const KgsAddNorm& a, hipStrea
   return launched("add_norm forward");
 }
 
-template <class T, bool WAVES, int NV, bool WHOLE> int backward(const KgsAddNorm& a, hipStream_t s) {
+template <class T, bool WAVES, int NV, bool WHOLE, int THREADS> int backward(const KgsAddNorm& a, hipStream_t s) {
   int threads, rows;
   shape<WAVES, NV>(a, threads, rows);
-  if (is_full(a)) add_norm_bwd_kernel<T, WAVES, NV, true, WHOLE><<<a.parts, threads, 0, s>>>(a);
-  else add_norm_bwd_kernel<T, WAVES, NV, false, WHOLE><<<a.parts, threads, 0, s>>>(a);
+  if (is_full(a)) add_norm_bwd_kernel<T, WAVES, NV, true, WHOLE, THREADS><<<a.parts, threads, 0, s>>>(a);
+  else add_norm_bwd_kernel<T, WAVES, NV, false, WHOLE, THREADS><<<a.parts, threads, 0, s>>>(a);
   if (launched("add_norm backward")) return -1;
   const bool second = a.dpost_weight || a.dgate;
   add_norm_join_kernel<T><<<dim3((a.width + 15) / 16, second ? 2 : 1), 1024, 0, s>>>(a);
   return launched("add_norm join");
 }
 
-template <class T, bool WAVES, int NV> int backward(const KgsAddNorm& a, hipStream_t s) {
-  return a.width % kV ? backward<T, WAVES, NV, false>(a, s) : backward<T, WAVES, NV, true>(a, s);
+template <class T, bool WAVES, int NV, int THREADS> int backward(const KgsAddNorm& a, hipStream_t s) {
+  return a.width % kV ? backward<T, WAVES, NV, false, THREADS>(a, s) : backward<T, WAVES, NV, true, THREADS>(a, s);
 }
 
 template <class T> int run(const KgsAddNorm& a, bool back, hipStream_t s) {
-  if (a.width <= 512) return back ? backward<T, true, 1>(a, s) : forward<T, true, 1>(a, s);
-  if (a.width <= 8192 && back) return backward<T, false, 1>(a, s);
-  if (a.width <= 2048) return forward<T, false, 1>(a, s);
-  return back ? backward<T, false, 2>(a, s) : forward<T, false, 2>(a, s);
+  if (a.width <= 512) return back ? backward<T, true, 1, 256>(a, s) : forward<T, true, 1>(a, s);
+  // (forward of 16384 x 8192 with all weights: 197 us with one chunk a thread, 227 us with two)
+  if (!back) return a.width <= 8192 ? forward<T, false, 1>(a, s) : forward<T, false, 2>(a, s);
+  if (a.width <= 8192) return backward<T, false, 1, 1024>(a, s);
+  // two chunks a thread need more than the 128 registers of 16 waves, and have them with 12
+  if (a.width <= 12288) return backward<T, false, 2, 768>(a, s);
+  return backward<T, false, 2, 1024>(a, s);
 }
 
 int dispatch(const KgsAddNorm* a, bool back, void* stream) {
   const char* w = "add_norm";
-  if (!a || !a->branch || !a->weight || !a->stream) return fail(w, "a tensor is missing");
-  if (!back && (!a->residual || !a->out)) return fail(w, "a tensor is missing");
+  if (!a || !a->residual || !a->branch || !a->weight) return fail(w, "a tensor is missing");
+  if (!back && (!a->stream || !a->out)) return fail(w, "a tensor is missing");
   if (back && (!a->rstd || !a->dresidual || !a->dbranch || !a->dweight || !a->partial)) return fail(w, "a tensor is missing");
   if (back && ((a->post_weight && !a->dpost_weight) || (a->gate && !a->dgate))) return fail(w, "a tensor is missing");
   if (a->rows <= 0 || a->rows >= 1 << 30 || a->width <= 0 || a->width > 16384) return fail(w, "bad sizes");

@@ -302,13 +302,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
     }
     delta += other_half(delta);
   }
-  const int64_t stat = (static_cast<int64_t>(b) * a.H + h) * a.S + row;
-  const float lse = row < n ? a.lse[stat] : 0.f;
-  // For dk, dv: the 32 rows' lse, then their delta, side by side.  Rows past the end get
-  // zeros: with zeros for q and do they are p = 1 times zero there.
-  const int groups = (a.S + 31) / 32, group = qw / 32;
-  if (group < groups)
-    a.delta[(static_cast<int64_t>(b * a.H + h) * groups + group) * 64 + lane] = lane < 32 ? lse : delta;
+  const float lse = row < n ? a.lse[(static_cast<int64_t>(b) * a.H + h) * a.S + row] : 0.f;
 
   const int end = CAUSAL ? min(n, q0 + kRows) : n;
   const int limit = CAUSAL ? min(row + 1, n) : n;
@@ -346,25 +340,42 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
     const char* vt = kt + kTile;
     slot = slot == NS - 1 ? 0 : slot + 1;
     if (s0 >= last) continue;
+    // s and do.v of 32 keys
+    const auto scores = [&](int t, f32x16& s, f32x16& dp) {
+      s = dp = f32x16{};
+      typename E::x8 f[2][2];
+      auto read = [&](int kk) {
+        f[kk & 1][0] = Tl::template rows<T>(kt, t * 32, kk, lane);
+        f[kk & 1][1] = Tl::template rows<T>(vt, t * 32, kk, lane);
+      };
+      read(0);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        if (kk + 1 < D / 16) read(kk + 1);
+        in_order();
+        s = E::mfma(f[kk & 1][0], q[kk], s);
+        dp = E::mfma(f[kk & 1][1], g[kk], dp);
+        in_order();
+      }
+    };
+    if (last <= kStep) {
+      // The only step of these rows: delta as sum p (do.v).  Few keys have large p, whose
+      // rounding in the forward pass would show in delta = do.o.
+      delta = 0.f;
+#pragma unroll 1
+      for (int t = 0; t < 2; ++t) {
+        f32x16 s, dp;
+        scores(t, s, dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          delta += s0 + t * 32 + acc_row(r, lane) < limit ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * dp[r] : 0.f;
+      }
+      delta += other_half(delta);
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      f32x16 s = {}, dp = {};
-      {
-        typename E::x8 f[2][2];
-        auto read = [&](int kk) {
-          f[kk & 1][0] = Tl::template rows<T>(kt, t * 32, kk, lane);
-          f[kk & 1][1] = Tl::template rows<T>(vt, t * 32, kk, lane);
-        };
-        read(0);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          if (kk + 1 < D / 16) read(kk + 1);
-          in_order();
-          s = E::mfma(f[kk & 1][0], q[kk], s);
-          dp = E::mfma(f[kk & 1][1], g[kk], dp);
-          in_order();
-        }
-      }
+      f32x16 s, dp;
+      scores(t, s, dp);
       const bool edge = s0 + t * 32 + 32 > open;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -388,6 +399,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   }
   copies_done();
   barrier();
+  // For dk, dv: the 32 rows' lse, then their delta, side by side.  Rows past the end get
+  // zeros: with zeros for q and do they are p = 1 times zero there.
+  const int groups = (a.S + 31) / 32, group = qw / 32;
+  if (group < groups)
+    a.delta[(static_cast<int64_t>(b * a.H + h) * groups + group) * 64 + lane] =
+        row >= n ? 0.f : lane < 32 ? lse : delta;
   if (row >= n)
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) acc[t] = f32x16{};

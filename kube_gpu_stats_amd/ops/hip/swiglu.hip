@@ -371,6 +371,8 @@ template <class T, bool TA, bool TB, bool PAIR> int product(const Product& p, in
   switch (tile) {
     case 0: return product_tiled<T, 128, 128, 2, 2, TA, TB, PAIR>(p, s);
     case 1: return product_tiled<T, 256, 256, 2, 4, TA, TB, PAIR>(p, s);
+    case 2:  // few rows, forward
+      if constexpr (PAIR) return product_tiled<T, 32, 256, 1, 4, TA, TB, PAIR>(p, s);
   }
   return fail("swiglu", "unknown tile");
 }
