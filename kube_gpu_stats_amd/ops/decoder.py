@@ -95,13 +95,21 @@ def _type(t, name: str, allowed: str) -> int:
 
 
 def _same(first, name: str, **others) -> None:
+    dtype, index = first.dtype, first.get_device()
     for other, t in others.items():
         if t is None:
             continue
-        if t.dtype != first.dtype:
-            raise TypeError(f"{other} is {t.dtype}, {name} is {first.dtype}")
-        if t.device != first.device:
+        if t.dtype != dtype:
+            raise TypeError(f"{other} is {t.dtype}, {name} is {dtype}")
+        if t.get_device() != index:
             raise ValueError(f"{other} is on {t.device}, {name} is on {first.device}")
+
+
+def _kept(t, name: str, dtype, shape, index: int, maker: str) -> None:
+    """What a forward pass kept, come back as it was."""
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{name} must be the tensor that {maker} returned: {dtype}, {tuple(shape)}, contiguous, "
+                         f"not {t.dtype}, {tuple(t.shape)} on {t.device}")
 
 
 def _on_gpu(t, name: str) -> None:
@@ -120,6 +128,8 @@ def _heads(t):
     """``t`` [B, S, heads, D] as the kernels read it, and its strides of (B, S, heads):
     D contiguous, positions apart, 16-byte rows.  Other layouts are copied."""
     B, S, H, D = t.shape
+    if t.is_contiguous() and not t.data_ptr() % 16:
+        return t, (S * H * D, H * D, D)
     b, s, h, d = t.stride()
     # A dimension of one may come with any stride; rows behind the last have to lie past it.
     st = (b if B > 1 else D, s if S > 1 else D, h if H > 1 else D)
@@ -129,24 +139,28 @@ def _heads(t):
     return t, t.stride()[:3]
 
 
-def _attention_checks(q, k, v, scale, lengths, **more):
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be [batch, positions, heads, head dimension], not {tuple(t.shape)}")
+def _attention_checks(q, k, v, scale, lengths, back=None):
+    """(B, S, H, Hk, D, type, scale, lengths) of a call's tensors; ``back``: (dout, out, lse, low)."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        for t, name in ((q, "q"), (k, "k"), (v, "v")):
+            if t.dim() != 4:
+                raise ValueError(f"{name} must be [batch, positions, heads, head dimension], not {tuple(t.shape)}")
     B, S, H, D = q.shape
     Hk = k.shape[2]
+    dtype, index, want = q.dtype, q.get_device(), (B, S, Hk, D)
     code = _type(q, "q", "bfloat16 or float16")
-    dtype, device = q.dtype, q.device
-    if not (k.dtype == v.dtype == dtype and k.device == v.device == device):
+    if not (k.shape == want and v.shape == want and k.dtype == dtype and v.dtype == dtype and k.get_device() == index
+            and v.get_device() == index):
         _same(q, "q", k=k, v=v)
-    want = (B, S, Hk, D)
-    if k.shape != want or v.shape != want:
         _shape(k, "k", want)
         _shape(v, "v", want)
-    if more:
-        _same(q, "q", **{n: t for n, t in more.items() if n not in ("lse", "low")})
-        for name, t in more.items():
-            _shape(t, name, (B, H, S) if name == "lse" else (B, S, H, D))
+    if back is not None:
+        dout, out, lse, low = back
+        _same(q, "q", dout=dout, out=out)
+        _shape(dout, "dout", (B, S, H, D))
+        _shape(out, "out", (B, S, H, D))
+        _kept(lse, "lse", torch.float32, (B, H, S), index, "attention_fwd")
+        _kept(low, "low", torch.uint8, (B, S, H, D), index, "attention_fwd")
     if D != 128 and D != 64:
         raise ValueError(f"the head dimension must be 64 or 128, not {D}")
     if H == 0 or Hk == 0 or H % Hk:
@@ -160,13 +174,9 @@ def _attention_checks(q, k, v, scale, lengths, **more):
         if lengths.dtype != torch.int32:
             raise TypeError(f"lengths must be int32, not {lengths.dtype}")
         _shape(lengths, "lengths", (B,))
-        if lengths.device != device:
-            raise ValueError(f"lengths is on {lengths.device}, q is on {device}")
+        if lengths.get_device() != index:
+            raise ValueError(f"lengths is on {lengths.device}, q is on {q.device}")
         lengths = lengths.contiguous()
-    if more:
-        for name, t in (("lse", torch.float32), ("low", torch.uint8)):
-            if more[name].dtype != t or not more[name].is_contiguous() or more[name].device != device:
-                raise ValueError(f"{name} must be the {t} tensor that attention_fwd returned")
     _on_gpu(q, "q")
     return B, S, H, Hk, D, code, scale, lengths
 
@@ -252,7 +262,7 @@ def attention_bwd(dout, q, k, v, out, saved, *, causal: bool = True, scale: floa
 
 
 def _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, stream, into):
-    B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths, dout=dout, out=out, lse=lse, low=low)
+    B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths, (dout, out, lse, low))
     if not _here(q, stream):
         return _there(q, stream, lambda: _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, None, into))
     (q, qs), (k, ks), (v, vs), (out, os_), (dout, gs) = _heads(q), _heads(k), _heads(v), _heads(out), _heads(dout)
@@ -287,23 +297,21 @@ def _matrix(t):
     return m.clone(memory_format=torch.contiguous_format), n
 
 
-def _swiglu_checks(x, w, **more):
+def _swiglu_checks(x, w, dh=None, saved=None):
     if x.dim() < 1 or w.dim() != 2:
         raise ValueError(f"x must be [..., width] and w [2 inner, width], not {tuple(x.shape)} and {tuple(w.shape)}")
     K, F = x.shape[-1], w.shape[0] // 2
-    code = _type(x, "x", "bfloat16 or float16")
-    if w.dtype != x.dtype or w.device != x.device or w.shape != (2 * F, K):
+    code, index = _type(x, "x", "bfloat16 or float16"), x.get_device()
+    if w.dtype != x.dtype or w.get_device() != index or w.shape != (2 * F, K):
         _same(x, "x", w=w)
         _shape(w, "w", (2 * F, K))
     if K == 0 or F == 0 or K % 8 or F % 8 or K > 1 << 20 or F > 1 << 20:
         raise ValueError(f"width and inner must be multiples of 8, at most {1 << 20}, not {K} and {F}")
-    if more:
-        _same(x, "x", dh=more["dh"])
-        for name, t in more.items():
-            _shape(t, name, (*x.shape[:-1], F if name == "dh" else 6 * F))
-        saved = more["saved"]
-        if saved.dtype != torch.uint8 or not saved.is_contiguous() or saved.device != x.device:
-            raise ValueError("saved must be the uint8 tensor that swiglu_fwd returned")
+    if dh is not None:
+        lead = x.shape[:-1]
+        _same(x, "x", dh=dh)
+        _shape(dh, "dh", (*lead, F))
+        _kept(saved, "saved", torch.uint8, (*lead, 6 * F), index, "swiglu_fwd")
     T = x.numel() // K
     if T >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} rows, not {T}")
@@ -391,7 +399,7 @@ def swiglu_bwd(dh, x, w, saved, *, stream=None):
 
 
 def _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, stream):
-    T, K, F, code = _swiglu_checks(x, w, dh=dh, saved=saved)
+    T, K, F, code = _swiglu_checks(x, w, dh, saved)
     if not _here(x, stream):
         return _there(x, stream, lambda: _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, None))
     dx = x.new_empty(x.shape) if want_dx else None
@@ -425,30 +433,31 @@ def _lines(t):
     return m, m.stride(0)
 
 
-def _add_norm_checks(first, name, weight, post_weight, gate, scale, eps, **rows):
-    if first.dim() < 1:
-        raise ValueError(f"{name} must be [..., width], not a single value")
-    shape, dtype, device = first.shape, first.dtype, first.device
+def _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps):
+    if residual.dim() < 1:
+        raise ValueError("residual must be [..., width], not a single value")
+    shape, dtype, index = residual.shape, residual.dtype, residual.get_device()
     C = shape[-1]
-    code = _type(first, name, "bfloat16, float16 or float32")
-    for other, t in rows.items():
-        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != device):
-            _shape(t, other, shape)
-            _same(first, name, **{other: t})
-    for other, t in (("weight", weight), ("post_weight", post_weight), ("gate", gate)):
-        if t is not None and (t.shape != (C,) or t.dtype != dtype or t.device != device):
-            _shape(t, other, (C,))
-            _same(first, name, **{other: t})
+    code, vector = _type(residual, "residual", "bfloat16, float16 or float32"), (C,)
+    if not (branch.shape == shape and branch.dtype == dtype and branch.get_device() == index and weight.shape == vector
+            and weight.dtype == dtype and weight.get_device() == index):
+        _shape(branch, "branch", shape)
+        _shape(weight, "weight", vector)
+        _same(residual, "residual", branch=branch, weight=weight)
+    for name, t in (("post_weight", post_weight), ("gate", gate)):
+        if t is not None and (t.shape != vector or t.dtype != dtype or t.get_device() != index):
+            _shape(t, name, vector)
+            _same(residual, "residual", **{name: t})
     if not 0 < C <= MAX_NORM_WIDTH:
         raise ValueError(f"the width must be 1 to {MAX_NORM_WIDTH}, not {C}")
-    T = first.numel() // C
+    T = residual.numel() // C
     if T >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} rows, not {T}")
     if not -math.inf < scale < math.inf:
         raise ValueError(f"scale must be finite, not {scale}")
     if not 0 <= eps < math.inf:
         raise ValueError(f"eps must be finite and not negative, not {eps}")
-    _on_gpu(first, name)
+    _on_gpu(residual, "residual")
     return T, C, code
 
 
@@ -479,7 +488,7 @@ def add_norm_fwd(residual, branch, weight, *, post_weight=None, gate=None, scale
 
 
 def _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, keep):
-    T, C, code = _add_norm_checks(residual, "residual", weight, post_weight, gate, scale, eps, branch=branch)
+    T, C, code = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps)
     if not _here(residual, stream):
         return _there(residual, stream,
                       lambda: _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, keep))
@@ -513,12 +522,13 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
     dresidual, the same tensor; gradients of absent weights are None."""
     if dstream is None and dout is None:
         raise ValueError("one of dstream and dout must be given")
-    T, C, code = _add_norm_checks(residual, "residual", weight, post_weight, gate, scale, eps, dstream=dstream, dout=dout,
-                                  branch=branch)
-    if saved.dtype != torch.float32 or saved.shape != (2, T) or not saved.is_contiguous():
-        raise ValueError("saved must be the float32 tensor that add_norm_fwd returned")
-    if saved.device != residual.device:
-        raise ValueError(f"saved is on {saved.device}, residual is on {residual.device}")
+    T, C, code = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps)
+    shape = residual.shape
+    for name, t in (("dstream", dstream), ("dout", dout)):
+        if t is not None:
+            _shape(t, name, shape)
+            _same(residual, "residual", **{name: t})
+    _kept(saved, "saved", torch.float32, (2, T), residual.get_device(), "add_norm_fwd")
     if not _here(residual, stream):
         return _there(residual, stream, lambda: add_norm_bwd(dstream, dout, residual, branch, weight, saved, eps=eps,
                                                             post_weight=post_weight, gate=gate, scale=scale))
