@@ -58,6 +58,9 @@ def parse_args(argv=None):
     ap.add_argument("--load", default="synthetic", choices=["synthetic", "train"],
                     help="GPU work per unit: the synthetic gfx950 kernels (default) or a PyTorch bf16 "
                     "decoder training step (forward + backward + AdamW, DDP when N > 1)")
+    ap.add_argument("--train-ops", default="torch", choices=["torch", "hip"],
+                    help="the training step's attention, gate and norms: torch's library kernels, or this package's own "
+                    "(ops/decoder.py), whose operations are known")
     ap.add_argument("--train-dim", type=int, default=4096)
     ap.add_argument("--train-layers", type=int, default=4)
     ap.add_argument("--train-batch", type=int, default=4)

@@ -265,7 +265,11 @@ class TrainLoad(GpuLoad):
     backward + AdamW, DDP over RCCL when N > 1.  Hundreds of library kernels
     (hipBLASLt GEMMs, flash attention, elementwise) per step, which is the kind of
     workload a DaemonSet exporter shares the GPU with.  Random-init weights and
-    synthetic tokens; the exporter is measured exactly as with the synthetic load."""
+    synthetic tokens; the exporter is measured exactly as with the synthetic load.
+
+    ``--train-ops hip``: the same model with the block's attention, gate and norms as this
+    package's kernels (kube_gpu_stats_amd/ops/decoder.py), whose operations a step are
+    known and reported by calibrate()."""
 
     burst_timed = None  # no MFMA burst kernel of known length: phase U is skipped
 
@@ -276,6 +280,9 @@ class TrainLoad(GpuLoad):
 
         self.torch = torch
         dev = torch.device("cuda", device) if device >= 0 else torch.device("cpu")  # cpu: tests only
+        self.hip = a.train_ops == "hip"
+        if self.hip:
+            from kube_gpu_stats_amd.ops import decoder
         d, h, L, ff = a.train_dim, a.train_dim // 128, a.train_layers, int(a.train_dim * 8 / 3 / 256 + 0.5) * 256
         self.batch, self.seq, self.vocab = a.train_batch, a.train_seq, a.train_vocab
 
@@ -311,9 +318,28 @@ class TrainLoad(GpuLoad):
                     x = b(x)
                 return self.head(self.norm(x))
 
+        class HipModel(Model):
+            """The same with the residual sums and the norms behind them as one operator."""
+
+            def forward(self, t):
+                x = self.emb(t)
+                B, S, _ = x.shape
+                eps = torch.finfo(x.dtype).eps  # nn.RMSNorm's
+                y = self.blocks[0].n1(x)
+                after = [b.n1 for b in self.blocks[1:]] + [self.norm]
+                for b, norm in zip(self.blocks, after):
+                    z = decoder.attention_qkv(b.qkv(y).view(B, S, 3 * h, d // h), h)
+                    x, y = decoder.add_norm(x, b.o(z.view(B, S, d)), b.n2.weight, eps=eps)
+                    x, y = decoder.add_norm(x, b.down(decoder.swiglu(y, b.up.weight)), norm.weight, eps=eps)
+                return self.head(y)
+
         torch.manual_seed(1234)
-        model = Model(self.vocab).to(device=dev, dtype=torch.bfloat16)
+        model = (HipModel if self.hip else Model)(self.vocab).to(device=dev, dtype=torch.bfloat16)
         self.params = sum(p.numel() for p in model.parameters())
+        # What the operators of ops/decoder.py have to compute in a step: causal attention (two products
+        # forward, five backward over half the square), the gate's projections and their gradients.
+        pairs = self.batch * self.seq * (self.seq + 1) / 2
+        self.op_flops = L * (14.0 * pairs * d + 12.0 * self.batch * self.seq * d * ff)
         if ctx is not None and ctx.is_dist:
             from torch.nn.parallel import DistributedDataParallel
 
@@ -362,7 +388,8 @@ class TrainLoad(GpuLoad):
         s = sorted(ts)[1]
         toks = self.batch * self.seq
         # 6·N·T for the dense weights + causal attention (fwd 2·S·d per token per layer, x3 with bwd)
-        return {"train_step_ms": s * 1e3, "train_tokens_per_s": toks / s, "train_params": self.params,
+        own = {"train_ops": "hip", "train_op_tflop_per_step": self.op_flops * 1e-12} if self.hip else {}
+        return {**own, "train_step_ms": s * 1e3, "train_tokens_per_s": toks / s, "train_params": self.params,
                 "train_tflops": 6.0 * self.params * toks / s / 1e12}
 
 

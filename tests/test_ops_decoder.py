@@ -765,6 +765,32 @@ def test_streams(dev):
     assert all(torch.equal(p, r) for p, r in zip(n2, decoder.add_norm_bwd(x, x, x, x, ws[0], s3[2])) if p is not None)
 
 
+@gpu
+def test_train_load_on_own_operators(dev):
+    """bench.py --load train --train-ops hip: the step runs, and its gradients are the torch model's."""
+    import bench
+
+    loads = []
+    for ops in ("torch", "hip"):
+        a = bench.parse_args(["--load", "train", "--train-ops", ops, "--train-dim", "256", "--train-layers", "2",
+                              "--train-batch", "2", "--train-seq", "96", "--train-vocab", "512"])
+        loads.append(bench.TrainLoad(a, 0, None))
+    grads = []
+    for ld in loads:
+        logits = ld.model(ld.tok[:, :-1])
+        ld.F.cross_entropy(logits.float().view(-1, ld.vocab), ld.tok[:, 1:].reshape(-1)).backward()
+        grads.append({n: p.grad.double() for n, p in ld.model.named_parameters()})
+    # The two differ by what either rounds: about 30 tensors on the longest way (two layers, there and
+    # back), each half a step of bfloat16 in the mean square at most, on both sides.
+    for n, g in grads[0].items():
+        assert (grads[1][n] - g).norm() <= 2 * math.sqrt(30) * half_step(BF16) * g.norm(), n
+    ld = loads[1]
+    ld.opt.zero_grad(set_to_none=True)
+    ld.step()
+    assert all(torch.isfinite(p).all() for p in ld.model.parameters())
+    assert ld.calibrate()["train_ops"] == "hip" and ld.op_flops > 0
+
+
 # ----------------------------------------------------------------------------- refusals (CPU)
 
 def z(*shape, t=BF16):
