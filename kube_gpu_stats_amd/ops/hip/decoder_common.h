@@ -65,6 +65,26 @@ __device__ __forceinline__ i32x4 buffer(const void* base, int64_t bytes) {
   return r;
 }
 
+// A descriptor that walks through a matrix: `step` bytes further each time, and as many
+// fewer to the end.  Few scalar instructions: they stand between a workgroup's products.
+struct Walk {
+  uint64_t base;
+  int64_t left;
+  __device__ __forceinline__ Walk() {}
+  __device__ __forceinline__ Walk(const void* p, int64_t bytes) : base(reinterpret_cast<uint64_t>(p)), left(bytes) {}
+  __device__ __forceinline__ void go(int64_t step) {
+    base += step;
+    left -= step;
+  }
+  __device__ __forceinline__ i32x4 descriptor() const {
+    const int high = static_cast<int>(left >> 32);
+    const uint32_t low = static_cast<uint32_t>(left);
+    const uint32_t some = high > 0 || low > kFar ? kFar : low;
+    return i32x4{static_cast<int>(base), static_cast<int>(base >> 32) & 0xFFFF, high < 0 ? 0 : static_cast<int>(some),
+                 0x00027000};
+  }
+};
+
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(i32x4 d) {
   const uint64_t p = static_cast<uint32_t>(d[0]) | (static_cast<uint64_t>(static_cast<uint32_t>(d[1])) << 32);
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(p), 0, d[2], 0x00027000);
@@ -84,10 +104,10 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 // next LDS read; there is no result register, and copies_done() is the wait.  The s_nop
 // covers what the compiler would: a scalar register written by a vector instruction (the
 // descriptor's readfirstlane) is not read by a memory instruction within 5 states.
-__device__ __forceinline__ void copy16(i32x4 d, int voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+__device__ __forceinline__ void copy16(i32x4 d, int voff, uint32_t lds, int soff = 0) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
-               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(d)
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(d), "s"(soff)
                : "memory");
 }
 __device__ __forceinline__ void copy4(i32x4 d, int voff, uint32_t lds) {
@@ -156,10 +176,10 @@ template <int W> struct Tile {
         voff[i] = static_cast<int>(row * stride) + ((pc ^ swizzle(row)) << 4);
       }
     }
-    __device__ __forceinline__ void go(i32x4 d, uint32_t lds, int wave) const {
+    __device__ __forceinline__ void go(i32x4 d, uint32_t lds, int wave, int soff = 0) const {
 #pragma unroll
       for (int i = 0; i < kN; ++i)
-        if (kAll % NW == 0 || wave * kN + i < kAll) copy16(d, voff[i], lds + (wave * kN + i) * 1024);
+        if (kAll % NW == 0 || wave * kN + i < kAll) copy16(d, voff[i], lds + (wave * kN + i) * 1024, soff);
     }
   };
 };

@@ -40,19 +40,28 @@ template <class T, int ROWS, int NW> struct Operand<T, ROWS, false, NW> {
   using Cp = typename Tl::template Copy<ROWS, NW>;
   static constexpr int kBytes = ROWS * kK * 2;
   Cp copy;
-  __device__ __forceinline__ void init(int wave, int lane, int64_t ld) { copy.init(wave, lane, ld * 2); }
-  // rows r0.. (rows - r0 of them), sum indexes k0.. of K; chunks past K are read as zero
-  __device__ __forceinline__ void go(const void* p, int64_t ld, int r0, int rows, int k0, int K, uint32_t lds, int wave,
-                                     int lane) const {
-    const int64_t bytes = rows > r0 ? ((rows - 1 - r0) * ld + (K - k0)) * 2 : 0;
-    const i32x4 d = buffer(static_cast<const T*>(p) + r0 * ld + k0, bytes);
-    if (k0 + kK <= K) return copy.go(d, lds, wave);
+  i32x4 d;
+  int k0, K;
+  // rows r0.. (rows - r0 of them), sum indexes from k of K.  The descriptor is that of the
+  // whole rows and stands; the sum index is the scalar offset.  Whether that is part of
+  // the range check or not, rows past the last are out of range and the others in it.
+  __device__ __forceinline__ void init(const void* p, int64_t ld, int r0, int rows, int k, int sum, int wave, int lane) {
+    copy.init(wave, lane, ld * 2);
+    d = buffer(static_cast<const T*>(p) + r0 * ld, rows > r0 ? ((rows - 1 - r0) * ld + sum) * 2 : 0);
+    k0 = k;
+    K = sum;
+  }
+  // the next kK of the sum; chunks past K are read as zero
+  __device__ __forceinline__ void go(uint32_t lds, int wave, int lane) {
+    const int k = k0;
+    k0 += kK;
+    if (k0 <= K) return copy.go(d, lds, wave, k * 2);
 #pragma unroll
     for (int i = 0; i < Cp::kN; ++i) {
       const int byte = (wave * Cp::kN + i) * 1024 + lane * 16, row = byte / Tl::kRow;
       const int chunk = ((byte >> 4) & 7) ^ Tl::swizzle(row);
       if (Cp::kAll % NW == 0 || wave * Cp::kN + i < Cp::kAll)
-        copy16(d, k0 + chunk * 8 < K ? copy.voff[i] : static_cast<int>(kFar), lds + (wave * Cp::kN + i) * 1024);
+        copy16(d, k + chunk * 8 < K ? copy.voff[i] : static_cast<int>(kFar), lds + (wave * Cp::kN + i) * 1024, k * 2);
     }
   }
   static __device__ __forceinline__ typename El<T>::x8 read(const char* t, int r0, int kk, int lane) {
@@ -66,14 +75,22 @@ template <class T, int ROWS, int NW> struct Operand<T, ROWS, true, NW> {
   using Cp = typename Tl::template Copy<kK, NW>;
   static constexpr int kBytes = kSub * kSubBytes;
   Cp copy;
-  __device__ __forceinline__ void init(int wave, int lane, int64_t ld) { copy.init(wave, lane, ld * 2); }
-  __device__ __forceinline__ void go(const void* p, int64_t ld, int r0, int rows, int k0, int K, uint32_t lds, int wave,
-                                     int) const {
+  Walk walk[kSub];
+  int64_t step;
+  __device__ __forceinline__ void init(const void* p, int64_t ld, int r0, int rows, int k, int sum, int wave, int lane) {
+    copy.init(wave, lane, ld * 2);
+    step = kK * ld * 2;
 #pragma unroll
     for (int s = 0; s < kSub; ++s) {
       const int r = r0 + s * W;
-      const int64_t bytes = rows > r ? ((K - 1 - k0) * ld + (rows - r)) * 2 : 0;
-      copy.go(buffer(static_cast<const T*>(p) + k0 * ld + r, bytes), lds + s * kSubBytes, wave);
+      walk[s] = Walk(static_cast<const T*>(p) + k * ld + r, rows > r ? ((sum - 1 - k) * ld + (rows - r)) * 2 : 0);
+    }
+  }
+  __device__ __forceinline__ void go(uint32_t lds, int wave, int) {
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) {
+      copy.go(walk[s].descriptor(), lds + s * kSubBytes, wave);
+      walk[s].go(step);
     }
   }
   static __device__ __forceinline__ typename El<T>::x8 read(const char* t, int r0, int kk, int lane) {
@@ -155,16 +172,16 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_kernel(Product p) {
   const int hi = static_cast<int>(static_cast<int64_t>(steps_all) * (split + 1) / p.splits);
 
   OA oa;
-  OB ob;
-  oa.init(wave, lane, p.a_ld);
-  ob.init(wave, lane, p.b_ld);
+  OB ob, ou;  // ou: the columns of the second half
+  oa.init(p.a, p.a_ld, m0, p.M, lo * kK, p.K, wave, lane);
+  ob.init(p.b, p.b_ld, n0, N, lo * kK, p.K, wave, lane);
+  if (PAIR) ou.init(static_cast<const T*>(p.b) + N * p.b_ld, p.b_ld, n0, N, lo * kK, p.K, wave, lane);
   const uint32_t lds = lds_address(smem);
   auto fetch = [&](int j) {
     const uint32_t to = lds + (j & 1) * kStage;
-    oa.go(p.a, p.a_ld, m0, p.M, j * kK, p.K, to, wave, lane);
-    ob.go(p.b, p.b_ld, n0, N, j * kK, p.K, to + OA::kBytes, wave, lane);
-    if (PAIR)
-      ob.go(static_cast<const T*>(p.b) + N * p.b_ld, p.b_ld, n0, N, j * kK, p.K, to + OA::kBytes + OB::kBytes, wave, lane);
+    oa.go(to, wave, lane);
+    ob.go(to + OA::kBytes, wave, lane);
+    if (PAIR) ou.go(to + OA::kBytes + OB::kBytes, wave, lane);
   };
 
   // The fragments of a sixteenth of the sum, read while the products of the one before
