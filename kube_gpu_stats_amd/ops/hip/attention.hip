@@ -163,25 +163,28 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
   ck.init(wave, lane, a.k_st[1] * 2);
   cv.init(wave, lane, a.v_st[1] * 2);
   const uint32_t lds = lds_address(smem);
-  auto fetch = [&](int j, int slot) {
-    const int s = j * kStep;
-    ck.go(buffer(at<T>(a.k, a.k_st, b, s, hk), span<T, D>(n, s, a.k_st[1])), lds + slot * 2 * kTile, wave);
-    cv.go(buffer(at<T>(a.v, a.v_st, b, s, hk), span<T, D>(n, s, a.v_st[1])), lds + slot * 2 * kTile + kTile, wave);
+  Walk wk(at<T>(a.k, a.k_st, b, 0, hk), span<T, D>(n, 0, a.k_st[1]));
+  Walk wv(at<T>(a.v, a.v_st, b, 0, hk), span<T, D>(n, 0, a.v_st[1]));
+  auto fetch = [&](int slot) {  // the next step
+    ck.go(wk.descriptor(), lds + slot * 2 * kTile, wave);
+    cv.go(wv.descriptor(), lds + slot * 2 * kTile + kTile, wave);
+    wk.go(kStep * 2 * a.k_st[1]);
+    wv.go(kStep * 2 * a.v_st[1]);
   };
 
   f32x16 o[D / 32] = {};
   float top = -INFINITY, sum = 0.f;
   const float c = a.scale * kLog2e;
-  if (steps > 0) fetch(0, 0);
+  if (steps > 0) fetch(0);
   loads_done();
   if (steps > 0)
 #pragma unroll
-    for (int j = 1; j < NS - 1; ++j) fetch(j, j);
+    for (int j = 1; j < NS - 1; ++j) fetch(j);
   int slot = 0;
   for (int j = 0; j < steps; ++j) {
     copies_left<(NS - 2) * 2 * Cp::kN>();
     barrier();  // step j has landed for every wave, and nobody reads the slot before it any more
-    fetch(j + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+    fetch(slot == 0 ? NS - 1 : slot - 1);
     const int s0 = j * kStep;
     const char* kt = smem + slot * 2 * kTile;
     const char* vt = kt + kTile;
@@ -317,24 +320,27 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   ck.init(wave, lane, a.k_st[1] * 2);
   cv.init(wave, lane, a.v_st[1] * 2);
   const uint32_t lds = lds_address(smem);
-  auto fetch = [&](int j, int slot) {
-    const int s = j * kStep;
-    ck.go(buffer(at<T>(a.k, a.k_st, b, s, hk), span<T, D>(n, s, a.k_st[1])), lds + slot * 2 * kTile, wave);
-    cv.go(buffer(at<T>(a.v, a.v_st, b, s, hk), span<T, D>(n, s, a.v_st[1])), lds + slot * 2 * kTile + kTile, wave);
+  Walk wk(at<T>(a.k, a.k_st, b, 0, hk), span<T, D>(n, 0, a.k_st[1]));
+  Walk wv(at<T>(a.v, a.v_st, b, 0, hk), span<T, D>(n, 0, a.v_st[1]));
+  auto fetch = [&](int slot) {  // the next step
+    ck.go(wk.descriptor(), lds + slot * 2 * kTile, wave);
+    cv.go(wv.descriptor(), lds + slot * 2 * kTile + kTile, wave);
+    wk.go(kStep * 2 * a.k_st[1]);
+    wv.go(kStep * 2 * a.v_st[1]);
   };
 
   f32x16 acc[D / 32] = {};
   const float c = a.scale * kLog2e;
-  if (steps > 0) fetch(0, 0);
+  if (steps > 0) fetch(0);
   loads_done();
   if (steps > 0)
 #pragma unroll
-    for (int j = 1; j < NS - 1; ++j) fetch(j, j);
+    for (int j = 1; j < NS - 1; ++j) fetch(j);
   int slot = 0;
   for (int j = 0; j < steps; ++j) {
     copies_left<(NS - 2) * 2 * Cp::kN>();
     barrier();
-    fetch(j + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+    fetch(slot == 0 ? NS - 1 : slot - 1);
     const int s0 = j * kStep;
     const char* kt = smem + slot * 2 * kTile;
     const char* vt = kt + kTile;
@@ -459,16 +465,27 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
   // end of the walk the descriptors are empty, as in the forward pass.
   int fh = hi > lo ? lo / each : 0, fs = hi > lo ? lo % each : 0, fi = lo;
   const int groups = (a.S + 31) / 32;
+  Walk wq, wg, ws;  // q, do, and lse and delta of the rows
+  auto head = [&] {
+    const int h = hk * G + fh, s = (first + fs) * kQ;
+    wq = Walk(at<T>(a.q, a.q_st, b, s, h), span<T, D>(n, s, a.q_st[1]));
+    wg = Walk(at<T>(a.dout, a.g_st, b, s, h), span<T, D>(n, s, a.g_st[1]));
+    ws = Walk(a.delta + (static_cast<int64_t>(b * a.H + h) * groups + first + fs) * 64, (groups - first - fs) * 256ll);
+  };
+  if (lo < hi) head();
   auto fetch = [&](int slot) {
-    const int h = hk * G + fh, s = (first + fs) * kQ, end = fi < hi ? n : 0;
+    if (fi++ >= hi) wq.left = wg.left = ws.left = 0;
     const uint32_t to = lds + kV + slot * kStage;
-    cq.go(buffer(at<T>(a.q, a.q_st, b, s, h), span<T, D>(end, s, a.q_st[1])), to, wave);
-    cg.go(buffer(at<T>(a.dout, a.g_st, b, s, h), span<T, D>(end, s, a.g_st[1])), to + kTile, wave);
-    if (wave == 0)  // lse and delta of the rows
-      copy4(buffer(a.delta + (static_cast<int64_t>(b * a.H + h) * groups + first + fs) * 64, end ? 256 : 0), lane * 4,
-            to + 2 * kTile);
-    ++fi;
-    if (++fs == each) fs = 0, ++fh;
+    cq.go(wq.descriptor(), to, wave);
+    cg.go(wg.descriptor(), to + kTile, wave);
+    if (wave == 0) copy4(ws.descriptor(), lane * 4, to + 2 * kTile);
+    wq.go(kQ * 2 * a.q_st[1]);
+    wg.go(kQ * 2 * a.g_st[1]);
+    ws.go(256);
+    if (++fs == each) {
+      fs = 0;
+      if (++fh < G) head();
+    }
   };
 
   f32x16 dka[D / 32] = {}, dva[D / 32] = {};

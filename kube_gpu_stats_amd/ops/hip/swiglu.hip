@@ -256,7 +256,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_kernel(Product p) {
   char* const own = smem + wave * (PAIR ? 4 : 1) * kArea;
   const int row = lane & 31, half = lane >> 5;
   // 16-byte chunk c of row r; 8 (or 4) rows lie side by side in the banks
-  const auto place = [](int r, int c) { return r * kRow + ((c ^ ((r >> (W == 64 ? 1 : 2)) & (W / 8 - 1))) << 4); };
+  const auto place = [](int r, int c) { return r * kRow + ((c ^ ((r >> (W == 128 ? 0 : W == 64 ? 1 : 2)) & (W / 8 - 1))) << 4); };
   const auto out = [&](const char* from, char* base, int64_t stride, int m, int n) {
 #pragma unroll
     for (int i = 0; i < 32 / kRows; ++i) {
