@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.S + kRows - 1) / kRows;
   int bh, rank;
-  if (!head_item(blockIdx.x, a.B * a.H, tiles, CAUSAL ? 16 : 1, bh, rank)) return;
+  if (!head_item(blockIdx.x, a.B * a.H, tiles, CAUSAL ? 16 : 1, a.lengths != nullptr, bh, rank)) return;
   const int tile = tiles - 1 - rank;  // causal: the long rows first
   const int h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk);
   const int n = length_of(a, b);
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.S + kRows - 1) / kRows;
   int bh, rank;
-  if (!head_item(blockIdx.x, a.B * a.H, tiles, CAUSAL ? 16 : 1, bh, rank)) return;
+  if (!head_item(blockIdx.x, a.B * a.H, tiles, CAUSAL ? 16 : 1, a.lengths != nullptr, bh, rank)) return;
   const int tile = tiles - 1 - rank;
   const int h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk);
   const int n = length_of(a, b);
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.S + kRows - 1) / kRows;
   int bh, rank;
-  if (!head_item(blockIdx.x, a.B * a.Hk, tiles * a.splits, CAUSAL ? 16 : 1, bh, rank)) return;
+  if (!head_item(blockIdx.x, a.B * a.Hk, tiles * a.splits, CAUSAL ? 16 : 1, a.lengths != nullptr, bh, rank)) return;
   const int split = rank % a.splits, tile = rank / a.splits;  // causal: the first keys have the most rows
   const int hk = bh % a.Hk, b = bh / a.Hk, G = a.H / a.Hk;
   const int n = length_of(a, b);
@@ -563,7 +563,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
   }
   copies_done();
   if (a.splits > 1) {
-    if (key < a.S) {
+    if (key < n) {  // the join reads no more
       const int64_t part = static_cast<int64_t>(a.B) * a.S * a.Hk * D;
       float* w = a.partial + split * 2 * part + ((static_cast<int64_t>(b) * a.S + key) * a.Hk + hk) * D;
 #pragma unroll
@@ -632,15 +632,15 @@ int check(const KgsAttention* a, bool backward) {
 
 template <class T, int D, bool CAUSAL> int forward(const KgsAttention& a, hipStream_t s) {
   const int64_t tiles = (a.S + kRows - 1) / kRows;
-  attention_fwd_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(a.B * static_cast<int64_t>(a.H), tiles)), kThreads, 0, s>>>(a);
+  attention_fwd_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(a.B * static_cast<int64_t>(a.H), tiles, a.lengths)), kThreads, 0, s>>>(a);
   return launched("attention forward");
 }
 
 template <class T, int D, bool CAUSAL> int backward(const KgsAttention& a, hipStream_t s) {
   const int64_t tiles = (a.S + kRows - 1) / kRows, b = a.B;
-  attention_dq_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(b * a.H, tiles)), kThreads, 0, s>>>(a);
+  attention_dq_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(b * a.H, tiles, a.lengths)), kThreads, 0, s>>>(a);
   if (launched("attention dq")) return -1;
-  attention_dkv_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(b * a.Hk, tiles * a.splits)), kThreads, 0, s>>>(a);
+  attention_dkv_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(b * a.Hk, tiles * a.splits, a.lengths)), kThreads, 0, s>>>(a);
   if (launched("attention dk, dv")) return -1;
   if (a.splits > 1) {
     const int64_t n = 2 * b * a.S * a.Hk * D / 4;

@@ -199,12 +199,14 @@ __device__ __forceinline__ int64_t xcd_item(int64_t id, int64_t total) {
 // 16 heads fill up the end (forward of 4 x 32 heads, 2048 positions: 192 us, 208 us head
 // by head); where they do not, head by head keeps fewer keys in the L2 in use (280 us,
 // 297 us by 16).  The heads that are left when 8 do not divide them are dealt to the
-// XCDs piece by piece, so that none has more than its share.
-__host__ __device__ __forceinline__ int64_t head_items(int64_t heads, int64_t ranks) {
-  return 8 * ((heads % 8 * ranks + 7) / 8 + heads / 8 * ranks);
+// XCDs piece by piece, so that none has more than its share; so are all of them (deal)
+// where sequences differ in length, or an XCD could hold the long ones' heads.
+__host__ __device__ __forceinline__ int64_t head_items(int64_t heads, int64_t ranks, bool deal) {
+  const int64_t left = deal ? heads : heads % 8;
+  return 8 * ((left * ranks + 7) / 8 + (heads - left) / 8 * ranks);
 }
-__device__ __forceinline__ bool head_item(int id, int heads, int ranks, int group, int& head, int& rank) {
-  const int x = id & 7, left = heads & 7, own = heads >> 3, dealt = (left * ranks + 7) / 8;
+__device__ __forceinline__ bool head_item(int id, int heads, int ranks, int group, bool deal, int& head, int& rank) {
+  const int x = id & 7, left = deal ? heads : heads & 7, own = (heads - left) >> 3, dealt = (left * ranks + 7) / 8;
   int k = id >> 3;
   if (k < dealt) {
     const int i = k * 8 + x;
