@@ -504,15 +504,19 @@ def _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, strea
     return s, out, saved
 
 
+@functools.lru_cache(maxsize=4096)
 def _norm_parts(T: int, C: int) -> int:
     """Workgroups of the backward, each of which leaves a part of the column sums: as many as
     run at once, 16 waves a CU.  Rows up to 512 wide share a workgroup of four waves, a
-    power of two of lanes with 8 elements each to a row."""
+    power of two of lanes with 8 elements each to a row.  Up to 8 turns are one workgroup's:
+    it writes the sums itself, which saves a launch (7 x 517, all weights: a call of 18.8 us
+    became one of 14.1 us)."""
     if C <= 512:
         lanes = 1 << (-(-C // 8) - 1).bit_length()
-        return min(-(-T // (256 // lanes)), 1024)
-    waves = -(-C // 512) if C <= 8192 else -(-C // 1024)
-    return min(T, 256 * (16 // waves))
+        turns, most = -(-T // (256 // lanes)), 1024
+    else:
+        turns, most = T, 256 * (16 // (-(-C // 512) if C <= 8192 else -(-C // 1024)))
+    return 1 if turns <= 8 else min(turns, most)
 
 
 def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=None, gate=None, scale: float = 1.0,
@@ -542,11 +546,11 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
         dy, dy_ld = _lines(dout) if dout is not None else (None, 0)
         w, pw, g = _vector(weight), _vector(post_weight), _vector(gate)
         parts = _norm_parts(T, C)
-        work = torch.empty(parts * 2 * C, dtype=torch.float32, device=r.device)
+        work = torch.empty(parts * 2 * C, dtype=torch.float32, device=r.device) if parts > 1 else None
         _call("kgs_add_norm_bwd",
               _ADD_NORM.pack(r.data_ptr(), b.data_ptr(), w.data_ptr(), _ptr(pw), _ptr(g), 0, 0, saved.data_ptr(),
                              _ptr(ds), _ptr(dy), dr.data_ptr(), db.data_ptr(), dw.data_ptr(), _ptr(dpw), _ptr(dg),
-                             work.data_ptr(), r_ld, b_ld, 0, ds_ld, dy_ld, T, C, code, parts, scale, eps), r.get_device())
+                             _ptr(work), r_ld, b_ld, 0, ds_ld, dy_ld, T, C, code, parts, scale, eps), r.get_device())
     return dr, db, dw, dpw, dg
 
 

@@ -172,6 +172,19 @@ __global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_fwd_kernel(KgsAdd
   }
 }
 
+// A column's finished sum: v 0 is dweight's, v 1 is A.
+template <class T> __device__ __forceinline__ void finish(const KgsAddNorm& a, int v, int c, float sum) {
+  if (v == 0) {
+    static_cast<T*>(a.dweight)[c] = static_cast<T>(sum);
+    return;
+  }
+  sum *= a.scale;
+  const float pw = a.post_weight ? static_cast<float>(static_cast<const T*>(a.post_weight)[c]) : 1.f;
+  const float gate = a.gate ? static_cast<float>(static_cast<const T*>(a.gate)[c]) : 1.f;
+  if (a.dpost_weight) static_cast<T*>(a.dpost_weight)[c] = static_cast<T>(sum * gate);
+  if (a.dgate) static_cast<T*>(a.dgate)[c] = static_cast<T>(sum * pw);
+}
+
 // The next row's loads are under way while this one is reduced; with one chunk a thread
 // that fits the registers of 16 waves a CU.  Two chunks (rows over 8192 wide) do without,
 // and read the weights again for every row.  WHOLE: the width is a multiple of 8, so that
@@ -307,8 +320,9 @@ __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
       }
     }
   }
-  // this workgroup's column sums
+  // This workgroup's column sums: a part, or, if it is the only one, the results.
   float* part = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * C;
+  const bool only = gridDim.x == 1;
   if constexpr (WAVES) {
     // over the wave's rows, then over the four waves
     const int n = at.lanes * kV, wave = threadIdx.x >> 6;
@@ -327,14 +341,25 @@ __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
     for (int v = 0; v < (FULL ? 2 : 1); ++v)
       for (int c = threadIdx.x; c < n && c < C; c += 256) {
         const float* x = sums + v * 4 * 512 + c;
-        part[v * C + c] = (x[0] + x[512]) + (x[1024] + x[1536]);
+        const float total = (x[0] + x[512]) + (x[1024] + x[1536]);
+        if (only) finish<T>(a, v, c, total);
+        else part[v * C + c] = total;
       }
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = column(i);
-      store(dw[i], part + c, C - c);
-      if constexpr (FULL) store(sum[i], part + C + c, C - c);
+      if (only) {
+#pragma unroll
+        for (int j = 0; j < kV; ++j)
+          if (c + j < C) {
+            finish<T>(a, 0, c + j, dw[i][j]);
+            if constexpr (FULL) finish<T>(a, 1, c + j, sum[i][j]);
+          }
+      } else {
+        store(dw[i], part + c, C - c);
+        if constexpr (FULL) store(sum[i], part + C + c, C - c);
+      }
     }
   }
 }
@@ -354,15 +379,7 @@ template <class T> __global__ __launch_bounds__(1024) void add_norm_join_kernel(
   if (group == 0 && c < C) {
     sum = 0.f;
     for (int i = 0; i < 64; ++i) sum += sums[i][col];
-    if (blockIdx.y == 0) {
-      static_cast<T*>(a.dweight)[c] = static_cast<T>(sum);
-    } else {
-      sum *= a.scale;
-      const float pw = a.post_weight ? static_cast<float>(static_cast<const T*>(a.post_weight)[c]) : 1.f;
-      const float gate = a.gate ? static_cast<float>(static_cast<const T*>(a.gate)[c]) : 1.f;
-      if (a.dpost_weight) static_cast<T*>(a.dpost_weight)[c] = static_cast<T>(sum * gate);
-      if (a.dgate) static_cast<T*>(a.dgate)[c] = static_cast<T>(sum * pw);
-    }
+    finish<T>(a, blockIdx.y, c, sum);
   }
 }
 
@@ -389,6 +406,7 @@ template <class T, bool WAVES, int NV, bool WHOLE, int THREADS> int backward(con
   if (is_full(a)) add_norm_bwd_kernel<T, WAVES, NV, true, WHOLE, THREADS><<<a.parts, threads, 0, s>>>(a);
   else add_norm_bwd_kernel<T, WAVES, NV, false, WHOLE, THREADS><<<a.parts, threads, 0, s>>>(a);
   if (launched("add_norm backward")) return -1;
+  if (a.parts == 1) return 0;
   const bool second = a.dpost_weight || a.dgate;
   add_norm_join_kernel<T><<<dim3((a.width + 15) / 16, second ? 2 : 1), 1024, 0, s>>>(a);
   return launched("add_norm join");
@@ -412,10 +430,10 @@ int dispatch(const KgsAddNorm* a, bool back, void* stream) {
   const char* w = "add_norm";
   if (!a || !a->residual || !a->branch || !a->weight) return fail(w, "a tensor is missing");
   if (!back && (!a->stream || !a->out)) return fail(w, "a tensor is missing");
-  if (back && (!a->rstd || !a->dresidual || !a->dbranch || !a->dweight || !a->partial)) return fail(w, "a tensor is missing");
+  if (back && (!a->rstd || !a->dresidual || !a->dbranch || !a->dweight)) return fail(w, "a tensor is missing");
   if (back && ((a->post_weight && !a->dpost_weight) || (a->gate && !a->dgate))) return fail(w, "a tensor is missing");
   if (a->rows <= 0 || a->rows >= 1 << 30 || a->width <= 0 || a->width > 16384) return fail(w, "bad sizes");
-  if (back && (a->parts < 1 || a->parts > 65536)) return fail(w, "bad parts");
+  if (back && (a->parts < 1 || a->parts > 65536 || (a->parts > 1 && !a->partial))) return fail(w, "bad parts");
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->type) {
     case 0: return run<bf16>(*a, back, s);
