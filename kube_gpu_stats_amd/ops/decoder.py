@@ -546,11 +546,11 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
         dy, dy_ld = _lines(dout) if dout is not None else (None, 0)
         w, pw, g = _vector(weight), _vector(post_weight), _vector(gate)
         parts = _norm_parts(T, C)
-        work = torch.empty(parts * 2 * C, dtype=torch.float32, device=r.device) if parts > 1 else None
+        work = torch.empty(parts * 2 * C, dtype=torch.float32, device=r.device)
         _call("kgs_add_norm_bwd",
               _ADD_NORM.pack(r.data_ptr(), b.data_ptr(), w.data_ptr(), _ptr(pw), _ptr(g), 0, 0, saved.data_ptr(),
                              _ptr(ds), _ptr(dy), dr.data_ptr(), db.data_ptr(), dw.data_ptr(), _ptr(dpw), _ptr(dg),
-                             _ptr(work), r_ld, b_ld, 0, ds_ld, dy_ld, T, C, code, parts, scale, eps), r.get_device())
+                             work.data_ptr(), r_ld, b_ld, 0, ds_ld, dy_ld, T, C, code, parts, scale, eps), r.get_device())
     return dr, db, dw, dpw, dg
 
 

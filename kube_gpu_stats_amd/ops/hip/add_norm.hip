@@ -30,6 +30,7 @@ constexpr int kV = 8;  // elements of a row a thread handles at a time
 // every wider boundary, which global memory instructions allow.
 template <class T> struct __attribute__((packed, aligned(sizeof(T)))) Loose { T v[kV]; };
 
+// (a row of fewer than 8 elements: zeros behind them)
 template <class T> __device__ __forceinline__ void load(float (&x)[kV], const T* p, int left) {
   if (left >= kV) {
     const Loose<T> r = *reinterpret_cast<const Loose<T>*>(p);
@@ -41,13 +42,22 @@ template <class T> __device__ __forceinline__ void load(float (&x)[kV], const T*
   }
 }
 
+// Element `start` of p, the same in the whole workgroup where a row is one's, and a
+// thread's bytes from there: one scalar address and 32 bits a thread.
+template <class T> __device__ __forceinline__ const T* place(const void* p, int64_t start, uint32_t bytes) {
+  return reinterpret_cast<const T*>(reinterpret_cast<const char*>(static_cast<const T*>(p) + start) + bytes);
+}
+template <class T> __device__ __forceinline__ T* place(void* p, int64_t start, uint32_t bytes) {
+  return const_cast<T*>(place<T>(static_cast<const void*>(p), start, bytes));
+}
+
 // The same as it lies in memory.
-template <class T> __device__ __forceinline__ void load_raw(Loose<T>& r, const T* p, int c, int left) {
+template <class T> __device__ __forceinline__ void load_raw(Loose<T>& r, const T* p, int left) {
   if (left >= kV) {
-    r = *reinterpret_cast<const Loose<T>*>(p + c);
+    r = *reinterpret_cast<const Loose<T>*>(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < kV; ++i) r.v[i] = i < left ? p[c + i] : static_cast<T>(0.f);
+    for (int i = 0; i < kV; ++i) r.v[i] = i < left ? p[i] : static_cast<T>(0.f);
   }
 }
 
@@ -90,8 +100,24 @@ __host__ __device__ __forceinline__ int lanes_of_row(int width) {
 
 // Where a thread stands: the first column chunk of its row, the row of its workgroup's
 // turn, and the rows a turn.  WAVES: widths up to 512.
+//
+// A width that is no multiple of 8 has its last chunk moved back to end with the row, so
+// that it too is loaded and stored at once; the first skip() of its elements are the
+// chunk's before it as well: both threads write the same there, and the last leaves them
+// out of the sums.  A thread past the end skips all 8.  (Element by element at the end of
+// each row 20000 x 1501 with all weights took 64 us forward and 111 us back, so 41 us and
+// 95 us.)
+enum Fit { kWhole, kRagged, kTiny };  // a multiple of 8; another width; fewer than 8
 template <bool WAVES> struct Place {
   int lanes, t, row, rows;
+  __device__ __forceinline__ int column(int i, int C) const {
+    const int c = (t + i * lanes) * kV;
+    return c < C ? max(0, min(c, C - kV)) : 0;
+  }
+  __device__ __forceinline__ int skip(int i, int C) const {
+    const int c = (t + i * lanes) * kV;
+    return c >= C ? kV : max(0, c - max(0, C - kV));
+  }
   __device__ __forceinline__ explicit Place(int width) {
     lanes = WAVES ? lanes_of_row(width) : blockDim.x;
     t = WAVES ? threadIdx.x & (lanes - 1) : threadIdx.x;
@@ -101,69 +127,72 @@ template <bool WAVES> struct Place {
 };
 
 // FULL: with post_weight, gate or a scale.  NV: chunks of 8 a thread.
-template <class T, bool WAVES, int NV, bool FULL>
+template <class T, bool WAVES, int NV, bool FULL, Fit FIT>
 __global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_fwd_kernel(KgsAddNorm a) {
   __shared__ float slots[2 * 16];
   int turn = 0;
   const Place<WAVES> at(a.width);
   const int C = a.width;
-  const T *residual = static_cast<const T*>(a.residual), *branch = static_cast<const T*>(a.branch);
+  const int size = FIT == kTiny ? C : kV;  // elements a chunk has
+  int skip[NV];
+  uint32_t column[NV];  // in bytes
   float w[NV][kV], pw[FULL ? NV : 1][kV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (at.t + i * at.lanes) * kV;
-    load(w[i], static_cast<const T*>(a.weight) + c, C - c);
+    const int c = at.column(i, C);
+    column[i] = c * sizeof(T);
+    skip[i] = at.skip(i, C);
+    load(w[i], static_cast<const T*>(a.weight) + c, size);
     if constexpr (FULL) {  // what the normalised branch is multiplied by
       for (float& x : pw[i]) x = a.scale;
       float f[kV];
       if (a.post_weight) {
-        load(f, static_cast<const T*>(a.post_weight) + c, C - c);
+        load(f, static_cast<const T*>(a.post_weight) + c, size);
         for (int j = 0; j < kV; ++j) pw[i][j] *= f[j];
       }
       if (a.gate) {
-        load(f, static_cast<const T*>(a.gate) + c, C - c);
+        load(f, static_cast<const T*>(a.gate) + c, size);
         for (int j = 0; j < kV; ++j) pw[i][j] *= f[j];
       }
     }
   }
+  // an element's part in a sum
+  const auto part = [&](int i, int j, float x) { return (FIT == kWhole ? skip[i] : j < skip[i]) ? 0.f : x; };
   const int step = gridDim.x * at.rows;
   for (int row = blockIdx.x * at.rows + at.row; row < a.rows; row += step) {
     float s[NV][kV], b[NV][kV];
     float sq = 0.f, rb = 1.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (at.t + i * at.lanes) * kV;
-      load(b[i], branch + row * a.branch_ld + c, C - c);
-      load(s[i], residual + row * a.residual_ld + c, C - c);
+      load(b[i], place<T>(a.branch, row * a.branch_ld, column[i]), size);
+      load(s[i], place<T>(a.residual, row * a.residual_ld, column[i]), size);
     }
     if constexpr (FULL) {
       if (a.post_weight) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int j = 0; j < kV; ++j) sq = fmaf(b[i][j], b[i][j], sq);
+          for (int j = 0; j < kV; ++j) sq = fmaf(b[i][j], part(i, j, b[i][j]), sq);
         rb = 1.f / sqrtf(row_sum<WAVES>(sq, at.lanes, slots, turn) / C + a.eps);
         sq = 0.f;
       }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (at.t + i * at.lanes) * kV;
 #pragma unroll
       for (int j = 0; j < kV; ++j) {
         if constexpr (FULL) s[i][j] = fmaf(pw[i][j], b[i][j] * rb, s[i][j]);
         else s[i][j] += b[i][j];
-        sq = fmaf(s[i][j], s[i][j], sq);
+        sq = fmaf(s[i][j], part(i, j, s[i][j]), sq);
       }
-      store(s[i], static_cast<T*>(a.stream) + row * a.stream_ld + c, C - c);
+      if (skip[i] < kV) store(s[i], place<T>(a.stream, row * a.stream_ld, column[i]), size);
     }
     const float rs = 1.f / sqrtf(row_sum<WAVES>(sq, at.lanes, slots, turn) / C + a.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (at.t + i * at.lanes) * kV;
 #pragma unroll
       for (int j = 0; j < kV; ++j) s[i][j] *= rs * w[i][j];
-      store(s[i], static_cast<T*>(a.out) + static_cast<int64_t>(row) * C + c, C - c);
+      if (skip[i] < kV) store(s[i], place<T>(a.out, static_cast<int64_t>(row) * C, column[i]), size);
     }
     if (a.rstd && at.t == 0) {
       a.rstd[row] = rs;
@@ -187,10 +216,8 @@ template <class T> __device__ __forceinline__ void finish(const KgsAddNorm& a, i
 
 // The next row's loads are under way while this one is reduced; with one chunk a thread
 // that fits the registers of 16 waves a CU.  Two chunks (rows over 8192 wide) do without,
-// and read the weights again for every row.  WHOLE: the width is a multiple of 8, so that
-// a chunk is there or not: a thread past the end reads the row's first chunk, without a
-// branch, and its zero weights keep it out of the sums.
-template <class T, bool WAVES, int NV, bool FULL, bool WHOLE, int THREADS>
+// and read the weights again for every row.
+template <class T, bool WAVES, int NV, bool FULL, Fit FIT, int THREADS>
 __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
   __shared__ float slots[2 * 16];
   __shared__ float sums[WAVES ? (FULL ? 2 : 1) * 4 * 512 : 1];
@@ -198,44 +225,52 @@ __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
   int turn = 0;
   const Place<WAVES> at(a.width);
   const int C = a.width;
-  const auto column = [&](int i) { return (at.t + i * at.lanes) * kV; };
-  const auto get = [&](Loose<T>& r, const void* p, int64_t start, int c) {
-    const T* from = static_cast<const T*>(p) + start;
-    if constexpr (WHOLE) r = *reinterpret_cast<const Loose<T>*>(from + (c < C ? c : 0));
-    else load_raw(r, from, c, C - c);
+  const int size = FIT == kTiny ? C : kV;
+  int skip[NV];
+  uint32_t column[NV];  // in bytes
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    column[i] = at.column(i, C) * sizeof(T);
+    skip[i] = at.skip(i, C);
+  }
+  // an element's part in a sum; of whole chunks zero weights leave out a thread past the end
+  const auto part_of = [&](int i, int j, float x) { return FIT != kWhole && j < skip[i] ? 0.f : x; };
+  const auto get = [&](Loose<T>& r, const void* p, int64_t start, uint32_t column) {
+    load_raw(r, place<T>(p, start, column), size);
   };
   // For residual and branch: last read by the forward pass, they are not in a cache, and
   // are not kept in one (8192 x 4096: 69 us to 61 us, all weights 88 us to 75 us; with the
   // gradients read so too, which the pass before has just written, 47 us for 45 us at a
-  // size that the caches hold).
-  const auto get_once = [&](Loose<T>& r, const void* p, int64_t start, int c) {
-    if constexpr (WHOLE) {
+  // size that the caches hold).  Ragged rows share lines with their neighbours, which are
+  // better kept (30000 x 537: 56 us, kept 43 us).
+  const auto get_once = [&](Loose<T>& r, const void* p, int64_t start, uint32_t column) {
+    if constexpr (FIT == kWhole) {
       typedef T V8 __attribute__((ext_vector_type(kV), aligned(sizeof(T))));
-      const V8 x = __builtin_nontemporal_load(reinterpret_cast<const V8*>(static_cast<const T*>(p) + start + (c < C ? c : 0)));
+      const V8 x = __builtin_nontemporal_load(reinterpret_cast<const V8*>(place<T>(p, start, column)));
 #pragma unroll
       for (int j = 0; j < kV; ++j) r.v[j] = x[j];
     } else {
-      get(r, p, start, c);
+      get(r, p, start, column);
     }
   };
-  // weight, and scale post_weight gate; zero past the end
+  // weight, and scale post_weight gate
   float w[NV][kV], full[FULL ? NV : 1][kV];
   const auto weights = [&] {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = column(i);
-      load(w[i], static_cast<const T*>(a.weight) + c, C - c);
+      const int c = at.column(i, C);
+      load(w[i], static_cast<const T*>(a.weight) + c, FIT == kWhole && skip[i] ? 0 : size);
       if constexpr (FULL) {
         float f[kV];
 #pragma unroll
-        for (int j = 0; j < kV; ++j) full[i][j] = c + j < C ? a.scale : 0.f;
+        for (int j = 0; j < kV; ++j) full[i][j] = FIT == kWhole && skip[i] ? 0.f : a.scale;
         if (a.post_weight) {
-          load(f, static_cast<const T*>(a.post_weight) + c, C - c);
+          load(f, static_cast<const T*>(a.post_weight) + c, size);
 #pragma unroll
           for (int j = 0; j < kV; ++j) full[i][j] *= f[j];
         }
         if (a.gate) {
-          load(f, static_cast<const T*>(a.gate) + c, C - c);
+          load(f, static_cast<const T*>(a.gate) + c, size);
 #pragma unroll
           for (int j = 0; j < kV; ++j) full[i][j] *= f[j];
         }
@@ -252,10 +287,10 @@ __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
     next.rb = FULL ? a.rstd[a.rows + row] : 1.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      get_once(next.s[i], a.residual, row * a.residual_ld, column(i));
-      get_once(next.b[i], a.branch, row * a.branch_ld, column(i));
-      if (a.dout) get(next.dy[i], a.dout, row * a.dout_ld, column(i));
-      if (a.dstream) get(next.ds[i], a.dstream, row * a.dstream_ld, column(i));
+      get_once(next.s[i], a.residual, row * a.residual_ld, column[i]);
+      get_once(next.b[i], a.branch, row * a.branch_ld, column[i]);
+      if (a.dout) get(next.dy[i], a.dout, row * a.dout_ld, column[i]);
+      if (a.dstream) get(next.ds[i], a.dstream, row * a.dstream_ld, column[i]);
     }
   };
 #pragma unroll
@@ -289,23 +324,22 @@ __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
         }
         dw[i][j] = fmaf(g, s[i][j], dw[i][j]);
         dy[i][j] = g * w[i][j];
-        dot = fmaf(dy[i][j], s[i][j], dot);
+        dot = fmaf(dy[i][j], part_of(i, j, s[i][j]), dot);
       }
     if (kAhead && row + step < a.rows) fetch(row + step);
     const float mean = row_sum<WAVES>(dot, at.lanes, slots, turn) / C;
     float dot2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = column(i);
 #pragma unroll
       for (int j = 0; j < kV; ++j) ds[i][j] = fmaf(rs, dy[i][j] - s[i][j] * mean, ds[i][j]);
-      store(ds[i], static_cast<T*>(a.dresidual) + static_cast<int64_t>(row) * C + c, C - c);
+      if (skip[i] < kV) store(ds[i], place<T>(a.dresidual, static_cast<int64_t>(row) * C, column[i]), size);
       if constexpr (FULL) {
 #pragma unroll
         for (int j = 0; j < kV; ++j) {
           sum[i][j] = fmaf(ds[i][j], b[i][j], sum[i][j]);
           ds[i][j] *= full[i][j];
-          dot2 = fmaf(ds[i][j], b[i][j], dot2);
+          dot2 = fmaf(ds[i][j], part_of(i, j, b[i][j]), dot2);
         }
       }
     }
@@ -313,55 +347,48 @@ __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
       const float mean2 = a.post_weight ? row_sum<WAVES>(dot2, at.lanes, slots, turn) / C : 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = column(i);
 #pragma unroll
         for (int j = 0; j < kV; ++j) ds[i][j] = rb * (ds[i][j] - b[i][j] * mean2);
-        store(ds[i], static_cast<T*>(a.dbranch) + static_cast<int64_t>(row) * C + c, C - c);
+        if (skip[i] < kV) store(ds[i], place<T>(a.dbranch, static_cast<int64_t>(row) * C, column[i]), size);
       }
     }
   }
-  // This workgroup's column sums: a part, or, if it is the only one, the results.
+  // This workgroup's column sums: a part, and if it is the only one, the results.
   float* part = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * C;
-  const bool only = gridDim.x == 1;
   if constexpr (WAVES) {
     // over the wave's rows, then over the four waves
-    const int n = at.lanes * kV, wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, c = at.column(0, C);
 #pragma unroll
     for (int j = 0; j < kV; ++j) {
       for (int m = at.lanes; m < 64; m <<= 1) {
         dw[0][j] += __shfl_xor(dw[0][j], m, 64);
         if constexpr (FULL) sum[0][j] += __shfl_xor(sum[0][j], m, 64);
       }
-      if ((threadIdx.x & 63) < at.lanes) {
-        sums[wave * 512 + at.t * kV + j] = dw[0][j];
-        if constexpr (FULL) sums[(4 + wave) * 512 + at.t * kV + j] = sum[0][j];
+      if ((threadIdx.x & 63) < at.lanes && skip[0] < kV) {
+        sums[wave * 512 + c + j] = dw[0][j];
+        if constexpr (FULL) sums[(4 + wave) * 512 + c + j] = sum[0][j];
       }
     }
     __syncthreads();
     for (int v = 0; v < (FULL ? 2 : 1); ++v)
-      for (int c = threadIdx.x; c < n && c < C; c += 256) {
+      for (int c = threadIdx.x; c < C; c += 256) {
         const float* x = sums + v * 4 * 512 + c;
-        const float total = (x[0] + x[512]) + (x[1024] + x[1536]);
-        if (only) finish<T>(a, v, c, total);
-        else part[v * C + c] = total;
+        part[v * C + c] = (x[0] + x[512]) + (x[1024] + x[1536]);
       }
   } else {
+    // (where chunks overlap, two threads have summed the same and write the same)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = column(i);
-      if (only) {
-#pragma unroll
-        for (int j = 0; j < kV; ++j)
-          if (c + j < C) {
-            finish<T>(a, 0, c + j, dw[i][j]);
-            if constexpr (FULL) finish<T>(a, 1, c + j, sum[i][j]);
-          }
-      } else {
-        store(dw[i], part + c, C - c);
-        if constexpr (FULL) store(sum[i], part + C + c, C - c);
-      }
+      const int c = at.column(i, C);
+      if (skip[i] == kV) continue;
+      store(dw[i], part + c, size);
+      if constexpr (FULL) store(sum[i], part + C + c, size);
     }
   }
+  if (gridDim.x > 1) return;
+  __syncthreads();
+  for (int v = 0; v < (FULL && (a.dpost_weight || a.dgate) ? 2 : 1); ++v)
+    for (int c = threadIdx.x; c < C; c += blockDim.x) finish<T>(a, v, c, part[v * C + c]);
 }
 
 // Column sums of the parts: 16 columns a workgroup, 64 threads a column.
@@ -395,25 +422,27 @@ template <class T, bool WAVES, int NV> int forward(const KgsAddNorm& a, hipStrea
   int threads, rows;
   shape<WAVES, NV>(a, threads, rows);
   const int want = (a.rows + rows - 1) / rows, grid = want < 8192 ? want : 8192;
-  if (is_full(a)) add_norm_fwd_kernel<T, WAVES, NV, true><<<grid, threads, 0, s>>>(a);
-  else add_norm_fwd_kernel<T, WAVES, NV, false><<<grid, threads, 0, s>>>(a);
+  const auto go = [&](auto kernel) { kernel<<<grid, threads, 0, s>>>(a); };
+  const bool full = is_full(a);
+  if (a.width % kV == 0) full ? go(add_norm_fwd_kernel<T, WAVES, NV, true, kWhole>) : go(add_norm_fwd_kernel<T, WAVES, NV, false, kWhole>);
+  else if (a.width > kV) full ? go(add_norm_fwd_kernel<T, WAVES, NV, true, kRagged>) : go(add_norm_fwd_kernel<T, WAVES, NV, false, kRagged>);
+  else if constexpr (WAVES) full ? go(add_norm_fwd_kernel<T, WAVES, NV, true, kTiny>) : go(add_norm_fwd_kernel<T, WAVES, NV, false, kTiny>);
   return launched("add_norm forward");
 }
 
-template <class T, bool WAVES, int NV, bool WHOLE, int THREADS> int backward(const KgsAddNorm& a, hipStream_t s) {
+template <class T, bool WAVES, int NV, int THREADS> int backward(const KgsAddNorm& a, hipStream_t s) {
   int threads, rows;
   shape<WAVES, NV>(a, threads, rows);
-  if (is_full(a)) add_norm_bwd_kernel<T, WAVES, NV, true, WHOLE, THREADS><<<a.parts, threads, 0, s>>>(a);
-  else add_norm_bwd_kernel<T, WAVES, NV, false, WHOLE, THREADS><<<a.parts, threads, 0, s>>>(a);
+  const auto go = [&](auto kernel) { kernel<<<a.parts, threads, 0, s>>>(a); };
+  const bool full = is_full(a);
+  if (a.width % kV == 0) full ? go(add_norm_bwd_kernel<T, WAVES, NV, true, kWhole, THREADS>) : go(add_norm_bwd_kernel<T, WAVES, NV, false, kWhole, THREADS>);
+  else if (a.width > kV) full ? go(add_norm_bwd_kernel<T, WAVES, NV, true, kRagged, THREADS>) : go(add_norm_bwd_kernel<T, WAVES, NV, false, kRagged, THREADS>);
+  else if constexpr (WAVES) full ? go(add_norm_bwd_kernel<T, WAVES, NV, true, kTiny, THREADS>) : go(add_norm_bwd_kernel<T, WAVES, NV, false, kTiny, THREADS>);
   if (launched("add_norm backward")) return -1;
   if (a.parts == 1) return 0;
   const bool second = a.dpost_weight || a.dgate;
   add_norm_join_kernel<T><<<dim3((a.width + 15) / 16, second ? 2 : 1), 1024, 0, s>>>(a);
   return launched("add_norm join");
-}
-
-template <class T, bool WAVES, int NV, int THREADS> int backward(const KgsAddNorm& a, hipStream_t s) {
-  return a.width % kV ? backward<T, WAVES, NV, false, THREADS>(a, s) : backward<T, WAVES, NV, true, THREADS>(a, s);
 }
 
 template <class T> int run(const KgsAddNorm& a, bool back, hipStream_t s) {
@@ -433,7 +462,7 @@ int dispatch(const KgsAddNorm* a, bool back, void* stream) {
   if (back && (!a->rstd || !a->dresidual || !a->dbranch || !a->dweight)) return fail(w, "a tensor is missing");
   if (back && ((a->post_weight && !a->dpost_weight) || (a->gate && !a->dgate))) return fail(w, "a tensor is missing");
   if (a->rows <= 0 || a->rows >= 1 << 30 || a->width <= 0 || a->width > 16384) return fail(w, "bad sizes");
-  if (back && (a->parts < 1 || a->parts > 65536 || (a->parts > 1 && !a->partial))) return fail(w, "bad parts");
+  if (back && (a->parts < 1 || a->parts > 65536 || !a->partial)) return fail(w, "bad parts");
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->type) {
     case 0: return run<bf16>(*a, back, s);

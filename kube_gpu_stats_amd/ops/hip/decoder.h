@@ -41,8 +41,8 @@ struct KgsSwiglu {
 
 // Rows of `width` elements; row strides in elements.  rstd float [2, rows] (of the stream, of
 // the branch); dstream and dout may be null (zero).  post_weight and gate may be null.
-// partial: float [parts, 2, width], parts the workgroups of the backward
-// (null if one).  dbranch may equal dresidual where they are the same.
+// partial: float [parts, 2, width], parts the workgroups of the backward.
+// dbranch may equal dresidual where they are the same.
 struct KgsAddNorm {
   const void *residual, *branch, *weight, *post_weight, *gate;
   void *stream, *out;
