@@ -72,16 +72,25 @@ def _here(t, stream) -> bool:
     return stream is None and t.get_device() == torch.cuda.current_device()
 
 
-def _there(t, stream, call):
-    """``call()`` with ``t``'s device and ``stream`` current: allocations and launches belong there."""
-    if stream is not None and stream.device != t.device:
-        raise ValueError(f"the stream is on {stream.device}, the tensors are on {t.device}")
+def _there(t, stream, call, *tensors):
+    """``call()`` with ``t``'s device and ``stream`` current: allocations and launches belong there.
+    On a given stream the call's ``tensors`` are not handed out again before it is through."""
+    if stream is not None:
+        if stream.device != t.device:
+            raise ValueError(f"the stream is on {stream.device}, the tensors are on {t.device}")
+        for x in (t, *tensors):
+            if x is not None:
+                x.record_stream(stream)
     with torch.cuda.device(t.device), torch.cuda.stream(stream):
         return call()
 
 
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+def _vector(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -140,7 +149,7 @@ def _heads(t):
 
 
 def _attention_checks(q, k, v, scale, lengths, back=None):
-    """(B, S, H, Hk, D, type, scale, lengths) of a call's tensors; ``back``: (dout, out, lse, low)."""
+    """(B, S, H, Hk, D, type, scale) of a call's tensors; ``back``: (dout, out, lse, low)."""
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         for t, name in ((q, "q"), (k, "k"), (v, "v")):
             if t.dim() != 4:
@@ -176,9 +185,8 @@ def _attention_checks(q, k, v, scale, lengths, back=None):
         _shape(lengths, "lengths", (B,))
         if lengths.get_device() != index:
             raise ValueError(f"lengths is on {lengths.device}, q is on {q.device}")
-        lengths = lengths.contiguous()
     _on_gpu(q, "q")
-    return B, S, H, Hk, D, code, scale, lengths
+    return B, S, H, Hk, D, code, scale
 
 
 def attention(q, k, v, *, causal: bool = True, scale: float | None = None, lengths=None):
@@ -226,9 +234,10 @@ def attention_fwd(q, k, v, *, causal: bool = True, scale: float | None = None, l
 
 
 def _attention_fwd(q, k, v, causal, scale, lengths, stream, keep):
-    B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths)
+    B, S, H, Hk, D, code, scale = _attention_checks(q, k, v, scale, lengths)
     if not _here(q, stream):
-        return _there(q, stream, lambda: _attention_fwd(q, k, v, causal, scale, lengths, None, keep))
+        return _there(q, stream, lambda: _attention_fwd(q, k, v, causal, scale, lengths, None, keep), k, v, lengths)
+    lengths = _vector(lengths)
     (q, qs), (k, ks), (v, vs) = _heads(q), _heads(k), _heads(v)
     out = q.new_empty((B, S, H, D))
     lse = low = None
@@ -262,9 +271,11 @@ def attention_bwd(dout, q, k, v, out, saved, *, causal: bool = True, scale: floa
 
 
 def _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, stream, into):
-    B, S, H, Hk, D, code, scale, lengths = _attention_checks(q, k, v, scale, lengths, (dout, out, lse, low))
+    B, S, H, Hk, D, code, scale = _attention_checks(q, k, v, scale, lengths, (dout, out, lse, low))
     if not _here(q, stream):
-        return _there(q, stream, lambda: _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, None, into))
+        return _there(q, stream, lambda: _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, None, into),
+                      k, v, dout, out, lse, low, lengths)
+    lengths = _vector(lengths)
     (q, qs), (k, ks), (v, vs), (out, os_), (dout, gs) = _heads(q), _heads(k), _heads(v), _heads(out), _heads(dout)
     if into is None:
         into = q.new_empty((B, S, H, D)), q.new_empty((B, S, Hk, D)), q.new_empty((B, S, Hk, D))
@@ -379,7 +390,7 @@ def swiglu_fwd(x, w, *, stream=None):
 def _swiglu_fwd(x, w, stream, keep):
     T, K, F, code = _swiglu_checks(x, w)
     if not _here(x, stream):
-        return _there(x, stream, lambda: _swiglu_fwd(x, w, None, keep))
+        return _there(x, stream, lambda: _swiglu_fwd(x, w, None, keep), w)
     lead = x.shape[:-1]
     h = x.new_empty((*lead, F))
     saved = torch.empty((*lead, 6 * F), dtype=torch.uint8, device=x.device) if keep else None
@@ -401,7 +412,7 @@ def swiglu_bwd(dh, x, w, saved, *, stream=None):
 def _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, stream):
     T, K, F, code = _swiglu_checks(x, w, dh, saved)
     if not _here(x, stream):
-        return _there(x, stream, lambda: _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, None))
+        return _there(x, stream, lambda: _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, None), w, dh, saved)
     dx = x.new_empty(x.shape) if want_dx else None
     dw = (w.new_empty if T else w.new_zeros)(w.shape) if want_dw else None
     if T and (want_dx or want_dw):
@@ -461,10 +472,6 @@ def _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps):
     return T, C, code
 
 
-def _vector(t):
-    return t if t is None or t.is_contiguous() else t.contiguous()
-
-
 def add_norm(residual, branch, weight, *, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-6):
     """(stream, out): stream = residual + scale · gate · norm(branch), out = norm(stream).
 
@@ -491,7 +498,8 @@ def _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, strea
     T, C, code = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps)
     if not _here(residual, stream):
         return _there(residual, stream,
-                      lambda: _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, keep))
+                      lambda: _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, keep),
+                      branch, weight, post_weight, gate)
     s, out = residual.new_empty(residual.shape), residual.new_empty(residual.shape)
     saved = torch.empty(2, T, dtype=torch.float32, device=residual.device) if keep else None
     if T:
@@ -534,8 +542,10 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
             _same(residual, "residual", **{name: t})
     _kept(saved, "saved", torch.float32, (2, T), residual.get_device(), "add_norm_fwd")
     if not _here(residual, stream):
-        return _there(residual, stream, lambda: add_norm_bwd(dstream, dout, residual, branch, weight, saved, eps=eps,
-                                                            post_weight=post_weight, gate=gate, scale=scale))
+        return _there(residual, stream,
+                      lambda: add_norm_bwd(dstream, dout, residual, branch, weight, saved, post_weight=post_weight,
+                                           gate=gate, scale=scale, eps=eps),
+                      dstream, dout, branch, weight, saved, post_weight, gate)
     dr = residual.new_empty(residual.shape)
     db = residual.new_empty(residual.shape) if post_weight is not None or gate is not None or scale != 1.0 else dr
     new = weight.new_empty if T else weight.new_zeros

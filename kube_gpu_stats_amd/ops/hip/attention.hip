@@ -592,7 +592,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
 template <class T, int D>
 __global__ __launch_bounds__(256) void attention_join_kernel(KgsAttention a) {
   using x4 = typename El<T>::x4;
-  const int64_t part = static_cast<int64_t>(a.B) * a.S * a.Hk * D, i = (blockIdx.x * 256ll + threadIdx.x) * 4;
+  const int64_t part = static_cast<int64_t>(a.B) * a.S * a.Hk * D;
+  const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4;  // under 2^28 parts of 4: splits are of few keys
   if (i >= 2 * part) return;
   const bool v = i >= part;
   const int64_t e = v ? i - part : i;
@@ -623,9 +624,10 @@ int check(const KgsAttention* a, bool backward) {
       // rows behind the last lie past the descriptor's end; offsets inside a tile stay under 2^30
       if (st[i][j] < 0 || st[i][j] % 8 || (j == 1 && (st[i][j] < a->D || st[i][j] > (1 << 22)))) return fail(w, "unsupported strides");
   if (a->H > (1 << 18)) return fail(w, "too many heads");  // offsets inside a tile of low
-  // workgroups, and the products of counts that head_item forms, stay under 2^31
-  const int64_t tiles = (a->S + 127) / 128;
-  if ((tiles + 16) * (static_cast<int64_t>(a->B) * a->H + 16) * (backward ? a->splits : 1) * 16 > 0x7FFFFFFFll)
+  // a launch has under 2^32 threads; the products of counts that head_item forms, 16 times
+  // its pieces at most, stay under 2^31
+  const int64_t tiles = (a->S + kRows - 1) / kRows;
+  if ((tiles + 16) * (static_cast<int64_t>(a->B) * a->H + 16) * (backward ? a->splits : 1) > (1 << 24) - 64)
     return fail(w, "too many workgroups");
   return 0;
 }

@@ -108,13 +108,13 @@ __device__ __forceinline__ void copy16(i32x4 d, int voff, uint32_t lds, int soff
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(d), "s"(soff)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ void copy4(i32x4 d, int voff, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(d)
-               : "memory");
+               : "memory", "m0");
 }
 // Waits until at most N of the wave's copies are under way.
 template <int N> __device__ __forceinline__ void copies_left() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }

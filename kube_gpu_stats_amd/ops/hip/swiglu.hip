@@ -321,23 +321,23 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_kernel(Product p) {
 template <class T, bool PAIR> __global__ __launch_bounds__(256) void join_kernel(Product p) {
   using x4 = typename El<T>::x4;
   const int N = PAIR ? p.N / 2 : p.N;
-  const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4;
-  if (i >= static_cast<int64_t>(p.M) * N) return;
-  const int64_t m = i / N, n = i % N, part = static_cast<int64_t>(p.M) * p.N;
-  f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-  const float* from = p.partial + m * p.N + n;
-  for (int s = 0; s < p.splits; ++s) {
-    x += *reinterpret_cast<const f32x4*>(from + s * part);
-    if (PAIR) y += *reinterpret_cast<const f32x4*>(from + s * part + N);
-  }
-  x4 h;
+  for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < static_cast<int64_t>(p.M) * N; i += gridDim.x * 1024ll) {
+    const int64_t m = i / N, n = i % N, part = static_cast<int64_t>(p.M) * p.N;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+    const float* from = p.partial + m * p.N + n;
+    for (int s = 0; s < p.splits; ++s) {
+      x += *reinterpret_cast<const f32x4*>(from + s * part);
+      if (PAIR) y += *reinterpret_cast<const f32x4*>(from + s * part + N);
+    }
+    x4 h;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) h[j] = static_cast<T>(PAIR ? x[j] * sigmoid(x[j]) * y[j] : x[j]);
-  *reinterpret_cast<x4*>(static_cast<T*>(p.c) + i) = h;
-  if (PAIR && p.saved) {
-    const Saved to(p.saved, m, p.N);
-    to.store(n, x);
-    to.store(N + n, y);
+    for (int j = 0; j < 4; ++j) h[j] = static_cast<T>(PAIR ? x[j] * sigmoid(x[j]) * y[j] : x[j]);
+    *reinterpret_cast<x4*>(static_cast<T*>(p.c) + i) = h;
+    if (PAIR && p.saved) {
+      const Saved to(p.saved, m, p.N);
+      to.store(n, x);
+      to.store(N + n, y);
+    }
   }
 }
 
@@ -345,22 +345,26 @@ template <class T, bool PAIR> __global__ __launch_bounds__(256) void join_kernel
 template <class T> __global__ __launch_bounds__(256) void gate_bwd_kernel(const T* dh, int64_t dh_ld, uint8_t* saved, T* d,
                                                                          int M, int F) {
   using x4 = typename El<T>::x4;
-  const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4;
-  if (i >= static_cast<int64_t>(M) * F) return;
-  const int64_t m = i / F, n = i % F;
-  const x4 a = *reinterpret_cast<const x4*>(dh + m * dh_ld + n);
-  const Saved from(saved, m, 2 * F);
-  const f32x4 g = from.load(n), u = from.load(F + n);
-  x4 dg, du;
+  for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < static_cast<int64_t>(M) * F; i += gridDim.x * 1024ll) {
+    const int64_t m = i / F, n = i % F;
+    const x4 a = *reinterpret_cast<const x4*>(dh + m * dh_ld + n);
+    const Saved from(saved, m, 2 * F);
+    const f32x4 g = from.load(n), u = from.load(F + n);
+    x4 dg, du;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float grad = static_cast<float>(a[j]), s = sigmoid(g[j]);
-    dg[j] = static_cast<T>(grad * u[j] * s * (1.f + g[j] * (1.f - s)));
-    du[j] = static_cast<T>(grad * g[j] * s);
+    for (int j = 0; j < 4; ++j) {
+      const float grad = static_cast<float>(a[j]), s = sigmoid(g[j]);
+      dg[j] = static_cast<T>(grad * u[j] * s * (1.f + g[j] * (1.f - s)));
+      du[j] = static_cast<T>(grad * g[j] * s);
+    }
+    *reinterpret_cast<x4*>(d + m * 2 * F + n) = dg;
+    *reinterpret_cast<x4*>(d + m * 2 * F + F + n) = du;
   }
-  *reinterpret_cast<x4*>(d + m * 2 * F + n) = dg;
-  *reinterpret_cast<x4*>(d + m * 2 * F + F + n) = du;
 }
+
+// Workgroups of 256 threads for n items, of which a thread takes more than one if they are
+// over 2^28 (a launch has under 2^32 threads).
+unsigned blocks(int64_t n) { return static_cast<unsigned>(n < (1 << 28) ? (n + 255) / 256 : 1 << 20); }
 
 template <class T, int BM, int BN, int WM, int WN, bool TA, bool TB, bool PAIR>
 int product_tiled(const Product& p, hipStream_t s) {
@@ -373,12 +377,12 @@ int product_tiled(const Product& p, hipStream_t s) {
   }
   const int N = PAIR ? p.N / 2 : p.N, bn = PAIR ? BN / 2 : BN;
   const int64_t total = static_cast<int64_t>((p.M + BM - 1) / BM) * ((N + bn - 1) / bn) * p.splits;
-  if (total > 0x7FFFFF00ll) return fail("swiglu", "too many workgroups");
+  if (total > (1 << 22)) return fail("swiglu", "too many workgroups");  // under 2^32 threads
   kernel<<<static_cast<unsigned>((total + 7) / 8 * 8), WM * WN * 64, kLds, s>>>(p);
   if (launched("swiglu product")) return -1;
   if (p.splits > 1) {
     const int64_t n = static_cast<int64_t>(p.M) * N / 4;
-    join_kernel<T, PAIR><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(p);
+    join_kernel<T, PAIR><<<blocks(n), 256, 0, s>>>(p);
     return launched("swiglu join");
   }
   return 0;
@@ -401,7 +405,7 @@ template <class T> int forward(const KgsSwiglu& a, hipStream_t s) {
 
 template <class T> int backward(const KgsSwiglu& a, hipStream_t s) {
   const int64_t n = static_cast<int64_t>(a.T) * a.F / 4;
-  gate_bwd_kernel<T><<<static_cast<unsigned>((n + 255) / 256), 256, 0, s>>>(
+  gate_bwd_kernel<T><<<blocks(n), 256, 0, s>>>(
       static_cast<const T*>(a.dh), a.dh_ld, static_cast<uint8_t*>(a.saved), static_cast<T*>(a.dgu), a.T, a.F);
   if (launched("swiglu gate backward")) return -1;
   if (a.dx) {

@@ -718,6 +718,41 @@ def test_graph_replays(dev):
 
 
 @gpu
+@pytest.mark.parametrize("tile,T", [(0, 300), (1, 300), (2, 9)])
+def test_graph_of_every_tile(dev, monkeypatch, tile, T):
+    """Products whose workgroups take more LDS than a launch has by default, captured before they ever ran."""
+    monkeypatch.setattr(decoder, "_product_plan", lambda M, N, K, forward=False: (tile if forward or tile != 2 else 0, 2))
+    x, w, dh = swiglu_inputs(T, 328, 264, F16, dev, seed=6)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        h, saved = decoder.swiglu_fwd(x, w)
+        got = (h, *decoder.swiglu_bwd(dh, x, w, saved))
+    for seed in (6, 7, 8):
+        y = swiglu_inputs(T, 328, 264, F16, dev, seed=seed)
+        for a, b in zip((x, w, dh), y):
+            a.copy_(b)
+        g.replay()
+        torch.cuda.synchronize()
+        h, saved = decoder.swiglu_fwd(*y[:2])
+        assert all(torch.equal(p, q) for p, q in zip(got, (h, *decoder.swiglu_bwd(y[2], *y[:2], saved))))
+
+
+@gpu
+def test_strided_lengths_and_stream(dev):
+    """lengths of any stride, with a given stream: its copy belongs to that stream too."""
+    q, k, v, do = attention_inputs(3, 70, 2, 2, 64, BF16, dev)
+    both = torch.tensor([[70, 1], [13, 2], [0, 3]], dtype=torch.int32, device=dev)
+    want = decoder.attention(q, k, v, lengths=both[:, 0].contiguous())
+    assert torch.equal(decoder.attention(q, k, v, lengths=both[:, 0]), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    out, saved = decoder.attention_fwd(q, k, v, lengths=both[:, 0], stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, want)
+
+
+@gpu
 def test_autograd_step_captured(dev):
     """A forward and backward pass of the differentiable forms in a graph, no eager graph of the leaves alive."""
     x, w, dh = swiglu_inputs(40, 64, 48, BF16, dev)
