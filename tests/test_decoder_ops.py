@@ -5,6 +5,7 @@ step of the tensors' type, every rounded operand of a sum adds u times that term
 magnitude, every 32-bit sum of n terms at most n 2^-24 times the sum of magnitudes, the
 rounded result u times itself.  The bounds are computed in 64 bits beside the reference.
 """
+import gc
 import math
 
 import pytest
@@ -124,7 +125,9 @@ def attention_check(q, k, v, do, causal, lengths=None, scale=None):
 @pytest.fixture(scope="module")
 def dev():
     assert torch.cuda.is_available(), "GPU tests need a GPU"
-    return torch.device("cuda", 0)
+    yield torch.device("cuda", 0)
+    gc.collect()
+    torch.cuda.empty_cache()  # other modules measure the GPU's memory
 
 
 gpu = pytest.mark.gpu
