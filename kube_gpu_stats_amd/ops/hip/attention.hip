@@ -220,11 +220,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
-    mx = fmaxf(mx, other_half(mx)) * c;
+    mx *= c;
     // The subtracted maximum may lag by a factor of 2^8: the quotient is the same, and
-    // the accumulators are rescaled a few times a row instead of at every step.
+    // the accumulators are rescaled a few times a row instead of at every step.  Until then
+    // each half of the lanes looks at its own keys only (1 x 16384, 8 heads: 560 us to 538 us).
     if (__any(mx > top + 8.f)) {
-      const float now = fmaxf(top, mx), f = __builtin_amdgcn_exp2f(top - now);
+      const float now = fmaxf(top, fmaxf(mx, other_half(mx))), f = __builtin_amdgcn_exp2f(top - now);
       top = now;
       sum *= f;
 #pragma unroll

@@ -190,6 +190,19 @@ def test_attention_large_scores(dev):
 
 
 @gpu
+@pytest.mark.parametrize("four", [0, 4])
+def test_attention_scores_rising_in_turn(dev, four):
+    """Keys whose scores rise lie in every other group of four, which half of a wave's lanes see."""
+    q, k, v, do = attention_inputs(1, 333, 2, 1, 64, F16, dev, seed=4)
+    j = torch.arange(333, device=dev)
+    ramp = torch.where((j & 4) == four, j / 333.0 * 30, torch.zeros_like(j, dtype=torch.float32))
+    k = (k.float() * 0.1 + ramp[None, :, None, None] * (torch.arange(64, device=dev) % 2)).to(F16)
+    q = (q.float() * 0.1 + 0.3 * (torch.arange(64, device=dev) % 2)).to(F16)
+    for causal in (True, False):
+        attention_check(q, k, v, do, causal)
+
+
+@gpu
 def test_attention_layouts(dev):
     """Views of a packed projection, heads before positions, expanded heads, odd strides, loose pointers."""
     B, S, H, Hk, D = 2, 77, 4, 2, 64
