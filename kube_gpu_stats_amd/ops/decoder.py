@@ -358,9 +358,9 @@ def _product_plan(M: int, N: int, K: int, forward: bool = False) -> tuple[int, i
     5.2 TB/s.  A round of workgroups has a start and an end of its own; the parts of a
     split sum are written and read as 32-bit numbers, at 4 TB/s, by one more launch; no
     plan is faster than reading and writing the operands once.  (2048 x 10752 over 2048:
-    115 us with 256 x 256, two rounds of which the second is a third full, and 103 us with
-    128 x 128; 8192 x 22016 over 4096: 1290 us and 1550 us; 5 x 22016 over 4096, weights
-    from memory: 37 us with 32 x 256 in 4 parts, 44 us with 128 x 128.)"""
+    110 us with 256 x 256, two rounds of which the second is a third full, and 95 us with
+    128 x 128; 8192 x 22016 over 4096: 1230 us and 1430 us; 5 x 22016 over 4096, weights
+    from memory: 38 us with 32 x 256 in 4 parts, 54 us with 128 x 128 in 3.)"""
     floor = 2 * (M * K + N * K + M * N) / 5.2e6
     best = None
     for tile, rows, columns, at_once, around in ((0, 128, 128, 512, 3.5), (1, 256, 256, 256, 8.0), (2, 32, 256, 512, 3.5)):

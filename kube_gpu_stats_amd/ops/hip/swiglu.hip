@@ -15,6 +15,12 @@
 // saved with 24 of them: rounded to 16 they would add as much error to dx and dw as the
 // rounding of dg and du, operands of the two products, which is not to be avoided, and
 // 32 cost a third more traffic.  Rounded besides those: the outputs.
+//
+// Bound by the matrix units (busy 56 % of the time, at the clock the power limit leaves),
+// by memory for few rows.  8192 x 4096, F = 11008, bf16: forward 1230 us (1200 TFLOP/s),
+// saving the projections 1320 us, dx 1290 us (1140), dW 1500 us (980: both operands read
+// transposed take about as many cycles at a lower clock), dg and du 205 us (5.3 TB/s).
+// 5 rows of the same, weights from memory: 38 us (4.8 TB/s), two launches.
 #include "decoder.h"
 #include "decoder_common.h"
 
