@@ -28,7 +28,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 import os
 import struct
 
@@ -116,6 +115,8 @@ def _same(first, name: str, **others) -> None:
 
 def _kept(t, name: str, dtype, shape, index: int, maker: str) -> None:
     """What a forward pass kept, come back as it was."""
+    if t is None:
+        raise TypeError(f"{name} must be the tensor that {maker} returned, not None")
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
         raise ValueError(f"{name} must be the tensor that {maker} returned: {dtype}, {tuple(shape)}, contiguous, "
                          f"not {t.dtype}, {tuple(t.shape)} on {t.device}")
@@ -177,8 +178,8 @@ def _attention_checks(q, k, v, scale, lengths, back=None):
     if S >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} positions, not {S}")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        raise ValueError(f"scale must be finite and positive, not {scale}")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 126:  # a 32-bit number, times log2 e too
+        raise ValueError(f"scale must be positive, from 2^-126 to 2^126, not {scale}")
     if lengths is not None:
         if lengths.dtype != torch.int32:
             raise TypeError(f"lengths must be int32, not {lengths.dtype}")
@@ -448,6 +449,7 @@ def _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, stream):
 # ---------------------------------------------------------------------------- add_norm
 
 MAX_NORM_WIDTH = 16384
+LARGEST = torch.finfo(torch.float32).max
 
 
 def _lines(t):
@@ -458,7 +460,8 @@ def _lines(t):
     return m, m.stride(0)
 
 
-def _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps):
+def _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps, back=None):
+    """(rows, width, type) of a call's tensors; ``back``: (dstream, dout, saved)."""
     if residual.dim() < 1:
         raise ValueError("residual must be [..., width], not a single value")
     shape, dtype, index = residual.shape, residual.dtype, residual.get_device()
@@ -478,10 +481,16 @@ def _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps):
     T = residual.numel() // C
     if T >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} rows, not {T}")
-    if not -math.inf < scale < math.inf:
-        raise ValueError(f"scale must be finite, not {scale}")
-    if not 0 <= eps < math.inf:
-        raise ValueError(f"eps must be finite and not negative, not {eps}")
+    if not -LARGEST <= scale <= LARGEST:
+        raise ValueError(f"scale must be a finite 32-bit number, not {scale}")
+    if not 0 <= eps <= LARGEST:
+        raise ValueError(f"eps must be a finite 32-bit number and not negative, not {eps}")
+    if back is not None:
+        for name, t in zip(("dstream", "dout"), back):
+            if t is not None:
+                _shape(t, name, shape)
+                _same(residual, "residual", **{name: t})
+        _kept(back[2], "saved", torch.float32, (2, T), index, "add_norm_fwd")
     _on_gpu(residual, "residual")
     return T, C, code
 
@@ -548,13 +557,7 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
     dresidual, the same tensor; gradients of absent weights are None."""
     if dstream is None and dout is None:
         raise ValueError("one of dstream and dout must be given")
-    T, C, code = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps)
-    shape = residual.shape
-    for name, t in (("dstream", dstream), ("dout", dout)):
-        if t is not None:
-            _shape(t, name, shape)
-            _same(residual, "residual", **{name: t})
-    _kept(saved, "saved", torch.float32, (2, T), residual.get_device(), "add_norm_fwd")
+    T, C, code = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps, (dstream, dout, saved))
     if not _here(residual, stream):
         return _there(residual, stream,
                       lambda: add_norm_bwd(dstream, dout, residual, branch, weight, saved, post_weight=post_weight,

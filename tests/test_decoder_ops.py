@@ -863,6 +863,9 @@ ATTENTION_REFUSED = [
     ("v's heads", lambda: decoder.attention(z(1, 4, 2, 64), z(1, 4, 2, 64), z(1, 4, 1, 64)), ValueError),
     ("scale", lambda: decoder.attention(*[z(1, 4, 2, 64)] * 3, scale=0.0), ValueError),
     ("scale", lambda: decoder.attention(*[z(1, 4, 2, 64)] * 3, scale=math.nan), ValueError),
+    ("scale", lambda: decoder.attention(*[z(1, 4, 2, 64)] * 3, scale=1e39), ValueError),
+    ("scale", lambda: decoder.attention(*[z(1, 4, 2, 64)] * 3, scale=1e-46), ValueError),
+    ("nothing kept", lambda: decoder.attention_bwd(*[z(1, 4, 2, 64)] * 5, (None, None)), TypeError),
     ("lengths type", lambda: decoder.attention(*[z(1, 4, 2, 64)] * 3, lengths=torch.tensor([4])), TypeError),
     ("lengths shape", lambda: decoder.attention(*[z(1, 4, 2, 64)] * 3, lengths=torch.tensor([4, 4], dtype=torch.int32)), ValueError),
     ("device", lambda: decoder.attention(*[z(1, 4, 2, 64)] * 3), ValueError),
@@ -900,18 +903,23 @@ NORM_REFUSED = [
     ("no width", lambda: decoder.add_norm(z(1, 0), z(1, 0), z(0)), ValueError),
     ("eps", lambda: decoder.add_norm(z(4, 64), z(4, 64), z(64), eps=-1.0), ValueError),
     ("scale", lambda: decoder.add_norm(z(4, 64), z(4, 64), z(64), scale=math.inf), ValueError),
+    ("scale", lambda: decoder.add_norm(z(4, 64), z(4, 64), z(64), scale=-1e39), ValueError),
+    ("eps", lambda: decoder.add_norm(z(4, 64), z(4, 64), z(64), eps=1e39), ValueError),
+    ("nothing kept", lambda: decoder.add_norm_bwd(z(4, 64), None, z(4, 64), z(4, 64), z(64), None), TypeError),
     ("device", lambda: decoder.add_norm(z(4, 64), z(4, 64), z(64)), ValueError),
     ("no gradient", lambda: decoder.add_norm_bwd(None, None, z(4, 64), z(4, 64), z(64), z(2, 4, t=F32)), ValueError),
     ("saved", lambda: decoder.add_norm_bwd(z(4, 64), None, z(4, 64), z(4, 64), z(64), z(4, 2, t=F32)), ValueError),
 ]
 
 
-@pytest.mark.parametrize("call,error", [pytest.param(c, e, id=f"{op} {n}") for op, cases in
+@pytest.mark.parametrize("name,call,error", [pytest.param(n, c, e, id=f"{op} {n}") for op, cases in
                                         (("attention", ATTENTION_REFUSED), ("swiglu", SWIGLU_REFUSED), ("add_norm", NORM_REFUSED))
                                         for n, c, e in cases])
-def test_refusals(call, error):
-    with pytest.raises(error):
+def test_refusals(name, call, error):
+    with pytest.raises(error) as raised:
         call()
+    # (where the tensors are is looked at last)
+    assert ("must be on a GPU" in str(raised.value)) == (name == "device")
 
 
 def test_plans_cover_their_ranges():
