@@ -299,6 +299,43 @@ def test_attention_empty(dev):
         assert all(x.shape == shape for x in decoder.attention_bwd(q, q, q, q, out, lse))
 
 
+@gpu
+def test_attention_far_apart(dev):
+    """Positions 8 MiB apart: a sequence spans more than 2^31 bytes."""
+    S, D = 300, 128
+    base = torch.empty(S, 1 << 22, dtype=BF16, device=dev)
+    views = []
+    for i, x in enumerate(attention_inputs(1, S, 2, 1, D, BF16, dev, seed=9)):
+        to = base[:, i * 1000 * 8:][:, :x.shape[2] * D].view(1, S, x.shape[2], D)
+        views.append(to.copy_(x))
+    assert views[0].stride(1) * S * 2 > 2 ** 31 and not views[0].is_contiguous()
+    for causal in (True, False):
+        attention_check(*views, causal)
+        attention_check(*views, causal, lengths=[271])
+
+
+@gpu
+def test_attention_long_padded(dev):
+    """Over 2^31 elements of mostly padding, which is NaN: not read, and zero in the results."""
+    B, S, H, D, ends = 2, (1 << 20) + 64, 16, 128, [70, 200]
+    full = lambda h: torch.full((B, S, h, D), math.nan, dtype=BF16, device=dev)  # noqa: E731
+    q, k, v, do = full(H), full(1), full(1), full(H)
+    small = attention_inputs(B, 200, H, 1, D, BF16, dev, seed=10)
+    for x, y in zip((q, k, v, do), small):
+        x[:, :200] = y
+        for b, n in enumerate(ends):
+            x[b, n:200] = math.nan
+            y[b, n:] = 0
+    kw = {"lengths": torch.tensor(ends, dtype=torch.int32, device=dev)}
+    out, saved = decoder.attention_fwd(q, k, v, **kw)
+    got = (out, *decoder.attention_bwd(do, q, k, v, out, saved, **kw))
+    ref, tol, _ = attention_oracle(*small, True, D ** -0.5, ends)
+    for name, x in zip(("out", "dq", "dk", "dv"), got):
+        close(x[:, :200], ref[name], tol[name], name)
+        for b in range(B):
+            assert not x[b, 200:].any()
+
+
 # ------------------------------------------------------------------------ swiglu's oracle
 
 def swiglu_oracle(x, w, dh):
@@ -425,6 +462,34 @@ def test_swiglu_extremes(dev):
     assert torch.isfinite(h).all() and torch.isfinite(dx).all() and torch.isfinite(dw).all()
     gd = w[:8].double().diagonal()
     assert torch.allclose(h.double().diagonal(), 2 * gd * torch.sigmoid(gd), rtol=2 ** -7, atol=1e-30)
+
+
+@gpu
+def test_swiglu_offsets(dev):
+    """Over 2^31 elements of h ; gradients of the last rows."""
+    T, K, F, n = 262147, 64, 8200, 5
+    g = torch.Generator(device=dev).manual_seed(11)
+    x = torch.randn(T, K, generator=g, device=dev).to(BF16)
+    w = (torch.randn(2 * F, K, generator=g, device=dev) * K ** -0.5).to(BF16)
+    dh = torch.zeros(T, F, dtype=BF16, device=dev)
+    dh[-n:] = torch.randn(n, F, generator=g, device=dev).to(BF16)
+    h, saved = decoder.swiglu_fwd(x, w)
+    dx, dw = decoder.swiglu_bwd(dh, x, w, saved)
+    rows = torch.cat([torch.arange(0, T - n, 26003), torch.arange(T - n, T)]).to(dev)
+    ref, tol = swiglu_oracle(x[rows], w, dh[rows])
+    for name, got in (("h", h[rows]), ("saved", projections(saved[rows])), ("dx", dx[rows]), ("dw", dw)):
+        close(got, ref[name], tol[name], name)
+
+
+@gpu
+def test_swiglu_far_apart(dev):
+    """Rows 4 MiB apart, over 2^31 bytes in all, of x and w."""
+    T, K, F = 600, 72, 296
+    x, w, dh = swiglu_inputs(T, K, F, BF16, dev, seed=12)
+    base = torch.empty(600, 1 << 21, dtype=BF16, device=dev)
+    far = [base[:len(t), i * 8000:][:, :t.shape[1]].copy_(t) for i, t in enumerate((x, w, dh))]
+    assert far[0].stride(0) * T * 2 > 2 ** 31
+    swiglu_check(*far)
 
 
 @gpu
@@ -596,6 +661,34 @@ def test_add_norm_zero_rows_and_layouts(dev):
             assert torch.equal(x, z)
     row = dy[:1].expand(12, 200)
     norm_check(r, b[:1].expand(12, 200), w, pw, gate, row, row)
+
+
+@gpu
+@pytest.mark.parametrize("C", [300, 1000])
+def test_add_norm_far_apart(dev, C):
+    """Rows 2 GiB apart."""
+    r, b, w, pw, gate, dS, dy = norm_inputs(3, C, BF16, dev, True, True, seed=13)
+    base = torch.empty(2 * (1 << 30) + 8192, dtype=BF16, device=dev)
+    far = [base[i * 1024 + 1:].as_strided((3, C), (1 << 30, 1)).copy_(t) for i, t in enumerate((r, b, dS, dy))]
+    norm_check(far[0], far[1], w, pw, gate, far[2], far[3])
+
+
+@gpu
+@pytest.mark.parametrize("T,C", [((1 << 21) + 3, 1024), ((1 << 26) + 3, 33)])
+def test_add_norm_offsets(dev, T, C):
+    """Over 2^31 elements; gradients of the last rows."""
+    n = 5
+    last = norm_inputs(n, C, BF16, dev, False, False, seed=14)
+    r, b, dS, dy = (torch.zeros(T, C, dtype=BF16, device=dev) for _ in range(4))
+    for to, x in zip((r, b, dS, dy), (last[0], last[1], last[5], last[6])):
+        to[-n:] = x
+    s, y, saved = decoder.add_norm_fwd(r, b, last[2], eps=1e-5)
+    grads = decoder.add_norm_bwd(dS, dy, r, b, last[2], saved, eps=1e-5)
+    ref, tol = norm_oracle(*last[:5], 1.0, 1e-5, *last[5:])
+    for name, x in (("stream", s), ("out", y), *zip(NORM_GRADS[:2], grads)):
+        close(x[-n:], ref[name], tol[name], name)
+        assert not x[:-n].any()
+    close(grads[2], ref["dweight"], tol["dweight"], "dweight")
 
 
 @gpu
