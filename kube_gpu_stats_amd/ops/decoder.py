@@ -230,7 +230,7 @@ def _split_qkv(qkv, heads: int):
 def attention_fwd(q, k, v, *, causal: bool = True, scale: float | None = None, lengths=None, stream=None):
     """``attention`` without autograd: (out, saved), saved for ``attention_bwd``: (lse, low), lse
     [B, H, S] float32 the base-2 logarithm of each row's sum (-inf behind a sequence's end),
-    low [B, S, H, D] uint8 what rounding took from out, in 254ths of its last place, plus 128."""
+    low [B, S, H, D] uint8 what rounding took from out, a signed number of 256ths of its last place."""
     return _attention_fwd(q, k, v, causal, scale, lengths, stream, True)
 
 

@@ -77,41 +77,47 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float f,
       *reinterpret_cast<x4*>(lds + Tl::at(lane & 31, t * 4 + g) + (lane >> 5) * 8) = v;
     }
   constexpr int kPer = 64 / (D / 8);  // rows a store
+  const i32x4 to = buffer(p, rows > 0 ? ((rows - 1) * stride + D) * 2 : 0);
 #pragma unroll
   for (int i = 0; i < 32 / kPer; ++i) {
     const int row = i * kPer + lane / (D / 8), chunk = lane % (D / 8);
     const i32x4 v = *reinterpret_cast<const i32x4*>(lds + Tl::at(row, chunk));
-    if (row < rows) *reinterpret_cast<i32x4*>(p + row * stride * 2 + chunk * 16) = v;
+    store16(v, to, static_cast<int>(row * stride * 2) + chunk * 16);
   }
 }
 
-// The power of two below x, times 2^-7 or 2^-10: x's last place in T.  Tiny x: 0.
-template <class T> __device__ __forceinline__ float last_place(float x) {
-  return __builtin_bit_cast(float, __builtin_bit_cast(int, x) & 0x7F800000) * (__is_same(T, bf16) ? 0x1p-7f : 0x1p-10f);
+// An accumulator's value x as the output keeps it, r rounded to T, and a byte: how many
+// 256ths of r's last place x is above r, rounded down.  As numbers of 32 bits they differ
+// by an integer of up to half a last place, 2^15 for bf16 and 2^12 for fp16; the upper
+// half is left out (a tie rounded down), and what fp16 rounds off below its normal range
+// is cut to that.  (In place of the difference times its exponent: forward of 4 x 2048, 32
+// heads, 164.6 us to 163.1 us, of which the bytes cost 11 us.)
+template <class T> constexpr int kLowShift = __is_same(T, bf16) ? 8 : 5;
+template <class T> __device__ __forceinline__ uint32_t low_of(float x) {  // in bits 8 to 15
+  const int d = __builtin_bit_cast(int, x) - __builtin_bit_cast(int, static_cast<float>(static_cast<T>(x)));
+  constexpr int most = 128 << kLowShift<T>;
+  return static_cast<uint32_t>(min(max(d, -most), most - 1)) << (8 - kLowShift<T>);
+}
+// x again, to half of a 256th
+template <class T> __device__ __forceinline__ float with_low(T r, int low) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(int, static_cast<float>(r)) + (low << kLowShift<T>) +
+                                       (1 << (kLowShift<T> - 1)));
 }
 
-// What the rounding of acc f took, beside store_rows: 128 + 254 (acc f - rounded) / last
-// place, a byte each, 1 to 255 because half a last place is the most.  Where last_place
-// is 0, and for fp16 below its normal range, the byte is anything: it counts for less
-// than the smallest normal number's last place.
+// What the rounding of acc f took, beside store_rows.
 template <class T, int D>
 __device__ __forceinline__ void store_low(const f32x16 (&acc)[D / 32], float f, char* lds, uint8_t* p, int64_t stride,
                                           int rows, int lane) {
   constexpr int kPer = 64 / (D / 16);
+  const i32x4 to = buffer(p, rows > 0 ? (rows - 1) * stride + D : 0);
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       uint32_t q[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = acc[t][g * 4 + j] * f, r = static_cast<float>(static_cast<T>(x));
-        // 1 / last place, by its exponent; 2^23 + 2^22 puts the rounded sum in the low bits
-        const float k = __builtin_bit_cast(
-            float, ((254 + (__is_same(T, bf16) ? 7 : 10)) << 23) - (__builtin_bit_cast(int, r) & 0x7F800000));
-        q[j] = __builtin_bit_cast(uint32_t, fmaf((x - r) * 254.f, k, 12582912.f + 128.f));
-      }
-      const uint32_t lo = __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0400), hi = __builtin_amdgcn_perm(q[3], q[2], 0x0C0C0400);
+      for (int j = 0; j < 4; ++j) q[j] = low_of<T>(acc[t][g * 4 + j] * f);
+      const uint32_t lo = __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0501), hi = __builtin_amdgcn_perm(q[3], q[2], 0x0C0C0501);
       const int row = lane & 31, e = t * 32 + g * 8 + (lane >> 5) * 4;
       *reinterpret_cast<uint32_t*>(lds + row * D + ((((e >> 4) ^ (row >> 1)) & (D / 16 - 1)) << 4) + (e & 15)) = lo | (hi << 16);
     }
@@ -119,7 +125,7 @@ __device__ __forceinline__ void store_low(const f32x16 (&acc)[D / 32], float f, 
   for (int i = 0; i < 32 / kPer; ++i) {
     const int row = i * kPer + lane / (D / 16), chunk = lane % (D / 16);
     const i32x4 v = *reinterpret_cast<const i32x4*>(lds + row * D + (((chunk ^ (row >> 1)) & (D / 16 - 1)) << 4));
-    if (row < rows) *reinterpret_cast<i32x4*>(p + row * stride + chunk * 16) = v;
+    store16(v, to, static_cast<int>(row * stride) + chunk * 16);
   }
 }
 
@@ -305,9 +311,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
           u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc(dl), r * a.H * D + kk * 16 + (lane >> 5) * 8, 0, 0));
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = static_cast<float>(o[j]);
-        const float rest = static_cast<float>((low[j >> 2] >> (8 * (j & 3))) & 0xFF) - 128.f;
-        delta = fmaf(static_cast<float>(g[kk][j]), fmaf(rest, last_place<T>(x) * (1.f / 254.f), x), delta);
+        const int rest = static_cast<int8_t>(low[j >> 2] >> (8 * (j & 3)));
+        delta = fmaf(static_cast<float>(g[kk][j]), with_low<T>(o[j], rest), delta);
       }
     }
     delta += other_half(delta);
@@ -387,6 +392,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+      if (t && s0 + 32 >= last) break;  // no row sees the second half (16 x 500: 59 us to 58.3 us)
       f32x16 s, dp;
       scores(t, s, dp);
       const bool edge = s0 + t * 32 + 32 > open;

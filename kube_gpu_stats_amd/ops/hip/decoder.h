@@ -9,7 +9,7 @@ extern "C" {
 // Tensors [B, S, heads, D]; strides in elements of (B, S, heads), D contiguous; pointers
 // 16-byte aligned, strides multiples of 8.  lse: float [B, H, S],
 // delta: float [B, H, ceil(S / 32), 2, 32] (workspace).  low: [B, S, H, D], what rounding
-// took from out, in 254ths of its last place, plus 128.  The forward pass writes lse and low if they
+// took from out, a signed byte of 256ths of its last place.  The forward pass writes lse and low if they
 // are not null.
 struct KgsAttention {
   const void *q, *k, *v;

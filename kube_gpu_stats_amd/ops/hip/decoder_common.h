@@ -94,6 +94,13 @@ template <class V> __device__ __forceinline__ V load16(i32x4 d, int voff) {
   return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(rsrc(d), voff, 0, 0));
 }
 
+// 16 bytes a lane; past the descriptor's end nothing.  (A test of the row instead keeps the
+// compiler from reading several rows out of LDS before the first is stored.)
+__device__ __forceinline__ void store16(i32x4 v, i32x4 d, int voff) {
+  using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rsrc(d), voff, 0, 0);
+}
+
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)p));
 }
