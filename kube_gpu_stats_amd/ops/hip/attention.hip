@@ -34,10 +34,8 @@ namespace {
 // or five steps under way instead of two was within 10 % either way (for forward and dq
 // best on few key heads, worse on many or short rows; for dk and dv always worse).
 constexpr int NW = 4, kThreads = NW * kWave, kRows = NW * 32;
-constexpr int NS = 2;       // slots of LDS: one step in work, one under way
 constexpr int kStep = 64;   // keys a step of forward and dq
 constexpr int kQStep = 32;  // rows a step of dk, dv
-constexpr int kAhead = 1;   // fragments of k read ahead of the products, forward
 
 // Matrix products and LDS reads stay on their side of this; arithmetic may cross.  The
 // compiler would place each read right before its product, with a wait between them.
@@ -146,7 +144,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
   using E = El<T>;
   using Tl = Tile<D>;
   constexpr int kTile = kStep * Tl::kRow;
-  __shared__ __attribute__((aligned(1024))) char smem[NS * 2 * kTile];
+  __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * kTile];  // a step in work, one under way
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.S + kRows - 1) / kRows;
   int bh, rank;
@@ -168,8 +166,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
   const int last = CAUSAL ? min(qw + 32, n) : n;            // keys that any row of the wave sees
   const int steps = q0 < n ? (end + kStep - 1) / kStep : 0;
 
-  // Steps NS - 1 ahead of the one in work are under way.  Past the last key the
-  // descriptors are empty: the copies count, so the wait is the same everywhere.
+  // The step after the one in work is under way.  Past the last key the descriptors are
+  // empty: the copies leave zeros.
   using Cp = typename Tl::template Copy<kStep, NW>;
   Cp ck, cv;
   ck.init(wave, lane, a.k_st[1] * 2);
@@ -189,34 +187,30 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
   const float c = a.scale * kLog2e;
   if (steps > 0) fetch(0);
   loads_done();
-  if (steps > 0)
-#pragma unroll
-    for (int j = 1; j < NS - 1; ++j) fetch(j);
   int slot = 0;
   for (int j = 0; j < steps; ++j) {
-    copies_left<(NS - 2) * 2 * Cp::kN>();
+    copies_done();
     barrier();  // step j has landed for every wave, and nobody reads the slot before it any more
-    fetch(slot == 0 ? NS - 1 : slot - 1);
+    fetch(slot ^ 1);
     const int s0 = j * kStep;
     const char* kt = smem + slot * 2 * kTile;
     const char* vt = kt + kTile;
-    slot = slot == NS - 1 ? 0 : slot + 1;
+    slot ^= 1;
     if (s0 >= last) continue;
     f32x16 s[2] = {};
     {
-      typename E::x8 f[kAhead + 1][2];
+      typename E::x8 f[2][2];  // read one step ahead of the products
       auto read = [&](int kk) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) f[kk % (kAhead + 1)][t] = Tl::template rows<T>(kt, t * 32, kk, lane);
+        for (int t = 0; t < 2; ++t) f[kk & 1][t] = Tl::template rows<T>(kt, t * 32, kk, lane);
       };
-#pragma unroll
-      for (int kk = 0; kk < kAhead; ++kk) read(kk);
+      read(0);
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        if (kk + kAhead < D / 16) read(kk + kAhead);
+        if (kk + 1 < D / 16) read(kk + 1);
         in_order();
 #pragma unroll
-        for (int t = 0; t < 2; ++t) s[t] = E::mfma(f[kk % (kAhead + 1)][t], q[kk], s[t]);
+        for (int t = 0; t < 2; ++t) s[t] = E::mfma(f[kk & 1][t], q[kk], s[t]);
         in_order();
       }
     }
@@ -283,7 +277,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   using E = El<T>;
   using Tl = Tile<D>;
   constexpr int kTile = kStep * Tl::kRow;
-  __shared__ __attribute__((aligned(1024))) char smem[NS * 2 * kTile];
+  __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * kTile];  // a step in work, one under way
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.S + kRows - 1) / kRows;
   int bh, rank;
@@ -325,8 +319,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   const int last = CAUSAL ? min(qw + 32, n) : n;
   const int steps = q0 < n ? (end + kStep - 1) / kStep : 0;
 
-  // Steps NS - 1 ahead of the one in work are under way.  Past the last key the
-  // descriptors are empty: the copies count, so the wait is the same everywhere.
+  // The step after the one in work is under way.  Past the last key the descriptors are
+  // empty: the copies leave zeros.
   using Cp = typename Tl::template Copy<kStep, NW>;
   Cp ck, cv;
   ck.init(wave, lane, a.k_st[1] * 2);
@@ -345,18 +339,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   const float c = a.scale * kLog2e;
   if (steps > 0) fetch(0);
   loads_done();
-  if (steps > 0)
-#pragma unroll
-    for (int j = 1; j < NS - 1; ++j) fetch(j);
   int slot = 0;
   for (int j = 0; j < steps; ++j) {
-    copies_left<(NS - 2) * 2 * Cp::kN>();
+    copies_done();
     barrier();
-    fetch(slot == 0 ? NS - 1 : slot - 1);
+    fetch(slot ^ 1);
     const int s0 = j * kStep;
     const char* kt = smem + slot * 2 * kTile;
     const char* vt = kt + kTile;
-    slot = slot == NS - 1 ? 0 : slot + 1;
+    slot ^= 1;
     if (s0 >= last) continue;
     // s and do.v of 32 keys
     const auto scores = [&](int t, f32x16& s, f32x16& dp) {
@@ -440,8 +431,9 @@ template <class T, int D, bool CAUSAL>
 __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention a) {
   using E = El<T>;
   using Tl = Tile<D>;
+  // a step: q, do, and lse and delta of its rows
   constexpr int kQ = kQStep, kTile = kQ * Tl::kRow, kV = kRows * Tl::kRow, kStage = 2 * kTile + 256;
-  __shared__ __attribute__((aligned(1024))) char smem[kV + NS * kStage];
+  __shared__ __attribute__((aligned(1024))) char smem[kV + 2 * kStage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles = (a.S + kRows - 1) / kRows;
   int bh, rank;
@@ -505,20 +497,16 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
   const float c = a.scale * kLog2e;
   if (lo < hi) fetch(0);
   loads_done();
-  if (lo < hi)
-#pragma unroll
-    for (int j = 1; j < NS - 1; ++j) fetch(j);
   int slot = 0, ss = hi > lo ? lo % each : 0;
   for (int i = lo; i < hi; ++i) {
-    if (wave == 0) copies_left<(NS - 2) * (2 * Cp::kN + 1)>();
-    else copies_left<(NS - 2) * 2 * Cp::kN>();
+    copies_done();
     barrier();
-    fetch(slot == 0 ? NS - 1 : slot - 1);
+    fetch(slot ^ 1);
     const int s0 = (first + ss) * kQ;
     const char* qt = smem + kV + slot * kStage;
     const char* gt = qt + kTile;
     const float* lse = reinterpret_cast<const float*>(gt + kTile);
-    slot = slot == NS - 1 ? 0 : slot + 1;
+    slot ^= 1;
     if (++ss == each) ss = 0;
     if (CAUSAL && s0 + kQ <= kw) continue;  // no row of the step sees the wave's keys
     f32x16 s = {}, dp = {};

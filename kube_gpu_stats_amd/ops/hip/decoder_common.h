@@ -123,9 +123,8 @@ __device__ __forceinline__ void copy4(i32x4 d, int voff, uint32_t lds) {
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(d)
                : "memory", "m0");
 }
-// Waits until at most N of the wave's copies are under way.
-template <int N> __device__ __forceinline__ void copies_left() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void copies_done() { copies_left<0>(); }
+// Waits until none of the wave's copies is under way.
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 // The same wait in a form the compiler knows: what it loaded before is there, and it puts
 // no wait of its own for that into the loop that follows.
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0F70); }
