@@ -461,7 +461,8 @@ def _lines(t):
 
 
 def _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps, back=None):
-    """(rows, width, type) of a call's tensors; ``back``: (dstream, dout, saved)."""
+    """(rows, width, type, scale) of a call's tensors; ``back``: (dstream, dout, saved).  The scale is
+    rounded to the kernels' 32 bits here: whether it is 1 is asked on both sides."""
     if residual.dim() < 1:
         raise ValueError("residual must be [..., width], not a single value")
     shape, dtype, index = residual.shape, residual.dtype, residual.get_device()
@@ -492,7 +493,7 @@ def _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps, ba
                 _same(residual, "residual", **{name: t})
         _kept(back[2], "saved", torch.float32, (2, T), index, "add_norm_fwd")
     _on_gpu(residual, "residual")
-    return T, C, code
+    return T, C, code, ctypes.c_float(scale).value
 
 
 def add_norm(residual, branch, weight, *, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-6):
@@ -518,7 +519,7 @@ def add_norm_fwd(residual, branch, weight, *, post_weight=None, gate=None, scale
 
 
 def _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, keep):
-    T, C, code = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps)
+    T, C, code, scale = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps)
     if not _here(residual, stream):
         return _there(residual, stream,
                       lambda: _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, keep),
@@ -557,7 +558,7 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
     dresidual, the same tensor; gradients of absent weights are None."""
     if dstream is None and dout is None:
         raise ValueError("one of dstream and dout must be given")
-    T, C, code = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps, (dstream, dout, saved))
+    T, C, code, scale = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps, (dstream, dout, saved))
     if not _here(residual, stream):
         return _there(residual, stream,
                       lambda: add_norm_bwd(dstream, dout, residual, branch, weight, saved, post_weight=post_weight,
