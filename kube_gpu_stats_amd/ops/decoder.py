@@ -57,7 +57,7 @@ def lib() -> ctypes.CDLL:
 # The C structures of ops/hip/decoder.h, field by field.
 _ATTENTION = struct.Struct("@13P24q8if")
 _SWIGLU = struct.Struct("@9P3q4i3i3i")
-_ADD_NORM = struct.Struct("@16P5q4i2f")
+_ADD_NORM = struct.Struct("@16P5q4iP2f")
 
 
 def _call(entry: str, args: bytes, index: int) -> None:
@@ -514,24 +514,57 @@ def add_norm(residual, branch, weight, *, post_weight=None, gate=None, scale: fl
 
 def add_norm_fwd(residual, branch, weight, *, post_weight=None, gate=None, scale: float = 1.0, eps: float = 1e-6,
                  stream=None):
-    """``add_norm`` without autograd: (stream, out, saved), saved for ``add_norm_bwd``."""
-    return _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, True)
+    """``add_norm`` without autograd: (stream, out, saved), saved for ``add_norm_bwd``: [2, rows]
+    float32, the factors of the two norms, in the stream's memory and with it 8 more bits of
+    each of a 16-bit stream's elements."""
+    return _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, True, True)
 
 
-def _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, keep):
+def _norm_room(T: int, C: int, size: int) -> tuple[int, int, int]:
+    """Where saved and the low bytes begin behind a stream of T x C elements of ``size`` bytes, and the end."""
+    saved = -(-T * C * size // 16) * 16
+    low = saved + 8 * T
+    return saved, low, low + (T * C if size == 2 else 0)
+
+
+def _from_stream(x, saved, T: int, C: int) -> bool:
+    """Whether ``x`` is the stream in whose memory ``saved`` is."""
+    store = saved.untyped_storage()
+    base = store.data_ptr()
+    if x.untyped_storage().data_ptr() != base:
+        return False
+    at, _, end = _norm_room(T, C, x.element_size())
+    if store.nbytes() != end or saved.data_ptr() != base + at:
+        return False  # a program's own memory, in which it keeps both
+    if x.data_ptr() != base or not x.is_contiguous():
+        raise ValueError("the stream must come as add_norm_fwd returned it, its rows in their order")
+    return True
+
+
+def _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, keep, together=False):
     T, C, code, scale = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps)
     if not _here(residual, stream):
         return _there(residual, stream,
-                      lambda: _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, keep),
+                      lambda: _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, None, keep, together),
                       branch, weight, post_weight, gate)
-    s, out = residual.new_empty(residual.shape), residual.new_empty(residual.shape)
-    saved = torch.empty(2, T, dtype=torch.float32, device=residual.device) if keep else None
+    out, low = residual.new_empty(residual.shape), 0
+    if together and T:
+        # (set_: tensors of one memory, not views of one another, whose versions autograd would count together)
+        at, low, end = _norm_room(T, C, residual.element_size())
+        room = torch.empty(end, dtype=torch.uint8, device=residual.device)
+        store = room.untyped_storage()
+        s = residual.new_empty(0).set_(store, 0, residual.shape)
+        saved = torch.empty(0, dtype=torch.float32, device=residual.device).set_(store, at // 4, (2, T))
+        low = room.data_ptr() + low if low < end else 0
+    else:
+        s = residual.new_empty(residual.shape)
+        saved = torch.empty(2, T, dtype=torch.float32, device=residual.device) if keep else None
     if T:
         (r, r_ld), (b, b_ld) = _lines(residual), _lines(branch)
         w, pw, g = _vector(weight), _vector(post_weight), _vector(gate)
         _call("kgs_add_norm_fwd",
               _ADD_NORM.pack(r.data_ptr(), b.data_ptr(), w.data_ptr(), _ptr(pw), _ptr(g), s.data_ptr(), out.data_ptr(),
-                             _ptr(saved), 0, 0, 0, 0, 0, 0, 0, 0, r_ld, b_ld, C, 0, 0, T, C, code, 0, scale, eps),
+                             _ptr(saved), 0, 0, 0, 0, 0, 0, 0, 0, r_ld, b_ld, C, 0, 0, T, C, code, 0, low, scale, eps),
               r.get_device())
     return s, out, saved
 
@@ -554,8 +587,14 @@ def _norm_parts(T: int, C: int) -> int:
 def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=None, gate=None, scale: float = 1.0,
                  eps: float = 1e-6, stream=None):
     """(dresidual, dbranch, dweight, dpost_weight, dgate) of ``add_norm`` from the gradients of
-    its two results (either may be None: zero), its arguments, and ``saved`` of ``add_norm_fwd``.  Without post_weight, gate and scale dbranch is
-    dresidual, the same tensor; gradients of absent weights are None."""
+    its two results (either may be None: zero), its arguments, and ``saved`` of ``add_norm_fwd``.
+
+    In the residual's place the stream that ``add_norm_fwd`` returned with ``saved`` does as
+    well: then the residual need not be kept, and without post_weight, gate and scale the
+    branch is not read either.  It has to be that tensor, or one of its memory and order
+    (``saved`` lies in the same memory, by which it is known); a copy of it is taken for a
+    residual.  Without post_weight, gate and scale dbranch is dresidual, the same tensor;
+    gradients of absent weights are None."""
     if dstream is None and dout is None:
         raise ValueError("one of dstream and dout must be given")
     T, C, code, scale = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps, (dstream, dout, saved))
@@ -569,16 +608,20 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
     new = weight.new_empty if T else weight.new_zeros
     dw, dpw, dg = new((C,)), new((C,)) if post_weight is not None else None, new((C,)) if gate is not None else None
     if T:
-        (r, r_ld), (b, b_ld) = _lines(residual), _lines(branch)
+        (r, r_ld), (b, b_ld), s, s_ld, low = _lines(residual), _lines(branch), None, 0, 0
+        if _from_stream(residual, saved, T, C):
+            s, s_ld, r = residual, C, None
+            low = s.data_ptr() + _norm_room(T, C, s.element_size())[1] if code < 2 else 0
         ds, ds_ld = _lines(dstream) if dstream is not None else (None, 0)
         dy, dy_ld = _lines(dout) if dout is not None else (None, 0)
         w, pw, g = _vector(weight), _vector(post_weight), _vector(gate)
         parts = _norm_parts(T, C)
-        work = torch.empty(parts * 2 * C, dtype=torch.float32, device=r.device)
+        work = torch.empty(parts * 2 * C, dtype=torch.float32, device=residual.device)
         _call("kgs_add_norm_bwd",
-              _ADD_NORM.pack(r.data_ptr(), b.data_ptr(), w.data_ptr(), _ptr(pw), _ptr(g), 0, 0, saved.data_ptr(),
+              _ADD_NORM.pack(_ptr(r), b.data_ptr(), w.data_ptr(), _ptr(pw), _ptr(g), _ptr(s), 0, saved.data_ptr(),
                              _ptr(ds), _ptr(dy), dr.data_ptr(), db.data_ptr(), dw.data_ptr(), _ptr(dpw), _ptr(dg),
-                             work.data_ptr(), r_ld, b_ld, 0, ds_ld, dy_ld, T, C, code, parts, scale, eps), r.get_device())
+                             work.data_ptr(), r_ld, b_ld, s_ld, ds_ld, dy_ld, T, C, code, parts, low, scale, eps),
+              residual.get_device())
     return dr, db, dw, dpw, dg
 
 

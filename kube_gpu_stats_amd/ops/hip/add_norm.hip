@@ -15,9 +15,9 @@
 // second kernel in a fixed order (no atomics, so equal calls give equal bits).
 //
 // Everything is computed in 32 bits and rounded once, as an output.  Both passes use the
-// unrounded stream: the backward adds it up again from residual and branch.  (The stored
-// one would save it a read where there are no post_weight, gate and scale, but add half
-// as much error again to dweight.)
+// unrounded stream.  The backward adds it up again from residual and branch, or reads the
+// stream that the forward wrote with 8 more bits of each element beside it.  (The 16-bit
+// stream alone would add half as much error again to dweight.)
 #include "decoder.h"
 #include "decoder_common.h"
 
@@ -90,6 +90,23 @@ template <bool WAVES> __device__ __forceinline__ float row_sum(float x, int lane
     for (unsigned i = 0; i < blockDim.x / 64; ++i) x += s[i];
   }
   return x;
+}
+
+// What rounding took from 8 elements of a 16-bit stream, a byte each.  With no byte below
+// it an infinity is read back as a NaN: so is an element that rounding made infinite, whose
+// difference would make it a finite one.
+template <class T> __device__ __forceinline__ void store_low(const float (&x)[kV], uint8_t* p, int left) {
+  Loose<uint8_t> r;
+#pragma unroll
+  for (int i = 0; i < kV; ++i)
+    r.v[i] = __builtin_isinf(static_cast<float>(static_cast<T>(x[i]))) ? 0 : static_cast<uint8_t>(low_of<T>(x[i]) >> 8);
+  if (left >= kV) {
+    *reinterpret_cast<Loose<uint8_t>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kV; ++i)
+      if (i < left) p[i] = r.v[i];
+  }
 }
 
 __host__ __device__ __forceinline__ int lanes_of_row(int width) {
@@ -185,7 +202,12 @@ __global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_fwd_kernel(KgsAdd
         else s[i][j] += b[i][j];
         sq = fmaf(s[i][j], part(i, j, s[i][j]), sq);
       }
-      if (skip[i] < kV) store(s[i], place<T>(a.stream, row * a.stream_ld, column[i]), size);
+      if (skip[i] < kV) {
+        store(s[i], place<T>(a.stream, row * a.stream_ld, column[i]), size);
+        if constexpr (sizeof(T) == 2) {
+          if (a.low) store_low<T>(s[i], a.low + static_cast<int64_t>(row) * C + column[i] / sizeof(T), size);
+        }
+      }
     }
     const float rs = 1.f / sqrtf(row_sum<WAVES>(sq, at.lanes, slots, turn) / C + a.eps);
 #pragma unroll
@@ -216,8 +238,11 @@ template <class T> __device__ __forceinline__ void finish(const KgsAddNorm& a, i
 
 // The next row's loads are under way while this one is reduced; with one chunk a thread
 // that fits the registers of 16 waves a CU.  Two chunks (rows over 8192 wide) do without,
-// and read the weights again for every row.
-template <class T, bool WAVES, int NV, bool FULL, Fit FIT, int THREADS>
+// and read the weights again for every row.  STORED: from the stream and its low bytes, one
+// byte an element less to read than residual and branch, with FULL one more (8192 x 4096:
+// 57 us, 63 us from the residual; 16384 x 8192 with all weights 310 us, 288 us; the forward,
+// which writes them, 7 and 24 us more).
+template <class T, bool WAVES, int NV, bool FULL, bool STORED, Fit FIT, int THREADS>
 __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
   __shared__ float slots[2 * 16];
   __shared__ float sums[WAVES ? (FULL ? 2 : 1) * 4 * 512 : 1];
@@ -278,8 +303,10 @@ __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
     }
   };
   if (kAhead) weights();
+  constexpr bool kLow = STORED && sizeof(T) == 2;
   struct Row {
-    Loose<T> s[NV], dy[NV], ds[NV], b[NV];
+    Loose<T> s[NV], dy[NV], ds[NV], b[STORED && !FULL ? 1 : NV];  // s: the residual, or the stream
+    u32x2 low[kLow ? NV : 1];  // 8 bytes (as bytes they would take a register each)
     float rs, rb;
   } next;
   const auto fetch = [&](int row) {
@@ -287,8 +314,22 @@ __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
     next.rb = FULL ? a.rstd[a.rows + row] : 1.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      get_once(next.s[i], a.residual, row * a.residual_ld, column[i]);
-      get_once(next.b[i], a.branch, row * a.branch_ld, column[i]);
+      if constexpr (STORED) get_once(next.s[i], a.stream, row * a.stream_ld, column[i]);
+      else get_once(next.s[i], a.residual, row * a.residual_ld, column[i]);
+      if constexpr (kLow) {
+        const uint8_t* p = a.low + static_cast<int64_t>(row) * C + column[i] / sizeof(T);
+        if constexpr (FIT == kWhole) {
+          next.low[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+        } else if constexpr (FIT == kRagged) {
+          __builtin_memcpy(&next.low[i], p, kV);
+        } else {
+          next.low[i] = u32x2{0, 0};
+#pragma unroll
+          for (int j = 0; j < kV; ++j)
+            if (j < C) next.low[i][j >> 2] |= static_cast<uint32_t>(p[j]) << (8 * (j & 3));
+        }
+      }
+      if constexpr (FULL || !STORED) get_once(next.b[i], a.branch, row * a.branch_ld, column[i]);
       if (a.dout) get(next.dy[i], a.dout, row * a.dout_ld, column[i]);
       if (a.dstream) get(next.ds[i], a.dstream, row * a.dstream_ld, column[i]);
     }
@@ -315,13 +356,13 @@ __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
       for (int j = 0; j < kV; ++j) {
         const float g = static_cast<float>(next.dy[i].v[j]);
         ds[i][j] = static_cast<float>(next.ds[i].v[j]);
-        const float r = static_cast<float>(next.s[i].v[j]), x = static_cast<float>(next.b[i].v[j]);
-        if constexpr (FULL) {
-          b[i][j] = x * rb;
-          s[i][j] = fmaf(full[i][j], b[i][j], r) * rs;
-        } else {
-          s[i][j] = (r + x) * rs;
-        }
+        float r;
+        if constexpr (kLow) r = with_low<T>(next.s[i].v[j], static_cast<int8_t>(next.low[i][j >> 2] >> (8 * (j & 3))));
+        else r = static_cast<float>(next.s[i].v[j]);
+        if constexpr (FULL) b[i][j] = static_cast<float>(next.b[i].v[j]) * rb;
+        if constexpr (STORED) s[i][j] = r * rs;
+        else if constexpr (FULL) s[i][j] = fmaf(full[i][j], b[i][j], r) * rs;
+        else s[i][j] = (r + static_cast<float>(next.b[i].v[j])) * rs;
         dw[i][j] = fmaf(g, s[i][j], dw[i][j]);
         dy[i][j] = g * w[i][j];
         dot = fmaf(dy[i][j], part_of(i, j, s[i][j]), dot);
@@ -430,19 +471,23 @@ template <class T, bool WAVES, int NV> int forward(const KgsAddNorm& a, hipStrea
   return launched("add_norm forward");
 }
 
-template <class T, bool WAVES, int NV, int THREADS> int backward(const KgsAddNorm& a, hipStream_t s) {
+template <class T, bool WAVES, int NV, bool STORED, int THREADS> int backward_from(const KgsAddNorm& a, hipStream_t s) {
   int threads, rows;
   shape<WAVES, NV>(a, threads, rows);
   const auto go = [&](auto kernel) { kernel<<<a.parts, threads, 0, s>>>(a); };
   const bool full = is_full(a);
-  if (a.width % kV == 0) full ? go(add_norm_bwd_kernel<T, WAVES, NV, true, kWhole, THREADS>) : go(add_norm_bwd_kernel<T, WAVES, NV, false, kWhole, THREADS>);
-  else if (a.width > kV) full ? go(add_norm_bwd_kernel<T, WAVES, NV, true, kRagged, THREADS>) : go(add_norm_bwd_kernel<T, WAVES, NV, false, kRagged, THREADS>);
-  else if constexpr (WAVES) full ? go(add_norm_bwd_kernel<T, WAVES, NV, true, kTiny, THREADS>) : go(add_norm_bwd_kernel<T, WAVES, NV, false, kTiny, THREADS>);
+  if (a.width % kV == 0) full ? go(add_norm_bwd_kernel<T, WAVES, NV, true, STORED, kWhole, THREADS>) : go(add_norm_bwd_kernel<T, WAVES, NV, false, STORED, kWhole, THREADS>);
+  else if (a.width > kV) full ? go(add_norm_bwd_kernel<T, WAVES, NV, true, STORED, kRagged, THREADS>) : go(add_norm_bwd_kernel<T, WAVES, NV, false, STORED, kRagged, THREADS>);
+  else if constexpr (WAVES) full ? go(add_norm_bwd_kernel<T, WAVES, NV, true, STORED, kTiny, THREADS>) : go(add_norm_bwd_kernel<T, WAVES, NV, false, STORED, kTiny, THREADS>);
   if (launched("add_norm backward")) return -1;
   if (a.parts == 1) return 0;
   const bool second = a.dpost_weight || a.dgate;
   add_norm_join_kernel<T><<<dim3((a.width + 15) / 16, second ? 2 : 1), 1024, 0, s>>>(a);
   return launched("add_norm join");
+}
+
+template <class T, bool WAVES, int NV, int THREADS> int backward(const KgsAddNorm& a, hipStream_t s) {
+  return a.residual ? backward_from<T, WAVES, NV, false, THREADS>(a, s) : backward_from<T, WAVES, NV, true, THREADS>(a, s);
 }
 
 template <class T> int run(const KgsAddNorm& a, bool back, hipStream_t s) {
@@ -457,7 +502,8 @@ template <class T> int run(const KgsAddNorm& a, bool back, hipStream_t s) {
 
 int dispatch(const KgsAddNorm* a, bool back, void* stream) {
   const char* w = "add_norm";
-  if (!a || !a->residual || !a->branch || !a->weight) return fail(w, "a tensor is missing");
+  if (!a || !a->branch || !a->weight) return fail(w, "a tensor is missing");
+  if (!a->residual && (!back || !a->stream || (a->type != 2 && !a->low))) return fail(w, "a tensor is missing");
   if (!back && (!a->stream || !a->out)) return fail(w, "a tensor is missing");
   if (back && (!a->rstd || !a->dresidual || !a->dbranch || !a->dweight)) return fail(w, "a tensor is missing");
   if (back && ((a->post_weight && !a->dpost_weight) || (a->gate && !a->dgate))) return fail(w, "a tensor is missing");

@@ -43,6 +43,9 @@ struct KgsSwiglu {
 // the branch); dstream and dout may be null (zero).  post_weight and gate may be null.
 // partial: float [parts, 2, width], parts the workgroups of the backward.
 // dbranch may equal dresidual where they are the same.
+// The backward starts from residual and branch or, where residual is null, from the stream
+// (contiguous, as the forward wrote it) and low [rows, width]: what rounding took from the
+// stream of a 16-bit type, bytes as attention's.  The forward writes low if it is not null.
 struct KgsAddNorm {
   const void *residual, *branch, *weight, *post_weight, *gate;
   void *stream, *out;
@@ -52,6 +55,7 @@ struct KgsAddNorm {
   float* partial;
   int64_t residual_ld, branch_ld, stream_ld, dstream_ld, dout_ld;
   int32_t rows, width, type, parts;  // type: 0 bfloat16, 1 float16, 2 float32
+  uint8_t* low;
   float scale, eps;
 };
 

@@ -190,6 +190,24 @@ template <int W> struct Tile {
   };
 };
 
+// A 32-bit value x as a result keeps it, r rounded to T, and a byte: how many
+// 256ths of r's last place x is above r, rounded down.  As numbers of 32 bits they differ
+// by an integer of up to half a last place, 2^15 for bf16 and 2^12 for fp16; the upper
+// half is left out (a tie rounded down), and what fp16 rounds off below its normal range
+// is cut to that.  (In place of the difference times its exponent: attention forward of 4 x
+// 2048, 32 heads, 164.6 us to 163.1 us, of which the bytes cost 11 us.)
+template <class T> constexpr int kLowShift = __is_same(T, bf16) ? 8 : 5;
+template <class T> __device__ __forceinline__ uint32_t low_of(float x) {  // in bits 8 to 15
+  const int d = __builtin_bit_cast(int, x) - __builtin_bit_cast(int, static_cast<float>(static_cast<T>(x)));
+  constexpr int most = 128 << kLowShift<T>;
+  return static_cast<uint32_t>(min(max(d, -most), most - 1)) << (8 - kLowShift<T>);
+}
+// x again, to half of a 256th
+template <class T> __device__ __forceinline__ float with_low(T r, int low) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(int, static_cast<float>(r)) + (low << kLowShift<T>) +
+                                       (1 << (kLowShift<T> - 1)));
+}
+
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
 // Workgroup id -> work item so that neighbouring items run on one of the 8 XCDs (ids

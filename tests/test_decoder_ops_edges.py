@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from kube_gpu_stats_amd.ops import decoder
-from test_decoder_ops import BF16, F16, F32, NORM_GRADS, close, norm_check, norm_inputs, z
+from test_decoder_ops import BF16, F16, F32, NORM_GRADS, close, norm_check, norm_inputs, norm_oracle, z
 
 gpu = pytest.mark.gpu
 
@@ -61,3 +61,140 @@ def test_gradients_of_scales_next_to_one(dev, scale, t):
     r, b = a[0].clone().requires_grad_(), a[1].clone().requires_grad_()
     torch.autograd.backward(decoder.add_norm(r, b, a[2], scale=scale, eps=1e-5), [a[5], a[6]])
     assert torch.equal(r.grad, want[0]) and torch.equal(b.grad, want[1])
+
+
+# ------------------------------------------------- add_norm: a backward that starts from the stream
+
+def stream_tolerance(ref, tol, a, scale, eps):
+    """tol, and what the stream's own error adds to the gradients: half of a 256th of its last place, twice (cut
+    and middle), where 16 bits and 8 are kept; below fp16's normal range what 16 bits leave."""
+    r, b, w, pw, gate, dS, dy = (None if x is None else x.double() for x in a)
+    t, u, C = a[0].dtype, torch.finfo(a[0].dtype).eps / 2, a[0].shape[1]
+    if t == F32:
+        return tol  # the stream as it was computed
+    tol = dict(tol)
+    s = ref["stream"]
+    e_s = 2.0 ** -7 * u * s.abs() + (2.0 ** -25 if t == F16 else 0.0)
+    rs = (s.square().mean(1, keepdim=True) + eps).rsqrt()
+    sh, e_sh = s * rs, e_s * rs
+    d = w * dy
+    m = (d * sh).mean(1, keepdim=True)
+    e_ds = 1.02 * rs * (e_sh * m.abs() + sh.abs() * (d.abs() * e_sh).mean(1, keepdim=True))
+    tol["dresidual"] = tol["dresidual"] + e_ds
+    tol["dweight"] = tol["dweight"] + (dy.abs() * e_sh).sum(0)
+    rb = (b.square().mean(1, keepdim=True) + eps).rsqrt() if pw is not None else torch.ones_like(rs)
+    one = torch.ones(C, dtype=torch.float64, device=s.device)
+    p, g = one if pw is None else pw, one if gate is None else gate
+    e_x = abs(scale) * (p * g).abs() * e_ds
+    tol["dbranch"] = tol["dbranch"] + 1.02 * rb * e_x
+    if pw is not None:
+        tol["dbranch"] = tol["dbranch"] + 1.02 * rb * (b * rb).abs() * ((b * rb).abs() * e_x).mean(1, keepdim=True)
+        tol["dpost_weight"] = tol["dpost_weight"] + abs(scale) * ((b * rb * g).abs() * e_ds).sum(0)
+    if gate is not None:
+        tol["dgate"] = tol["dgate"] + abs(scale) * ((b * rb * p).abs() * e_ds).sum(0)
+    return tol
+
+
+def stream_check(a, scale=1.0, eps=1e-5):
+    r, b, w, pw, gate, dS, dy = a
+    kw = {"post_weight": pw, "gate": gate, "scale": scale, "eps": eps}
+    s, y, saved = decoder.add_norm_fwd(r, b, w, **kw)
+    grads = decoder.add_norm_bwd(dS, dy, s, b, w, saved, **kw)
+    flat = lambda x: None if x is None else x.reshape(-1, x.shape[-1])  # noqa: E731
+    f = [flat(x) if x is not None and x.dim() > 1 else x for x in a]
+    ref, tol = norm_oracle(*f[:5], scale, eps, *f[5:])
+    tol = stream_tolerance(ref, tol, f, scale, eps)
+    for n, got in (("stream", s), ("out", y), *zip(NORM_GRADS, grads)):
+        if n not in ref:
+            assert got is None
+            continue
+        close(got.reshape(ref[n].shape), ref[n], tol[n], n)
+    assert (grads[0] is grads[1]) == (pw is None and gate is None and scale == 1.0)
+    return kw, s, y, saved, grads
+
+
+@gpu
+@pytest.mark.parametrize("t", [BF16, F16, F32])
+@pytest.mark.parametrize("C", [1, 7, 8, 300, 512, 513, 2056, 8192, 8200, 12296, 16384])
+@pytest.mark.parametrize("post,gate,scale", [(False, False, 1.0), (True, True, 0.7), (False, False, -0.5), (False, True, 1.0)])
+def test_add_norm_gradients_from_the_stream(dev, C, t, post, gate, scale):
+    """The residual's place taken by the stream that the forward pass returned: the same gradients."""
+    for T in (1, 37):
+        stream_check(norm_inputs(T, C, t, dev, post, gate, seed=C + T), scale)
+
+
+@gpu
+@pytest.mark.parametrize("t,T,C", [(BF16, 3000, 2048), (F16, 2100, 72), (F32, 9000, 16), (BF16, 1501, 8193)])
+def test_add_norm_many_rows_from_the_stream(dev, t, T, C):
+    stream_check(norm_inputs(T, C, t, dev, True, True, seed=T), 0.3)
+    stream_check(norm_inputs(T, C, t, dev, False, False, seed=T))
+
+
+@gpu
+@pytest.mark.parametrize("t", [BF16, F32])
+def test_stream_and_residual_are_told_apart(dev, t):
+    """By their memory: views of the stream count, a program's own buffer with everything in it does not."""
+    a = norm_inputs(12, 200, t, dev, True, False, seed=5)
+    r, b, w, pw, _, dS, dy = a
+    kw, s, y, saved, want = stream_check(a, 0.5)
+    shaped = [x.view(3, 4, 200) for x in (dS, dy, s, b)]
+    for x, q in zip(decoder.add_norm_bwd(*shaped, w, saved, **kw), want):
+        assert x is q is None or torch.equal(x.reshape(q.shape), q)
+    with pytest.raises(ValueError):
+        decoder.add_norm_bwd(*(x.view(3, 4, 200).transpose(0, 1) for x in (dS, dy, s, b)), w, saved, **kw)
+    plain = decoder.add_norm_bwd(dS, dy, r, b, w, saved, **kw)
+    room = torch.zeros(1 << 16, dtype=torch.uint8, device=dev)
+    size = r.numel() * r.element_size()
+    r2 = room[:size].view(t).view(r.shape).copy_(r)
+    at = -(-size // 16) * 16
+    k2 = room[at:at + 96].view(F32).view(2, 12).copy_(saved)
+    for x, q in zip(decoder.add_norm_bwd(dS, dy, r2, b, w, k2, **kw), plain):
+        assert x is q is None or torch.equal(x, q)
+    # a stream changed in place does not count as a change of saved, nor a pass's results as views
+    v = saved._version
+    s.add_(1)
+    assert saved._version == v and s._base is None and saved._base is None
+
+
+@gpu
+def test_add_norm_pair_from_the_stream_captured(dev):
+    """In a graph, replayed with other inputs between eager calls; on another stream."""
+    a = norm_inputs(33, 520, BF16, dev, True, True, seed=1)
+
+    def step(r, b, w, pw, gate, dS, dy, **on):
+        kw = {"post_weight": pw, "gate": gate, "scale": 0.5}
+        s, y, saved = decoder.add_norm_fwd(r, b, w, **kw, **on)
+        return (s, y, *decoder.add_norm_bwd(dS, dy, s, b, w, saved, **kw, **on))
+
+    step(*a)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step(*a)
+    for seed in (2, 3, 4):
+        fresh = norm_inputs(33, 520, BF16, dev, True, True, seed=seed)
+        want = step(*fresh)
+        for x, q in zip(a, fresh):
+            x.copy_(q)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, q) for x, q in zip(got, want)), seed
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    other = step(*a, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, q) for x, q in zip(other, want))
+
+
+@gpu
+def test_a_stream_that_overflowed_stays_infinite(dev):
+    """fp16 rows whose sum leaves the type's range: the gradients of those rows are not finite, the others are right."""
+    a = norm_inputs(4, 64, F16, dev, False, False, seed=7)
+    r, b, w, _, _, dS, dy = a
+    want = norm_check(*a)[3]
+    r[2, 5] = b[2, 5] = 60000.0
+    s, y, saved = decoder.add_norm_fwd(r, b, w, eps=1e-5)
+    dr = decoder.add_norm_bwd(dS, dy, s, b, w, saved, eps=1e-5)[0]
+    assert math.isinf(s[2, 5]) and not torch.isfinite(dr[2]).all()
+    for i in (0, 1, 3):
+        assert (dr[i].double() - want[0][i].double()).abs().max() <= 2 * torch.finfo(F16).eps * want[0][i].abs().max()
