@@ -164,7 +164,7 @@ def _own_add_norm(s, c):
         stream, out = decoder.add_norm(s["residual"], s["branch"], s["weight"], **kw)
         return {"stream": stream, "out": out}
     stream, out, saved = decoder.add_norm_fwd(s["residual"], s["branch"], s["weight"], **kw)
-    grads = decoder.add_norm_bwd(s["dstream"], s["dout"], s["residual"], s["branch"], s["weight"], saved, **kw)
+    grads = decoder.add_norm_bwd(s["dstream"], s["dout"], stream, s["branch"], s["weight"], saved, **kw)
     return {"stream": stream, "out": out, "dresidual": grads[0], "dbranch": grads[1], "dweight": grads[2],
             "dpost_weight": grads[3], "dgate": grads[4]}
 
