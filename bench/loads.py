@@ -324,7 +324,8 @@ class TrainLoad(GpuLoad):
             def forward(self, t):
                 x = self.emb(t)
                 B, S, _ = x.shape
-                eps = torch.finfo(x.dtype).eps  # nn.RMSNorm's
+                # nn.RMSNorm's where it is given none: of the type it computes in, not of its input's
+                eps = torch.finfo(torch.float32).eps if self.norm.eps is None else self.norm.eps
                 y = self.blocks[0].n1(x)
                 after = [b.n1 for b in self.blocks[1:]] + [self.norm]
                 for b, norm in zip(self.blocks, after):

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from kube_gpu_stats_amd.ops import decoder
-from test_decoder_ops import BF16, F16, F32, NORM_GRADS, close, norm_check, norm_inputs, norm_oracle, z
+from test_decoder_ops import BF16, F16, F32, NORM_GRADS, close, half_step, norm_check, norm_inputs, norm_oracle, z
 
 gpu = pytest.mark.gpu
 
@@ -198,3 +198,55 @@ def test_a_stream_that_overflowed_stays_infinite(dev):
     assert math.isinf(s[2, 5]) and not torch.isfinite(dr[2]).all()
     for i in (0, 1, 3):
         assert (dr[i].double() - want[0][i].double()).abs().max() <= 2 * torch.finfo(F16).eps * want[0][i].abs().max()
+
+
+# ----------------------------------------------------------- the training step's two models are one
+
+def train_loads(device, *more):
+    import bench
+
+    loads = []
+    for ops in ("torch", "hip"):
+        a = bench.parse_args(["--load", "train", "--train-ops", ops, "--train-dim", "256", "--train-layers", "2",
+                              "--train-batch", "2", "--train-seq", "96", "--train-vocab", "512", *more])
+        loads.append(bench.TrainLoad(a, device, None))
+    for ld in loads:  # small activations, at which the norms' eps counts
+        with torch.no_grad():
+            ld.model.emb.weight.mul_(0.01)
+    return loads
+
+
+def same_gradients(loads):
+    grads = []
+    for ld in loads:
+        logits = ld.model(ld.tok[:, :-1])
+        ld.F.cross_entropy(logits.float().view(-1, ld.vocab), ld.tok[:, 1:].reshape(-1)).backward()
+        grads.append({n: p.grad.double() for n, p in ld.model.named_parameters()})
+    # as many roundings, and as large ones, as in test_decoder_ops.py's test of the same models
+    for n, g in grads[0].items():
+        assert (grads[1][n] - g).norm() <= 2 * math.sqrt(30) * half_step(BF16) * g.norm(), n
+
+
+def test_train_models_agree_on_small_activations(monkeypatch):
+    """With the operators in torch's own words, on the CPU: what the two models pass to them is the same."""
+    import torch.nn.functional as TF
+
+    def attention_qkv(qkv, heads):
+        q, k, v = (x.transpose(1, 2) for x in qkv.split(heads, dim=2))
+        return TF.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2)
+
+    def add_norm(r, b, w, *, eps):
+        return r + b, TF.rms_norm(r + b, w.shape, w, eps)
+
+    def swiglu(x, w):
+        g, u = TF.linear(x, w).chunk(2, -1)
+        return TF.silu(g) * u
+
+    for f in (attention_qkv, add_norm, swiglu):
+        monkeypatch.setattr(decoder, f.__name__, f)
+    same_gradients(train_loads(-1))
+
+
+@gpu
+def test_train_models_agree_on_small_activations_on_gpu(dev):
+    same_gradients(train_loads(0))
