@@ -295,9 +295,11 @@ def _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, stream,
     if into is None:
         into = q.new_empty((B, S, H, D)), q.new_empty((B, S, Hk, D)), q.new_empty((B, S, Hk, D))
     splits = _dkv_splits(B, S, H, Hk, bool(causal), D, lengths is not None)
-    # delta, then the parts of a split walk
+    # delta, for float16 the norms of v's and dout's rows, then the parts of a split walk
     parts = splits * 2 * B * S * Hk * D if splits > 1 else 0
     rows = B * H * -(-S // 32) * 64
+    if code == 1:
+        rows += -(-(B * Hk * -(-S // 128) + B * H * -(-S // 32)) // 4) * 4
     if B and S:
         work = torch.empty(rows + parts, dtype=torch.float32, device=q.device)
         at = work.data_ptr()

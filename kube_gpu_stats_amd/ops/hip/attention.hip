@@ -121,6 +121,70 @@ template <class T> __device__ __forceinline__ typename El<T>::x8 operand(const f
 // The row index that register r of a 32x32 accumulator holds in this lane.
 __device__ __forceinline__ int acc_row(int r, int lane) { return (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3); }
 
+// fp16 has the precision for ds, not the range: ds is a probability, one of thousands, times
+// products of do, which may be as small as a mean over tokens makes them.  So it is rounded
+// times a power of two, which is taken out of the sum at the end; nothing is rounded but ds
+// itself.  The power comes from a bound that holds without a look at the products: out is a
+// mean of v's rows, so |do_i.v_j - do_i.out_i| <= 2 |do_i| max |v_j|.  dq takes it of each
+// row, dk and dv of all rows of the key head.  The norms of v's rows are a launch of their
+// own; those of do come with dq.  bf16 has the range and takes none of this.  (Backward of
+// 4 x 2048, 32 heads: 571 us, 543 us without; 8 x 1536, 12 heads of 64: 252 us, 238 us; with
+// the largest of the products themselves, looked for at every step, 615 us and 297 us.)
+template <class T> constexpr bool kRanged = __is_same(T, f16);
+constexpr float kNorm = 0x1p20f;  // over any norm of finite fp16; of others nothing is asked
+// The largest norms: of v's rows [B, Hk, tiles], of do's by 32 rows [B, H, groups].
+__device__ __forceinline__ float* v_norms(const KgsAttention& a) {
+  return a.delta + static_cast<int64_t>(a.B) * a.H * ((a.S + 31) / 32) * 64;
+}
+__device__ __forceinline__ float* do_norms(const KgsAttention& a) {
+  return v_norms(a) + static_cast<int64_t>(a.B) * a.Hk * ((a.S + kRows - 1) / kRows);
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) x = fmaxf(x, __shfl_xor(x, m, 64));
+  return x;
+}
+// The largest of n floats, in every lane.
+__device__ __forceinline__ float largest(const float* p, int64_t n, int lane) {
+  float x = 0.f;
+  for (int64_t i = lane; i < n; i += 64) x = fmaxf(x, p[i]);
+  return wave_max(x);
+}
+// The power of two that brings the bound to between 2^14 and 2^15 (1 % for rounding).
+__device__ __forceinline__ float power(float norm_do, float norm_v) {
+  return ldexpf(1.f, 15 - __builtin_amdgcn_frexp_expf(2.02f * norm_do * norm_v));
+}
+
+// Of 128 rows of v the largest norm.
+template <class T, int D> __global__ __launch_bounds__(kThreads) void attention_norms_kernel(KgsAttention a) {
+  constexpr int kLanes = D / 8, kAtOnce = kThreads / kLanes;
+  __shared__ float most[NW];
+  const int tiles = (a.S + kRows - 1) / kRows, tile = blockIdx.x % tiles, bh = blockIdx.x / tiles;
+  const int hk = bh % a.Hk, b = bh / a.Hk, n = length_of(a, b), lane = threadIdx.x & 63;
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < kRows / kAtOnce; ++i) {
+    const int row = tile * kRows + i * kAtOnce + threadIdx.x / kLanes;
+    float sq = 0.f;
+    if (row < n) {
+      const typename El<T>::x8 x = *reinterpret_cast<const typename El<T>::x8*>(
+          at<T>(a.v, a.v_st, b, row, hk) + threadIdx.x % kLanes * 16);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sq = fmaf(static_cast<float>(x[j]), static_cast<float>(x[j]), sq);
+    }
+#pragma unroll
+    for (int s = 1; s < kLanes; s <<= 1) sq += __shfl_xor(sq, s, 64);
+    m = fmaxf(m, sq);
+  }
+  m = wave_max(m);
+  if (lane == 0) most[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < NW; ++i) m = fmaxf(m, most[i]);
+    v_norms(a)[blockIdx.x] = fminf(sqrtf(m), kNorm);
+  }
+}
+
 template <class T, int D, bool CAUSAL>
 __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention a) {
   using E = El<T>;
@@ -270,7 +334,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   const int q0 = tile * kRows, qw = q0 + wave * 32, row = qw + (lane & 31);
 
   typename E::x8 q[D / 16], g[D / 16];
-  float delta = 0.f;
+  float delta = 0.f, norm = 0.f;
   {
     const i32x4 dq = buffer(at<T>(a.q, a.q_st, b, qw, h), span<T, D>(n, qw, a.q_st[1]));
     const i32x4 dg = buffer(at<T>(a.dout, a.g_st, b, qw, h), span<T, D>(n, qw, a.g_st[1]));
@@ -289,9 +353,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
       for (int j = 0; j < 8; ++j) {
         const int rest = static_cast<int8_t>(low[j >> 2] >> (8 * (j & 3)));
         delta = fmaf(static_cast<float>(g[kk][j]), with_low<T>(o[j], rest), delta);
+        if constexpr (kRanged<T>) norm = fmaf(static_cast<float>(g[kk][j]), static_cast<float>(g[kk][j]), norm);
       }
     }
     delta += other_half(delta);
+    norm += other_half(norm);
   }
   const float lse = row < n ? a.lse[(static_cast<int64_t>(b) * a.H + h) * a.S + row] : 0.f;
 
@@ -320,6 +386,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   f32x16 acc[D / 32] = {};
   const float c = a.scale * kLog2e;
   if (steps > 0) fetch(0);
+  float f = 1.f;
+  const int groups = (a.S + 31) / 32, group = qw / 32;
+  if constexpr (kRanged<T>) {
+    norm = fminf(sqrtf(norm), kNorm);
+    f = power(norm, largest(v_norms(a) + (static_cast<int64_t>(b) * a.Hk + hk) * tiles, tiles, lane));
+    const float most = wave_max(norm);
+    if (lane == 0 && group < groups) do_norms(a)[(static_cast<int64_t>(b) * a.H + h) * groups + group] = most;
+  }
   loads_done();
   int slot = 0;
   for (int j = 0; j < steps; ++j) {
@@ -369,11 +443,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
       f32x16 s, dp;
       scores(t, s, dp);
       const bool edge = s0 + t * 32 + 32 > open;
+      const float d = delta * f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
-        float ds = p * (dp[r] - delta);
-        s[r] = ds;
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse));
+        s[r] = p * (kRanged<T> ? fmaf(dp[r], f, -d) : dp[r] - delta);
       }
       if (edge) {
 #pragma unroll
@@ -393,10 +467,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   barrier();
   // For dk, dv: the 32 rows' lse, then their delta, side by side.  Rows past the end get
   // zeros: with zeros for q and do they are p = 1 times zero there.
-  const int groups = (a.S + 31) / 32, group = qw / 32;
   if (group < groups)
     a.delta[(static_cast<int64_t>(b * a.H + h) * groups + group) * 64 + lane] =
         row >= n ? 0.f : lane < 32 ? lse : delta;
+  if constexpr (kRanged<T>) {
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) acc[t] *= 1.f / f;
+  }
   if (row >= n)
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) acc[t] = f32x16{};
@@ -438,6 +515,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
   for (int kk = 0; kk < D / 16; ++kk)
     k[kk] = load16<typename E::x8>(dk, static_cast<int>((lane & 31) * a.k_st[1] * 2) + (kk * 2 + (lane >> 5)) * 16);
 
+  float f = 1.f;
+  if constexpr (kRanged<T>) {
+    const int64_t all_rows = static_cast<int64_t>(G) * ((a.S + 31) / 32);
+    f = power(largest(do_norms(a) + (static_cast<int64_t>(b) * a.Hk + hk) * all_rows, all_rows, lane),
+              largest(v_norms(a) + (static_cast<int64_t>(b) * a.Hk + hk) * tiles, tiles, lane));
+    f = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, f)));  // a scalar register
+  }
   const int first = CAUSAL ? k0 / kQ : 0;                                 // first step of rows
   const int each = k0 < n ? (n + kQ - 1) / kQ - first : 0;                // steps a head
   const int all = each * G;                                               // the whole walk
@@ -517,7 +601,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
       for (int j = 0; j < 4; ++j) {
         const int r = m * 4 + j;
         s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l[j]));
-        dp[r] = s[r] * (dp[r] - d[j]);
+        dp[r] = s[r] * (kRanged<T> ? (dp[r] - d[j]) * f : dp[r] - d[j]);
       }
     }
     if (CAUSAL && s0 < kw + 31) {
@@ -545,6 +629,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
     }
   }
   copies_done();
+  if constexpr (kRanged<T>) {
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) dka[t] *= 1.f / f;
+  }
   if (a.splits > 1) {
     if (key < n) {  // the join reads no more
       const int64_t part = static_cast<int64_t>(a.B) * a.S * a.Hk * D;
@@ -623,6 +711,10 @@ template <class T, int D, bool CAUSAL> int forward(const KgsAttention& a, hipStr
 
 template <class T, int D, bool CAUSAL> int backward(const KgsAttention& a, hipStream_t s) {
   const int64_t tiles = (a.S + kRows - 1) / kRows, b = a.B;
+  if constexpr (kRanged<T>) {
+    attention_norms_kernel<T, D><<<static_cast<unsigned>(b * a.Hk * tiles), kThreads, 0, s>>>(a);
+    if (launched("attention norms")) return -1;
+  }
   attention_dq_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(b * a.H, tiles, a.lengths)), kThreads, 0, s>>>(a);
   if (launched("attention dq")) return -1;
   attention_dkv_kernel<T, D, CAUSAL><<<static_cast<unsigned>(head_items(b * a.Hk, tiles * a.splits, a.lengths)), kThreads, 0, s>>>(a);

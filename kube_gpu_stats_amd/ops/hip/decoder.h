@@ -8,7 +8,8 @@ extern "C" {
 
 // Tensors [B, S, heads, D]; strides in elements of (B, S, heads), D contiguous; pointers
 // 16-byte aligned, strides multiples of 8.  lse: float [B, H, S],
-// delta: float [B, H, ceil(S / 32), 2, 32] (workspace).  low: [B, S, H, D], what rounding
+// delta: float [B, H, ceil(S / 32), 2, 32], for float16 then [B, Hk, ceil(S / 128)] and
+// [B, H, ceil(S / 32)] (workspace).  low: [B, S, H, D], what rounding
 // took from out, a signed byte of 256ths of its last place.  The forward pass writes lse and low if they
 // are not null.
 struct KgsAttention {

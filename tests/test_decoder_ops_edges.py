@@ -7,10 +7,12 @@ import gc
 import math
 
 import pytest
+import test_decoder_ops
 import torch
 
 from kube_gpu_stats_amd.ops import decoder
-from test_decoder_ops import BF16, F16, F32, NORM_GRADS, close, half_step, norm_check, norm_inputs, norm_oracle, z
+from test_decoder_ops import (BF16, F16, F32, NORM_GRADS, attention_inputs, close, half_step, norm_check, norm_inputs,
+                              norm_oracle, z)
 
 gpu = pytest.mark.gpu
 
@@ -250,3 +252,71 @@ def test_train_models_agree_on_small_activations(monkeypatch):
 @gpu
 def test_train_models_agree_on_small_activations_on_gpu(dev):
     same_gradients(train_loads(0))
+
+
+# -------------------------------------------------------- attention in fp16: ranges of ds
+
+def fp16_oracle(monkeypatch, q, k, v, do, causal, scale):
+    """attention_oracle without what it allows for fp16's lack of range, and in its place: results round to
+    multiples of 2^-24 at the least; ds is rounded times a power of two that brings a bound of |do.v - delta|,
+    2.02 |do| |v| of the largest norms, over 2^14, so to multiples of 2^-38 of that bound at the least;
+    probabilities to multiples of 2^-24."""
+    with monkeypatch.context() as m:
+        m.setattr(test_decoder_ops, "F16", None)
+        ref, tol, _ = test_decoder_ops.attention_oracle(q, k, v, do, causal, scale, [q.shape[1]] * q.shape[0])
+    n, G = q.shape[1], q.shape[2] // k.shape[2]
+    size = [x.double().abs().max() for x in (q, k, v, do)]
+    most = 2.02 * q.shape[3] * size[3] * size[2]  # a norm is at most the largest element by the root of D
+    tol["out"] += 2.0 ** -25 * n * size[2]
+    tol["dv"] += 2.0 ** -25 * n * G * size[3]
+    tol["dq"] += 2.0 ** -39 * scale * n * most * size[1]
+    tol["dk"] += 2.0 ** -39 * scale * n * G * most * size[0]
+    for x in tol.values():
+        x += 2.0 ** -25
+    return ref, tol
+
+
+def fp16_check(monkeypatch, q, k, v, do, causal, names=("out", "dq", "dk", "dv")):
+    scale = q.shape[3] ** -0.5
+    out, saved = decoder.attention_fwd(q, k, v, causal=causal)
+    got = dict(zip(("out", "dq", "dk", "dv"), (out, *decoder.attention_bwd(do, q, k, v, out, saved, causal=causal))))
+    ref, tol = fp16_oracle(monkeypatch, q, k, v, do, causal, scale)
+    for n in names:
+        close(got[n], ref[n], tol[n], n)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("B,S,H,Hk,D", [(1, 200, 2, 2, 128), (2, 61, 2, 1, 64), (1, 33, 1, 1, 64), (1, 1100, 4, 1, 128)])
+@pytest.mark.parametrize("e,a", [(-20, 10), (-20, -10), (-14, 5), (-8, 0), (0, 0), (8, 0)])
+def test_fp16_gradients_of_small_and_large_dout(dev, monkeypatch, e, a, B, S, H, Hk, D, causal):
+    """dout of 2^e, keys of 2^a and queries of 2^-a: dq (or dk) lies well inside fp16's range, ds far below it."""
+    q, k, v, do = (x.float() for x in attention_inputs(B, S, H, Hk, D, F32, dev, seed=S))
+    fp16_check(monkeypatch, *(x.to(F16) for x in (q * 2.0 ** -a, k * 2.0 ** a, v, do * 2.0 ** e)), causal)
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_gradients_of_large_products(dev, monkeypatch, D):
+    """do.v of over 2^20, ds of over fp16's largest, gradients of a few hundreds; rows that grow, and that shrink."""
+    q, k, v, do = attention_inputs(1, 300, 2, 1, D, F32, dev, seed=D)
+    q, k, v, do = q * 2.0 ** -8, k * 2.0 ** -8, v * 2.0 ** 6, do * 2.0 ** 12
+    for causal in (True, False):
+        fp16_check(monkeypatch, *(x.to(F16) for x in (q, k, v, do)), causal, ("out", "dq", "dk"))
+        for way in (1, -1):  # rows and keys of very different sizes, in rising and falling order
+            grow = 2.0 ** (torch.linspace(-12, 0, 300, device=dev) * way + min(0, way) * 12).view(1, 300, 1, 1)
+            fp16_check(monkeypatch, *(x.to(F16) for x in (q, k, v * grow, do * grow)), causal, ("out", "dq", "dk"))
+
+
+@gpu
+def test_fp16_gradients_of_zero_rows(dev, monkeypatch):
+    """Rows whose dout is zero, at the start, between others and all of them."""
+    q, k, v, do = attention_inputs(1, 150, 2, 2, 64, F32, dev, seed=2)
+    do = do * 2.0 ** -16
+    do[:, :40] = 0
+    do[:, 70] = 0
+    for causal in (True, False):
+        fp16_check(monkeypatch, *(x.to(F16) for x in (q, k * 64, v, do)), causal)
+        h = [x.to(F16) for x in (q, k, v)]
+        out, saved = decoder.attention_fwd(*h, causal=causal)
+        assert not any(x.any() for x in decoder.attention_bwd(torch.zeros_like(out), *h, out, saved, causal=causal))
