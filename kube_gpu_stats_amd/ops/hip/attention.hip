@@ -155,6 +155,14 @@ __device__ __forceinline__ float power(float norm_do, float norm_v) {
   return ldexpf(1.f, 15 - __builtin_amdgcn_frexp_expf(2.02f * norm_do * norm_v));
 }
 
+// Probabilities of fp16 too are rounded times a power of two, a constant: forward the largest
+// of a row may have 2^8 times the subtracted maximum's (a lag that is explained there) and
+// is 2^14 then; backward a probability is at most 1, and 16 where scores of 2^26 leave their
+// difference from lse no better.  Below 2^-14 rounding is coarser than 11 bits: that is 2^-20
+// of a row's largest forward, 2^-26 backward.
+template <class T> constexpr float kUpForward = kRanged<T> ? 6.f : 0.f;
+template <class T> constexpr float kUpBackward = kRanged<T> ? 12.f : 0.f;
+
 // Of 128 rows of v the largest norm.
 template <class T, int D> __global__ __launch_bounds__(kThreads) void attention_norms_kernel(KgsAttention a) {
   constexpr int kLanes = D / 8, kAtOnce = kThreads / kLanes;
@@ -283,11 +291,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
 #pragma unroll
       for (int t = 0; t < D / 32; ++t) o[t] *= f;
     }
+    const float base = top - kUpForward<T>;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], c, -top));
+        s[t][r] = __builtin_amdgcn_exp2f(fmaf(s[t][r], c, -base));
         sum += s[t][r];
       }
 #pragma unroll
@@ -314,7 +323,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
     store_low<T, D>(o, inv, own, a.low + ((static_cast<int64_t>(b) * a.S + qw) * a.H + h) * D, static_cast<int64_t>(a.H) * D,
                     a.S - qw, lane);
   if (a.lse && lane < 32 && row < a.S)
-    a.lse[(static_cast<int64_t>(b) * a.H + h) * a.S + row] = row < n ? top + __builtin_amdgcn_logf(sum) : -INFINITY;
+    a.lse[(static_cast<int64_t>(b) * a.H + h) * a.S + row] = row < n ? top - kUpForward<T> + __builtin_amdgcn_logf(sum) : -INFINITY;
 }
 
 // dq of 128 rows a workgroup, and delta of those rows for the kernel that follows.
@@ -465,11 +474,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(KgsAttention 
   }
   copies_done();
   barrier();
-  // For dk, dv: the 32 rows' lse, then their delta, side by side.  Rows past the end get
-  // zeros: with zeros for q and do they are p = 1 times zero there.
+  // For dk, dv: the 32 rows' lse (less the power that probabilities are rounded with), then
+  // their delta, side by side.  Rows past the end get zeros: with zeros for q and do they are
+  // p = 1 times zero there.
   if (group < groups)
     a.delta[(static_cast<int64_t>(b * a.H + h) * groups + group) * 64 + lane] =
-        row >= n ? 0.f : lane < 32 ? lse : delta;
+        row >= n ? 0.f : lane < 32 ? lse - kUpBackward<T> : delta;
   if constexpr (kRanged<T>) {
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) acc[t] *= 1.f / f;
@@ -561,6 +571,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
 
   f32x16 dka[D / 32] = {}, dva[D / 32] = {};
   const float c = a.scale * kLog2e;
+  const float rest = f * 0x1p-12f;  // the probabilities have 2^12 of it
   if (lo < hi) fetch(0);
   loads_done();
   int slot = 0, ss = hi > lo ? lo % each : 0;
@@ -601,7 +612,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
       for (int j = 0; j < 4; ++j) {
         const int r = m * 4 + j;
         s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l[j]));
-        dp[r] = s[r] * (kRanged<T> ? (dp[r] - d[j]) * f : dp[r] - d[j]);
+        dp[r] = s[r] * (kRanged<T> ? (dp[r] - d[j]) * rest : dp[r] - d[j]);
       }
     }
     if (CAUSAL && s0 < kw + 31) {
@@ -631,7 +642,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
   copies_done();
   if constexpr (kRanged<T>) {
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t) dka[t] *= 1.f / f;
+    for (int t = 0; t < D / 32; ++t) dka[t] *= 1.f / f, dva[t] *= 0x1p-12f;
   }
   if (a.splits > 1) {
     if (key < n) {  // the join reads no more
