@@ -74,6 +74,7 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float f,
       for (int j = 0; j < 4; ++j) v[j] = static_cast<T>(acc[t][g * 4 + j] * f);
       *reinterpret_cast<x4*>(lds + Tl::at(lane & 31, t * 4 + g) + (lane >> 5) * 8) = v;
     }
+  wave_order();
   constexpr int kPer = 64 / (D / 8);  // rows a store
   const i32x4 to = buffer(p, rows > 0 ? ((rows - 1) * stride + D) * 2 : 0);
 #pragma unroll
@@ -82,6 +83,7 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float f,
     const i32x4 v = *reinterpret_cast<const i32x4*>(lds + Tl::at(row, chunk));
     store16(v, to, static_cast<int>(row * stride * 2) + chunk * 16);
   }
+  wave_order();
 }
 
 // What the rounding of acc f took, beside store_rows.
@@ -101,6 +103,7 @@ __device__ __forceinline__ void store_low(const f32x16 (&acc)[D / 32], float f, 
       const int row = lane & 31, e = t * 32 + g * 8 + (lane >> 5) * 4;
       *reinterpret_cast<uint32_t*>(lds + row * D + ((((e >> 4) ^ (row >> 1)) & (D / 16 - 1)) << 4) + (e & 15)) = lo | (hi << 16);
     }
+  wave_order();
 #pragma unroll
   for (int i = 0; i < 32 / kPer; ++i) {
     const int row = i * kPer + lane / (D / 16), chunk = lane % (D / 16);

@@ -135,6 +135,14 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Between a wave's writes to LDS and the reads of them by its other lanes, and before it writes
+// there again.  The hardware does one wave's LDS operations in order; this keeps the
+// compiler, which looks at one lane's addresses, from changing the order.  No instruction.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // A tile of rows of W elements (W = 64 or 128) in LDS, in 16-byte chunks, chunk c of a
 // row at c ^ swizzle(row).  256 bytes (all 64 banks) are one row of 128 or two of 64.
 // Row-wise reads take the same chunk of 32 rows: 16 rows in turn land on 16 places.

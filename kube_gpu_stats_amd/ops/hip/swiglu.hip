@@ -301,6 +301,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_kernel(Product p) {
         for (int j = 0; j < 4; ++j) r[j] = static_cast<T>(c[j]);
         *reinterpret_cast<typename E::x4*>(own + at) = r;
       }
+    wave_order();
     out(own, static_cast<char*>(p.c), static_cast<int64_t>(N) * 2, m, nw);
     if constexpr (PAIR) {
       if (p.saved) {
@@ -320,6 +321,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_kernel(Product p) {
           }
       }
     }
+    wave_order();
   }
 }
 
