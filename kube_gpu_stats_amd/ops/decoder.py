@@ -55,7 +55,7 @@ def lib() -> ctypes.CDLL:
 
 
 # The C structures of ops/hip/decoder.h, field by field.
-_ATTENTION = struct.Struct("@13P24q8if")
+_ATTENTION = struct.Struct("@13P24q9if")
 _SWIGLU = struct.Struct("@9P3q4i3i3i")
 _ADD_NORM = struct.Struct("@16P5q4iP2f")
 
@@ -249,7 +249,7 @@ def _attention_fwd(q, k, v, causal, scale, lengths, stream, keep):
         _call("kgs_attention_fwd",
               _ATTENTION.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, 0, 0, 0, _ptr(lse), 0, 0,
                               _ptr(low), _ptr(lengths), *qs, *ks, *vs, S * H * D, H * D, D, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
-                              0, 0, B, S, H, Hk, D, code, bool(causal), 1, scale), q.get_device())
+                              0, 0, B, S, H, Hk, D, code, bool(causal), 1, 0, scale), q.get_device())
     return out, (lse, low) if keep else None
 
 
@@ -308,7 +308,7 @@ def _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, stream,
                               *(t.data_ptr() for t in into), lse.data_ptr(), at, at + rows * 4 if parts else 0,
                               low.data_ptr(), _ptr(lengths), *qs, *ks, *vs, *os_, *gs, *into[0].stride()[:3],
                               *into[1].stride()[:3], *into[2].stride()[:3], B, S, H, Hk, D, code, bool(causal), splits,
-                              scale), q.get_device())
+                              0, scale), q.get_device())
     return tuple(into)
 
 

@@ -1,7 +1,9 @@
 // C interface of libkgs_decoder.so (loaded with ctypes by kube_gpu_stats_amd/ops/decoder.py,
-// whose Structures repeat these layouts field by field).  Every entry launches on `stream`,
+// whose struct formats repeat these layouts field by field; none has padding at its end,
+// which a packed block would lack and an entry copy).  Every entry launches on `stream`,
 // returns 0, or -1 with kgs_decoder_last_error() set.
 #pragma once
+#include <cstddef>
 #include <cstdint>
 
 extern "C" {
@@ -21,9 +23,10 @@ struct KgsAttention {
   uint8_t* low;
   const int32_t* lengths;        // [B] or null
   int64_t q_st[3], k_st[3], v_st[3], o_st[3], g_st[3], dq_st[3], dk_st[3], dv_st[3];
-  int32_t B, S, H, Hk, D, type, causal, splits;  // type: 0 bfloat16, 1 float16
+  int32_t B, S, H, Hk, D, type, causal, splits, unused;  // type: 0 bfloat16, 1 float16
   float scale;
 };
+static_assert(sizeof(KgsAttention) == offsetof(KgsAttention, scale) + 4, "padding at the end");
 
 // x [T, K] and w [2F, K] with row strides, h [T, F], saved [T, 6F] bytes (null: not kept), dh [T, F]
 // with a row stride, dgu [T, 2F], dx [T, K], dw [2F, K] (either null: not wanted).  Pointers
@@ -39,6 +42,7 @@ struct KgsSwiglu {
   int32_t T, K, F, type;
   int32_t tile[3], splits[3];
 };
+static_assert(sizeof(KgsSwiglu) == offsetof(KgsSwiglu, splits) + 12, "padding at the end");
 
 // Rows of `width` elements; row strides in elements.  rstd float [2, rows] (of the stream, of
 // the branch); dstream and dout may be null (zero).  post_weight and gate may be null.
@@ -59,6 +63,7 @@ struct KgsAddNorm {
   uint8_t* low;
   float scale, eps;
 };
+static_assert(sizeof(KgsAddNorm) == offsetof(KgsAddNorm, eps) + 4, "padding at the end");
 
 const char* kgs_decoder_last_error();
 int kgs_swiglu_fwd(const KgsSwiglu* a, void* stream);

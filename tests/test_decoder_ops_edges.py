@@ -343,3 +343,21 @@ def test_fp16_probabilities_far_below_one(dev, monkeypatch, gap, D):
     v[:, 0] = 0
     fp16_check(monkeypatch, *(x.to(F16) for x in (q, k, v, do * 1024)), True, ("out", "dv"))
     fp16_check(monkeypatch, *(x.to(F16) for x in (q, k, v, do * 1024)), False, ("out", "dv"))
+
+
+# ----------------------------------------------------------------- argument blocks (CPU)
+
+def test_argument_blocks_are_whole_structures(tmp_path):
+    """The library copies each structure whole, with what pads it: so much has to be there to be read."""
+    import os
+    import shutil
+    import subprocess
+
+    if not shutil.which("g++"):
+        pytest.skip("no host compiler")
+    here = os.path.join(os.path.dirname(os.path.abspath(decoder.__file__)), "hip")
+    (tmp_path / "s.cpp").write_text('#include <cstdio>\n#include "decoder.h"\nint main() { std::printf("%zu %zu %zu", '
+                                    "sizeof(KgsAttention), sizeof(KgsSwiglu), sizeof(KgsAddNorm)); }\n")
+    subprocess.run(["g++", "-I", here, str(tmp_path / "s.cpp"), "-o", str(tmp_path / "s")], check=True)
+    got = subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(x) for x in got] == [decoder._ATTENTION.size, decoder._SWIGLU.size, decoder._ADD_NORM.size]
