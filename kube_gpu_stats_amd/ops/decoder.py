@@ -134,6 +134,11 @@ def _shape(t, name: str, want) -> None:
 
 # --------------------------------------------------------------------------- attention
 
+# Elements from one position to the next (offsets inside a tile of 128 fit 32 bits), and workgroups of 256
+# threads (a launch has under 2^32).
+MAX_ROW, MAX_PIECES = 1 << 22, (1 << 24) - 8
+
+
 def _heads(t):
     """``t`` [B, S, heads, D] as the kernels read it, and its strides of (B, S, heads):
     D contiguous, positions apart, 16-byte rows.  Other layouts are copied."""
@@ -143,7 +148,7 @@ def _heads(t):
     b, s, h, d = t.stride()
     # A dimension of one may come with any stride; rows behind the last have to lie past it.
     st = (b if B > 1 else D, s if S > 1 else D, h if H > 1 else D)
-    if d == 1 and D <= st[1] <= 1 << 22 and not (t.data_ptr() % 16 or (st[0] | st[1] | st[2]) % 8):
+    if d == 1 and D <= st[1] <= MAX_ROW and not (t.data_ptr() % 16 or (st[0] | st[1] | st[2]) % 8):
         return t, st
     t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride()[:3]
@@ -177,6 +182,10 @@ def _attention_checks(q, k, v, scale, lengths, back=None):
         raise ValueError(f"{H} query heads cannot share {Hk} key heads")
     if S >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} positions, not {S}")
+    if H * D > MAX_ROW:
+        raise ValueError(f"at most {MAX_ROW} elements a position over all heads, not {H * D}")
+    if B * H * -(-S // 128) > MAX_PIECES:
+        raise ValueError(f"at most {MAX_PIECES} pieces of 128 positions over batch and heads, not {B * H * -(-S // 128)}")
     scale = D ** -0.5 if scale is None else float(scale)
     if not 2.0 ** -126 <= scale <= 2.0 ** 126:  # a 32-bit number, times log2 e too
         raise ValueError(f"scale must be positive, from 2^-126 to 2^126, not {scale}")
@@ -199,7 +208,8 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, lengt
     output (other layouts are copied first).  ``causal``: position i sees positions up to i.
     ``scale``: D^-½ if None.  ``lengths`` [B] int32 on the GPU: sequence b is its first
     lengths[b] positions (clamped to 0..S); nothing behind them is read, the result and the
-    gradients are zero there.  Returns [B, S, H, D], contiguous.
+    gradients are zero there.  Returns [B, S, H, D], contiguous.  At most 2^22 elements a
+    position (H·D), and 2^24 - 8 pieces of 128 positions over batch and heads.
 
     A position that is masked by ``causal`` alone is multiplied by a zero probability, as in
     a plain matrix product: its v must be finite.
@@ -223,6 +233,8 @@ def _split_qkv(qkv, heads: int):
     if qkv.dim() != 4 or heads <= 0 or qkv.shape[2] <= heads or (qkv.shape[2] - heads) % 2:
         raise ValueError(f"qkv must be [batch, positions, {heads} + 2 key heads, head dimension], "
                          f"not {tuple(qkv.shape)}")
+    if qkv.shape[2] * qkv.shape[3] > MAX_ROW:
+        raise ValueError(f"at most {MAX_ROW} elements a position, not {qkv.shape[2] * qkv.shape[3]}")
     kv = (qkv.shape[2] - heads) // 2
     return qkv[:, :, :heads], qkv[:, :, heads:heads + kv], qkv[:, :, heads + kv:]
 
@@ -343,6 +355,9 @@ def _swiglu_checks(x, w, dh=None, saved=None):
     T = x.numel() // K
     if T >= 1 << 30:
         raise ValueError(f"at most {(1 << 30) - 1} rows, not {T}")
+    rows, inner, width = -(-T // 256), -(-2 * F // 256), -(-K // 256)
+    if max(rows * inner, rows * width, inner * width) > MAX_TILES:
+        raise ValueError(f"a product of {T} rows, width {K} and inner {F} has more than {MAX_TILES} tiles of 256 x 256")
     _on_gpu(x, "x")
     return T, K, F, code
 
@@ -350,6 +365,7 @@ def _swiglu_checks(x, w, dh=None, saved=None):
 # The tiles of swiglu.hip's product, rows by columns: 128 x 128, 256 x 256, and for the
 # forward pass of up to 32 rows 32 x 256.
 PRODUCT_TILES = (0, 1, 2)
+MAX_TILES = (1 << 23) - 8  # of 256 x 256, the largest: 512 threads each, a launch has under 2^32
 
 
 @functools.lru_cache(maxsize=4096)
@@ -366,13 +382,14 @@ def _product_plan(M: int, N: int, K: int, forward: bool = False) -> tuple[int, i
     from memory: 38 us with 32 x 256 in 4 parts, 54 us with 128 x 128 in 3.)"""
     floor = 2 * (M * K + N * K + M * N) / 5.2e6
     best = None
-    for tile, rows, columns, at_once, around in ((0, 128, 128, 512, 3.5), (1, 256, 256, 256, 8.0), (2, 32, 256, 512, 3.5)):
+    for tile, rows, columns, at_once, around, most in ((0, 128, 128, 512, 3.5, 2 * MAX_TILES), (1, 256, 256, 256, 8.0, MAX_TILES),
+                                                       (2, 32, 256, 512, 3.5, 2 * MAX_TILES)):
         if tile == 2 and not (forward and M <= 32):
             continue
         blocks = -(-M // rows) * -(-N // columns)
         for splits in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16):
             steps = -(-K // 64 // splits)
-            if splits > 1 and steps < 4:
+            if splits > 1 and steps < 4 or blocks * splits > most:
                 break
             step = (1.10 if blocks * splits > 256 else 0.74, 1.83, 1.5)[tile]
             # a step's columns come from memory once, however many row tiles share them
@@ -390,7 +407,8 @@ def swiglu(x, w):
 
     x [..., width], w [2 inner, width] (the gate's rows first) of bfloat16 or float16, width
     and inner multiples of 8; any row strides with contiguous, 16-byte aligned rows are read
-    in place.  Returns [..., inner].  With a gradient wanted the two projections are kept
+    in place.  Returns [..., inner].  At most 2^20 of width and of inner, 2^30 - 1 rows and
+    2^23 - 8 tiles of 256 x 256 in a product.  With a gradient wanted the two projections are kept
     for the backward pass, 24 bits of each value.
     """
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):

@@ -710,9 +710,9 @@ int check(const KgsAttention* a, bool backward) {
       if (st[i][j] < 0 || st[i][j] % 8 || (j == 1 && (st[i][j] < a->D || st[i][j] > (1 << 22)))) return fail(w, "unsupported strides");
   if (a->H > (1 << 18)) return fail(w, "too many heads");  // offsets inside a tile of low
   // a launch has under 2^32 threads; the products of counts that head_item forms, 16 times
-  // its pieces at most, stay under 2^31
-  const int64_t tiles = (a->S + kRows - 1) / kRows;
-  if ((tiles + 16) * (static_cast<int64_t>(a->B) * a->H + 16) * (backward ? a->splits : 1) > (1 << 24) - 64)
+  // a head's pieces at most, stay under 2^31 with that
+  const int64_t tiles = (a->S + kRows - 1) / kRows, most = (1 << 24) - 8;
+  if (a->B * static_cast<int64_t>(a->H) * tiles > most || (backward && a->B * static_cast<int64_t>(a->Hk) * tiles * a->splits > most))
     return fail(w, "too many workgroups");
   return 0;
 }

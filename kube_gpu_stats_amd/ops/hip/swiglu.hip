@@ -385,7 +385,7 @@ int product_tiled(const Product& p, hipStream_t s) {
   }
   const int N = PAIR ? p.N / 2 : p.N, bn = PAIR ? BN / 2 : BN;
   const int64_t total = static_cast<int64_t>((p.M + BM - 1) / BM) * ((N + bn - 1) / bn) * p.splits;
-  if (total > (1 << 22)) return fail("swiglu", "too many workgroups");  // under 2^32 threads
+  if (total > (1ll << 32) / (WM * WN * 64) - 8) return fail("swiglu", "too many workgroups");  // under 2^32 threads
   kernel<<<static_cast<unsigned>((total + 7) / 8 * 8), WM * WN * 64, kLds, s>>>(p);
   if (launched("swiglu product")) return -1;
   if (p.splits > 1) {

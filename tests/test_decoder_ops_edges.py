@@ -361,3 +361,61 @@ def test_argument_blocks_are_whole_structures(tmp_path):
     subprocess.run(["g++", "-I", here, str(tmp_path / "s.cpp"), "-o", str(tmp_path / "s")], check=True)
     got = subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(x) for x in got] == [decoder._ATTENTION.size, decoder._SWIGLU.size, decoder._ADD_NORM.size]
+
+
+# ----------------------------------------------------------------- limits of a launch
+
+def big(*shape, t=BF16):
+    return torch.zeros(1, dtype=t).expand(*shape)
+
+
+TOO_LARGE = [
+    ("attention pieces", lambda: decoder.attention(*[big(1 << 20, 1, 16, 64)] * 3)),
+    ("attention pieces of long rows", lambda: decoder.attention(*[big(1, (1 << 30) - 1, 3, 128)] * 3)),
+    ("attention pieces back", lambda: decoder.attention_bwd(*[big(1 << 20, 1, 16, 64)] * 5,
+                                                            (big(1 << 20, 16, 1, t=F32), big(1 << 20, 1, 16, 64, t=torch.uint8)))),
+    ("attention heads", lambda: decoder.attention(*[big(1, 4, (1 << 16) + 1, 64)] * 3)),
+    ("attention heads on few", lambda: decoder.attention(big(1, 4, 1 << 16, 128), *[big(1, 4, 1, 128)] * 2)),
+    ("qkv heads", lambda: decoder.attention_qkv(big(1, 4, 3 << 15, 64), 1 << 15)),
+    ("swiglu rows and inner", lambda: decoder.swiglu(big((1 << 30) - 1, 8), big(1 << 10, 8))),
+    ("swiglu weights", lambda: decoder.swiglu(big(4, 1 << 20), big(1 << 21, 1 << 20))),
+]
+
+
+@pytest.mark.parametrize("call", [pytest.param(c, id=n) for n, c in TOO_LARGE])
+def test_what_no_launch_holds_is_refused(call, monkeypatch):
+    """With a ValueError, before anything is launched."""
+    monkeypatch.setattr(decoder, "_kept", lambda *a: None)  # (expanded tensors are not contiguous)
+    with pytest.raises(ValueError) as raised:
+        call()
+    assert "must be on a GPU" not in str(raised.value)
+
+
+def test_every_product_that_is_not_refused_has_a_plan():
+    # (the most: 2^23 - 8 tiles of 256 x 256)
+    for M, N, K in ((1 << 20, 1 << 18, 8), (1 << 30, 128, 8), (1 << 19, 1 << 19, 1 << 20), (1 << 21, 8, 1 << 30), (1 << 29, 512, 64)):
+        for forward in (False, True):
+            tile, splits = decoder._product_plan(M, N, K, forward)
+            rows, columns, threads = ((128, 128, 256), (256, 256, 512))[tile]
+            assert (-(-M // rows) * -(-N // columns) * splits + 7) * threads < 1 << 32
+
+
+@gpu
+@pytest.mark.parametrize("B,S,H", [(65536, 1, 16), (40000, 3, 32), (1 << 19, 1, 16)])
+def test_attention_of_many_short_sequences(dev, B, S, H):
+    """Over a million heads of one piece each."""
+    g = torch.Generator(device=dev).manual_seed(B)
+    q, k, v, do = (torch.randn(B, S, H, 64, generator=g, device=dev).to(BF16) for _ in range(4))
+    out, saved = decoder.attention_fwd(q, k, v)
+    grads = decoder.attention_bwd(do, q, k, v, out, saved)
+    assert torch.equal(out[:, 0], v[:, 0])  # the first position sees itself
+    for b in (0, 1, B // 2 + 1, B - 1):
+        one = [x[b:b + 1].contiguous() for x in (q, k, v, do)]
+        o, keep = decoder.attention_fwd(*one[:3])
+        for x, y in zip((out, *grads), (o, *decoder.attention_bwd(one[3], *one[:3], o, keep))):
+            assert torch.equal(x[b:b + 1], y)
+    lengths = torch.arange(B, device=dev, dtype=torch.int32) % (S + 1)
+    padded = decoder.attention(q, k, v, lengths=lengths)
+    for s in range(S):
+        live = (lengths > s)[:, None, None]
+        assert torch.equal(padded[:, s], torch.where(live, out[:, s], torch.zeros_like(out[:, s])))
