@@ -17,8 +17,9 @@ All of them launch on the current stream of their tensors' device (or on ``strea
 allocate their results and workspaces from torch's allocator on that stream, never
 synchronise and keep nothing between calls, so they can be captured into a graph.
 Gradients are sums in a fixed order: equal calls give equal bits.  The autograd forms
-differentiate once.  To capture a whole autograd step, let no eager graph of the same
-leaves be alive (torch's own rule); the ``*_fwd`` / ``*_bwd`` pairs have no such rule.
+differentiate once, backwards; an argument with a forward-mode tangent is refused.  To
+capture a whole autograd step, let no eager graph of the same leaves be alive (torch's own
+rule); the ``*_fwd`` / ``*_bwd`` pairs have no such rule.
 
 There is deliberately no eager fallback: on a GPU the HIP library must load, or these
 functions raise.  Wrong arguments raise ``ValueError`` or ``TypeError`` before anything
@@ -32,6 +33,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ..native import build as _build
@@ -82,6 +84,14 @@ def _there(t, stream, call, *tensors):
                 x.record_stream(stream)
     with torch.cuda.device(t.device), torch.cuda.stream(stream):
         return call()
+
+
+def _no_tangents(*tensors) -> None:
+    """The kernels would drop a forward-mode tangent without a word."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise TypeError("the operators have no forward-mode derivative: an argument carries a tangent")
 
 
 def _ptr(t) -> int:
@@ -214,6 +224,7 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, lengt
     A position that is masked by ``causal`` alone is multiplied by a zero probability, as in
     a plain matrix product: its v must be finite.
     """
+    _no_tangents(q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attention.apply(q, k, v, causal, scale, lengths)
     return _attention_fwd(q, k, v, causal, scale, lengths, None, False)[0]
@@ -224,6 +235,7 @@ def attention_qkv(qkv, heads: int, *, causal: bool = True, scale: float | None =
     first, then the key heads, then the value heads; differentiable, with one gradient of
     the same layout (no gradients of views to be put together)."""
     q, k, v = _split_qkv(qkv, heads)
+    _no_tangents(qkv)
     if torch.is_grad_enabled() and qkv.requires_grad:
         return _AttentionQkv.apply(qkv, heads, causal, scale, lengths)
     return _attention_fwd(q, k, v, causal, scale, lengths, None, False)[0]
@@ -243,6 +255,7 @@ def attention_fwd(q, k, v, *, causal: bool = True, scale: float | None = None, l
     """``attention`` without autograd: (out, saved), saved for ``attention_bwd``: (lse, low), lse
     [B, H, S] float32 the base-2 logarithm of each row's sum (-inf behind a sequence's end),
     low [B, S, H, D] uint8 what rounding took from out, a signed number of 256ths of its last place."""
+    _no_tangents(q, k, v)
     return _attention_fwd(q, k, v, causal, scale, lengths, stream, True)
 
 
@@ -294,6 +307,7 @@ def attention_bwd(dout, q, k, v, out, saved, *, causal: bool = True, scale: floa
                   stream=None):
     """(dq, dk, dv) of ``attention`` from the gradient of its result, with ``out`` and ``saved``
     of ``attention_fwd`` and the same keywords; the probabilities are computed again."""
+    _no_tangents(dout, q, k, v, out)
     return _attention_bwd(dout, q, k, v, out, *saved, causal, scale, lengths, stream, None)
 
 
@@ -411,6 +425,7 @@ def swiglu(x, w):
     2^23 - 8 tiles of 256 x 256 in a product.  With a gradient wanted the two projections are kept
     for the backward pass, 24 bits of each value.
     """
+    _no_tangents(x, w)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         return _Swiglu.apply(x, w)
     return _swiglu_fwd(x, w, None, False)[0]
@@ -419,6 +434,7 @@ def swiglu(x, w):
 def swiglu_fwd(x, w, *, stream=None):
     """``swiglu`` without autograd: (h, saved), saved [..., 6 inner] uint8 for ``swiglu_bwd``: of
     each row the upper 16 bits of the two projections, then the 8 bits below."""
+    _no_tangents(x, w)
     return _swiglu_fwd(x, w, stream, True)
 
 
@@ -441,6 +457,7 @@ def _swiglu_fwd(x, w, stream, keep):
 
 def swiglu_bwd(dh, x, w, saved, *, stream=None):
     """(dx, dw) of ``swiglu`` from the gradient of its result and what ``swiglu_fwd`` saved."""
+    _no_tangents(dh, x, w)
     return _swiglu_bwd(dh, x, w, saved, True, True, stream)
 
 
@@ -526,6 +543,7 @@ def add_norm(residual, branch, weight, *, post_weight=None, gate=None, scale: fl
     [..., C], weight, post_weight, gate [C], all of one type (bfloat16, float16, float32),
     C up to 16384, of any row stride.  Differentiable in all five tensors.
     """
+    _no_tangents(residual, branch, weight, post_weight, gate)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                        for t in (residual, branch, weight, post_weight, gate)):
         return _AddNorm.apply(residual, branch, weight, post_weight, gate, scale, eps)
@@ -537,6 +555,7 @@ def add_norm_fwd(residual, branch, weight, *, post_weight=None, gate=None, scale
     """``add_norm`` without autograd: (stream, out, saved), saved for ``add_norm_bwd``: [2, rows]
     float32, the factors of the two norms, in the stream's memory and with it 8 more bits of
     each of a 16-bit stream's elements."""
+    _no_tangents(residual, branch, weight, post_weight, gate)
     return _add_norm_fwd(residual, branch, weight, post_weight, gate, scale, eps, stream, True, True)
 
 
@@ -617,6 +636,7 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
     gradients of absent weights are None."""
     if dstream is None and dout is None:
         raise ValueError("one of dstream and dout must be given")
+    _no_tangents(dstream, dout, residual, branch, weight, post_weight, gate)
     T, C, code, scale = _add_norm_checks(residual, branch, weight, post_weight, gate, scale, eps, (dstream, dout, saved))
     if not _here(residual, stream):
         return _there(residual, stream,

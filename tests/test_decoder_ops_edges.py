@@ -419,3 +419,29 @@ def test_attention_of_many_short_sequences(dev, B, S, H):
     for s in range(S):
         live = (lengths > s)[:, None, None]
         assert torch.equal(padded[:, s], torch.where(live, out[:, s], torch.zeros_like(out[:, s])))
+
+
+# ----------------------------------------------------------------- forward-mode derivatives (CPU)
+
+@pytest.mark.parametrize("call", [
+    pytest.param(lambda dual: decoder.attention(z(1, 4, 2, 64), dual(1, 4, 2, 64), z(1, 4, 2, 64)), id="attention"),
+    pytest.param(lambda dual: decoder.attention_qkv(dual(1, 4, 4, 64), 2), id="attention_qkv"),
+    pytest.param(lambda dual: decoder.attention_fwd(dual(1, 4, 2, 64), z(1, 4, 2, 64), z(1, 4, 2, 64)), id="attention_fwd"),
+    pytest.param(lambda dual: decoder.attention_bwd(dual(1, 4, 2, 64), *[z(1, 4, 2, 64)] * 4, test_decoder_ops.kept()), id="attention_bwd"),
+    pytest.param(lambda dual: decoder.swiglu(z(4, 64), dual(16, 64)), id="swiglu"),
+    pytest.param(lambda dual: decoder.swiglu_bwd(dual(4, 8), z(4, 64), z(16, 64), z(4, 48, t=torch.uint8)), id="swiglu_bwd"),
+    pytest.param(lambda dual: decoder.add_norm_bwd(None, dual(4, 64), z(4, 64), z(4, 64), z(64), z(2, 4, t=F32)), id="add_norm_bwd"),
+    pytest.param(lambda dual: decoder.swiglu_fwd(dual(4, 64), z(16, 64)), id="swiglu_fwd"),
+    pytest.param(lambda dual: decoder.add_norm(z(4, 64), z(4, 64), z(64), gate=dual(64)), id="add_norm"),
+    pytest.param(lambda dual: decoder.add_norm_fwd(z(4, 64), dual(4, 64), z(64)), id="add_norm_fwd"),
+])
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_tangents_are_refused(call, grad):
+    """They were dropped without a word."""
+    import torch.autograd.forward_ad as fw
+
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        with pytest.raises(TypeError, match="forward-mode"):
+            call(lambda *shape: fw.make_dual(z(*shape), z(*shape)))
+        with pytest.raises(ValueError, match="must be on a GPU"):  # no tangent among the arguments: as ever
+            decoder.swiglu(z(4, 64), z(16, 64))
