@@ -222,7 +222,8 @@ def attention(q, k, v, *, causal: bool = True, scale: float | None = None, lengt
     position (H·D), and 2^24 - 8 pieces of 128 positions over batch and heads.
 
     A position that is masked by ``causal`` alone is multiplied by a zero probability, as in
-    a plain matrix product: its v must be finite.
+    a plain matrix product: its v must be finite.  A key whose score is -inf has a probability
+    of zero (a row that sees no other: zeros).  Gradients need finite q, k, v and dout.
     """
     _no_tangents(q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

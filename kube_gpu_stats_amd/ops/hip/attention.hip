@@ -240,7 +240,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_fwd_kernel(KgsAttention
   };
 
   f32x16 o[D / 32] = {};
-  float top = -INFINITY, sum = 0.f;
+  float top = -0x1.fffffep127f, sum = 0.f;  // finite: a power of a difference of infinities is none
   const float c = a.scale * kLog2e;
   if (steps > 0) fetch(0);
   loads_done();

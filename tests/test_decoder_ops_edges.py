@@ -11,7 +11,7 @@ import test_decoder_ops
 import torch
 
 from kube_gpu_stats_amd.ops import decoder
-from test_decoder_ops import (BF16, F16, F32, NORM_GRADS, attention_inputs, close, half_step, norm_check, norm_inputs,
+from test_decoder_ops import (BF16, F16, F32, NORM_GRADS, attention_inputs, close, half_step, mm, norm_check, norm_inputs,
                               norm_oracle, z)
 
 gpu = pytest.mark.gpu
@@ -445,3 +445,28 @@ def test_forward_mode_tangents_are_refused(call, grad):
             call(lambda *shape: fw.make_dual(z(*shape), z(*shape)))
         with pytest.raises(ValueError, match="must be on a GPU"):  # no tangent among the arguments: as ever
             decoder.swiglu(z(4, 64), z(16, 64))
+
+
+# ----------------------------------------------------------------- scores of minus infinity
+
+@gpu
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("first", [1, 32, 64, 130, 200])
+@pytest.mark.parametrize("causal", [True, False])
+def test_keys_of_minus_infinity(dev, causal, first, t):
+    """Keys whose scores are -inf take no part, also where a row sees no others at first, or none at all."""
+    S, H, D = 200, 2, 64
+    q, k, v, _ = attention_inputs(1, S, H, 1, D, t, dev, seed=first)
+    q = q.abs()
+    k[:, :first] = -math.inf
+    out = decoder.attention(q, k, v, causal=causal)
+    assert torch.equal(decoder.attention_fwd(q, k, v, causal=causal)[0], out)
+    u = half_step(t)
+    for h in range(H):
+        s = mm(q[0, :, h].double(), k[0, first:, 0].double().t()) * D ** -0.5
+        if causal:
+            s = s.masked_fill(torch.arange(first, S, device=dev)[None] > torch.arange(S, device=dev)[:, None], -math.inf)
+        p = torch.softmax(s, 1).nan_to_num(0.0)
+        V = v[0, first:, 0].double()
+        # roundings of p and of the result; 32-bit scores, sums and powers: 2^-14 of p covers 200 terms of 2^-24
+        close(out[0, :, h], mm(p, V), u * mm(p, V).abs() + (1.01 * u + 2.0 ** -14) * mm(p, V.abs()), "out")
