@@ -15,7 +15,8 @@ Each operator comes three times:
 
 All of them launch on the current stream of their tensors' device (or on ``stream=``),
 allocate their results and workspaces from torch's allocator on that stream, never
-synchronise and keep nothing between calls, so they can be captured into a graph.
+synchronise and keep nothing between calls, so they can be captured into a graph.  With
+``stream=`` the results may be used on the current stream once it has waited for that one.
 Gradients are sums in a fixed order: equal calls give equal bits.  The autograd forms
 differentiate once, backwards; an argument with a forward-mode tangent is refused.  To
 capture a whole autograd step, let no eager graph of the same leaves be alive (torch's own
@@ -75,15 +76,24 @@ def _here(t, stream) -> bool:
 
 def _there(t, stream, call, *tensors):
     """``call()`` with ``t``'s device and ``stream`` current: allocations and launches belong there.
-    On a given stream the call's ``tensors`` are not handed out again before it is through."""
+    On a given stream the memory of the call's ``tensors`` is not handed out again before it is
+    through, that of its results not before what the current stream does with them is."""
+    now = None
     if stream is not None:
         if stream.device != t.device:
             raise ValueError(f"the stream is on {stream.device}, the tensors are on {t.device}")
         for x in (t, *tensors):
             if x is not None:
                 x.record_stream(stream)
+        now = torch.cuda.current_stream(t.device)
     with torch.cuda.device(t.device), torch.cuda.stream(stream):
-        return call()
+        results = call()
+    if now is not None and now != stream:
+        for x in results:
+            for y in x if isinstance(x, tuple) else (x,):
+                if y is not None:
+                    y.record_stream(now)
+    return results
 
 
 def _no_tangents(*tensors) -> None:

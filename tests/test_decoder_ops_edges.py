@@ -470,3 +470,40 @@ def test_keys_of_minus_infinity(dev, causal, first, t):
         V = v[0, first:, 0].double()
         # roundings of p and of the result; 32-bit scores, sums and powers: 2^-14 of p covers 200 terms of 2^-24
         close(out[0, :, h], mm(p, V), u * mm(p, V).abs() + (1.01 * u + 2.0 ** -14) * mm(p, V.abs()), "out")
+
+
+# ----------------------------------------------------------------- results of a given stream
+
+@gpu
+def test_results_of_a_given_stream_outlive_their_use_on_the_current_one(dev):
+    """Memory of a result that is dropped while the current stream still reads it is not handed out again."""
+    q = torch.randn(1, 512, 8, 64, device=dev).to(BF16)
+    x, w = torch.randn(512, 520, device=dev).to(BF16), torch.randn(520, device=dev).to(BF16)
+    wg = torch.randn(1024, 520, device=dev).to(BF16)
+    out, saved = decoder.attention_fwd(q, q, q)
+    _, kept = decoder.swiglu_fwd(x, wg)
+    s, _, rstd = decoder.add_norm_fwd(x, x, w)
+    h = torch.randn(512, 512, device=dev).to(BF16)
+    side = torch.cuda.Stream()
+    for call in (lambda: decoder.attention_fwd(q, q, q, stream=side), lambda: decoder.attention_bwd(out, q, q, q, out, saved, stream=side),
+                 lambda: decoder.swiglu_fwd(x, wg, stream=side), lambda: decoder.swiglu_bwd(h, x, wg, kept, stream=side),
+                 lambda: decoder.add_norm_fwd(x, x, w, stream=side), lambda: decoder.add_norm_bwd(x, x, s, x, w, rstd, gate=w, stream=side)):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        side.wait_stream(torch.cuda.current_stream())
+        flat = []
+        for r in call():
+            flat.extend(r if isinstance(r, tuple) else [r])
+        flat = [r for r in flat if r is not None]
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda._sleep(100_000_000)  # the current stream is about to read them
+        used = [r.clone() for r in flat]
+        was = {r.untyped_storage().data_ptr(): r.untyped_storage().nbytes() for r in flat}
+        side.synchronize()
+        del flat, r
+        with torch.cuda.stream(side):
+            again = {torch.empty(n, dtype=torch.uint8, device=dev).data_ptr(): n for n in list(was.values()) * 2}
+        assert not torch.cuda.current_stream().query(), "the use is over: nothing was shown"
+        assert not was.keys() & again.keys()
+        torch.cuda.synchronize()
+        del used
