@@ -269,7 +269,8 @@ class TrainLoad(GpuLoad):
 
     ``--train-ops hip``: the same model with the block's attention, gate and norms as this
     package's kernels (kube_gpu_stats_amd/ops/decoder.py), whose operations a step are
-    known and reported by calibrate()."""
+    known and reported by calibrate(): those of the formulas, and those that the matrix units
+    are given."""
 
     burst_timed = None  # no MFMA burst kernel of known length: phase U is skipped
 
@@ -338,9 +339,12 @@ class TrainLoad(GpuLoad):
         model = (HipModel if self.hip else Model)(self.vocab).to(device=dev, dtype=torch.bfloat16)
         self.params = sum(p.numel() for p in model.parameters())
         # What the operators of ops/decoder.py have to compute in a step: causal attention (two products
-        # forward, five backward over half the square), the gate's projections and their gradients.
-        pairs = self.batch * self.seq * (self.seq + 1) / 2
-        self.op_flops = L * (14.0 * pairs * d + 12.0 * self.batch * self.seq * d * ff)
+        # forward, five backward over half the square), the gate's projections and their gradients.  And what
+        # their kernels give the matrix units for it, which is what a counter of those sees.
+        tokens = self.batch * self.seq
+        self.op_flops = L * (14.0 * tokens * (self.seq + 1) / 2 * d + 12.0 * tokens * d * ff)
+        self.matrix_flops = L * (sum(decoder.attention_matrix_flops(self.batch, self.seq, h, d // h))
+                                 + sum(decoder.swiglu_matrix_flops(tokens, d, ff))) if self.hip else 0
         if ctx is not None and ctx.is_dist:
             from torch.nn.parallel import DistributedDataParallel
 
@@ -389,7 +393,8 @@ class TrainLoad(GpuLoad):
         s = sorted(ts)[1]
         toks = self.batch * self.seq
         # 6·N·T for the dense weights + causal attention (fwd 2·S·d per token per layer, x3 with bwd)
-        own = {"train_ops": "hip", "train_op_tflop_per_step": self.op_flops * 1e-12} if self.hip else {}
+        own = {"train_ops": "hip", "train_op_tflop_per_step": self.op_flops * 1e-12,
+               "train_op_matrix_tflop_per_step": self.matrix_flops * 1e-12} if self.hip else {}
         return {**own, "train_step_ms": s * 1e3, "train_tokens_per_s": toks / s, "train_params": self.params,
                 "train_tflops": 6.0 * self.params * toks / s / 1e12}
 

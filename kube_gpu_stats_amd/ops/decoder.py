@@ -349,6 +349,19 @@ def _attention_bwd(dout, q, k, v, out, lse, low, causal, scale, lengths, stream,
     return tuple(into)
 
 
+def attention_matrix_flops(B: int, S: int, H: int, D: int) -> tuple[int, int]:
+    """(forward, backward) operations that the kernels give the matrix units for causal attention
+    without lengths, of any key heads: nine products where the formula has seven, whole steps
+    along the diagonal and at the end.  A counter of the matrix units is held against these."""
+    forward = backward = 0  # products of 32 rows x 32 keys
+    for row in range(0, -(-S // 128) * 128, 32):
+        last = min(row + 32, S)  # keys that any row of the wave sees
+        forward += 2 * 2 * -(-last // 64)
+        backward += 3 * -(-last // 32) + (4 if last <= 64 else 0) + 4 * max(0, -(-S // 32) - row // 32)
+    each = 2 * 32 * 32 * D * B * H
+    return forward * each, backward * each
+
+
 # ------------------------------------------------------------------------------ swiglu
 
 def _matrix(t):
@@ -492,6 +505,19 @@ def _swiglu_bwd(dh, x, w, saved, want_dx, want_dw, stream):
               _SWIGLU.pack(x.data_ptr(), w.data_ptr(), 0, saved.data_ptr(), dh.data_ptr(), dgu.data_ptr(), _ptr(dx),
                            _ptr(dw), _ptr(part), x_ld, w_ld, dh_ld, T, K, F, code, 0, tx, tw, 1, sx, sw), x.get_device())
     return dx, dw
+
+
+def swiglu_matrix_flops(T: int, K: int, F: int) -> tuple[int, int]:
+    """(forward, backward) operations that the kernels give the matrix units: whole tiles, the
+    sum in steps of 64."""
+    def product(M, N, K, forward):
+        rows, columns = ((128, 128), (256, 256), (32, 256))[_product_plan(M, N, K, forward)[0]]
+        halves = 2 if forward else 1  # a forward tile has as many columns of either projection
+        blocks = -(-M // rows) * -(-(N // halves) // (columns // halves))
+        return 2 * blocks * rows * columns * -(-K // 64) * 64
+    if T == 0:
+        return 0, 0
+    return product(T, 2 * F, K, True), product(T, K, 2 * F, False) + product(2 * F, K, T, False)
 
 
 # ---------------------------------------------------------------------------- add_norm

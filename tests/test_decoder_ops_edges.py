@@ -507,3 +507,55 @@ def test_results_of_a_given_stream_outlive_their_use_on_the_current_one(dev):
         assert not was.keys() & again.keys()
         torch.cuda.synchronize()
         del used
+
+
+# ----------------------------------------------------------------- what the matrix units are given (CPU)
+
+def attention_products(S, D):
+    """Products of 32 x 32 x D of one head's causal forward and backward, by walking as the kernels do."""
+    forward = back = 0
+    for q0 in range(0, S, 128):
+        for qw in range(q0, q0 + 128, 32):
+            last = min(qw + 32, S)
+            for s0 in range(0, min(S, q0 + 128), 64):
+                if s0 >= last:
+                    continue
+                forward += 4  # scores and values of two halves of 32 keys
+                back += 4 if last <= 64 else 0  # the exact delta of a row's only step
+                back += 3 * (1 + (s0 + 32 < last))
+        for kw in range(q0, q0 + 128, 32):
+            for s0 in range(q0, S, 32):
+                back += 4 * (s0 + 32 > kw)
+    return forward * 2 * 32 * 32 * D, back * 2 * 32 * 32 * D
+
+
+@pytest.mark.parametrize("S", [1, 31, 64, 65, 100, 128, 200, 640, 1021])
+def test_attention_matrix_flops(S):
+    for D in (64, 128):
+        forward, back = attention_products(S, D)
+        assert decoder.attention_matrix_flops(3, S, 4, D) == (12 * forward, 12 * back)
+    assert decoder.attention_matrix_flops(1, 0, 4, 64) == (0, 0)
+
+
+def test_swiglu_matrix_flops():
+    for T, K, F in ((8192, 4096, 11008), (5, 4096, 11008), (1777, 1000, 2680), (1, 8, 8)):
+        up = lambda x, n: -(-x // n) * n  # noqa: E731
+        want = []
+        for M, N, sum_, forward in ((T, 2 * F, K, True), (T, K, 2 * F, False), (2 * F, K, T, False)):
+            rows, columns = ((128, 128), (256, 256), (32, 256))[decoder._product_plan(M, N, sum_, forward)[0]]
+            n = 2 * up(F, columns // 2) if forward else up(N, columns)
+            want.append(2 * up(M, rows) * n * up(sum_, 64))
+        assert decoder.swiglu_matrix_flops(T, K, F) == (want[0], want[1] + want[2])
+    assert decoder.swiglu_matrix_flops(0, 64, 64) == (0, 0)
+
+
+def test_train_load_reports_both_counts():
+    import bench
+
+    a = bench.parse_args(["--load", "train", "--train-ops", "hip", "--train-dim", "256", "--train-layers", "3",
+                          "--train-batch", "2", "--train-seq", "96", "--train-vocab", "512"])
+    ld = bench.TrainLoad(a, -1, None)
+    tokens, ff = 2 * 96, 768
+    assert ld.op_flops == 3 * (14.0 * 2 * 96 * 97 / 2 * 256 + 12.0 * tokens * 256 * ff)
+    assert ld.matrix_flops == 3 * (sum(decoder.attention_matrix_flops(2, 96, 2, 128)) + sum(decoder.swiglu_matrix_flops(tokens, 256, ff)))
+    assert ld.matrix_flops > ld.op_flops
