@@ -96,16 +96,24 @@ template <bool WAVES> __device__ __forceinline__ float row_sum(float x, int lane
 // it an infinity is read back as a NaN: so is an element that rounding made infinite, whose
 // difference would make it a finite one.
 template <class T> __device__ __forceinline__ void store_low(const float (&x)[kV], uint8_t* p, int left) {
-  Loose<uint8_t> r;
+  u32x2 bytes;
 #pragma unroll
-  for (int i = 0; i < kV; ++i)
-    r.v[i] = __builtin_isinf(static_cast<float>(static_cast<T>(x[i]))) ? 0 : static_cast<uint8_t>(low_of<T>(x[i]) >> 8);
+  for (int g = 0; g < 2; ++g) {
+    uint32_t q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float e = x[g * 4 + j];
+      q[j] = __builtin_isinf(static_cast<float>(static_cast<T>(e))) ? 0 : low_of<T>(e);
+    }
+    bytes[g] = __builtin_amdgcn_perm(q[1], q[0], 0x0C0C0501) | (__builtin_amdgcn_perm(q[3], q[2], 0x0C0C0501) << 16);
+    __builtin_amdgcn_sched_barrier(0);  // four at a time: over 64 registers half as many waves run
+  }
   if (left >= kV) {
-    *reinterpret_cast<Loose<uint8_t>*>(p) = r;
+    __builtin_memcpy(p, &bytes, kV);
   } else {
 #pragma unroll
     for (int i = 0; i < kV; ++i)
-      if (i < left) p[i] = r.v[i];
+      if (i < left) p[i] = static_cast<uint8_t>(bytes[i >> 2] >> (8 * (i & 3)));
   }
 }
 
@@ -143,9 +151,10 @@ template <bool WAVES> struct Place {
   }
 };
 
-// FULL: with post_weight, gate or a scale.  NV: chunks of 8 a thread.
-template <class T, bool WAVES, int NV, bool FULL, Fit FIT>
-__global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_fwd_kernel(KgsAddNorm a) {
+// FULL: with post_weight, gate or a scale.  NV: chunks of 8 a thread.  LOW: writes the low
+// bytes too.
+template <class T, bool WAVES, int NV, bool FULL, bool LOW, Fit FIT>
+__global__ __launch_bounds__(WAVES ? 256 : 1024, LOW && NV == 1 ? 8 : 1) void add_norm_fwd_kernel(KgsAddNorm a) {
   __shared__ float slots[2 * 16];
   int turn = 0;
   const Place<WAVES> at(a.width);
@@ -204,9 +213,7 @@ __global__ __launch_bounds__(WAVES ? 256 : 1024) void add_norm_fwd_kernel(KgsAdd
       }
       if (skip[i] < kV) {
         store(s[i], place<T>(a.stream, row * a.stream_ld, column[i]), size);
-        if constexpr (sizeof(T) == 2) {
-          if (a.low) store_low<T>(s[i], a.low + static_cast<int64_t>(row) * C + column[i] / sizeof(T), size);
-        }
+        if constexpr (LOW) store_low<T>(s[i], a.low + static_cast<int64_t>(row) * C + column[i] / sizeof(T), size);
       }
     }
     const float rs = 1.f / sqrtf(row_sum<WAVES>(sq, at.lanes, slots, turn) / C + a.eps);
@@ -459,16 +466,23 @@ template <bool WAVES, int NV> void shape(const KgsAddNorm& a, int& threads, int&
   rows = WAVES ? 256 / lanes_of_row(a.width) : 1;
 }
 
-template <class T, bool WAVES, int NV> int forward(const KgsAddNorm& a, hipStream_t s) {
+template <class T, bool WAVES, int NV, bool LOW> int forward_and(const KgsAddNorm& a, hipStream_t s) {
   int threads, rows;
   shape<WAVES, NV>(a, threads, rows);
   const int want = (a.rows + rows - 1) / rows, grid = want < 8192 ? want : 8192;
   const auto go = [&](auto kernel) { kernel<<<grid, threads, 0, s>>>(a); };
   const bool full = is_full(a);
-  if (a.width % kV == 0) full ? go(add_norm_fwd_kernel<T, WAVES, NV, true, kWhole>) : go(add_norm_fwd_kernel<T, WAVES, NV, false, kWhole>);
-  else if (a.width > kV) full ? go(add_norm_fwd_kernel<T, WAVES, NV, true, kRagged>) : go(add_norm_fwd_kernel<T, WAVES, NV, false, kRagged>);
-  else if constexpr (WAVES) full ? go(add_norm_fwd_kernel<T, WAVES, NV, true, kTiny>) : go(add_norm_fwd_kernel<T, WAVES, NV, false, kTiny>);
+  if (a.width % kV == 0) full ? go(add_norm_fwd_kernel<T, WAVES, NV, true, LOW, kWhole>) : go(add_norm_fwd_kernel<T, WAVES, NV, false, LOW, kWhole>);
+  else if (a.width > kV) full ? go(add_norm_fwd_kernel<T, WAVES, NV, true, LOW, kRagged>) : go(add_norm_fwd_kernel<T, WAVES, NV, false, LOW, kRagged>);
+  else if constexpr (WAVES) full ? go(add_norm_fwd_kernel<T, WAVES, NV, true, LOW, kTiny>) : go(add_norm_fwd_kernel<T, WAVES, NV, false, LOW, kTiny>);
   return launched("add_norm forward");
+}
+
+template <class T, bool WAVES, int NV> int forward(const KgsAddNorm& a, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (a.low) return forward_and<T, WAVES, NV, true>(a, s);
+  }
+  return forward_and<T, WAVES, NV, false>(a, s);
 }
 
 template <class T, bool WAVES, int NV, bool STORED, int THREADS> int backward_from(const KgsAddNorm& a, hipStream_t s) {
