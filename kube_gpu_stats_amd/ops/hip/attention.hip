@@ -147,10 +147,16 @@ __device__ __forceinline__ float wave_max(float x) {
   for (int m = 1; m < 64; m <<= 1) x = fmaxf(x, __shfl_xor(x, m, 64));
   return x;
 }
-// The largest of n floats, in every lane.
+// The largest of n floats and 0, in every lane; eight loads a lane under way.
 __device__ __forceinline__ float largest(const float* p, int64_t n, int lane) {
   float x = 0.f;
-  for (int64_t i = lane; i < n; i += 64) x = fmaxf(x, p[i]);
+  for (int64_t i = lane; i < n + lane; i += 64 * 8) {
+    float y[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) y[u] = p[min(i + u * 64, n - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) x = fmaxf(x, y[u]);
+  }
   return wave_max(x);
 }
 // The power of two that brings the bound to between 2^14 and 2^15 (1 % for rounding).
@@ -530,8 +536,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dkv_kernel(KgsAttention
 
   float f = 1.f;
   if constexpr (kRanged<T>) {
-    const int64_t all_rows = static_cast<int64_t>(G) * ((a.S + 31) / 32);
-    f = power(largest(do_norms(a) + (static_cast<int64_t>(b) * a.Hk + hk) * all_rows, all_rows, lane),
+    // (a quarter a wave: where 64 heads share one they are 32768 for 16384 positions)
+    __shared__ float most[NW];
+    const int64_t all_rows = static_cast<int64_t>(G) * ((a.S + 31) / 32), quarter = (all_rows + NW - 1) / NW;
+    const float m = largest(do_norms(a) + (static_cast<int64_t>(b) * a.Hk + hk) * all_rows + wave * quarter,
+                            min(quarter, all_rows - wave * quarter), lane);
+    if (lane == 0) most[wave] = m;
+    barrier();
+    f = power(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])),
               largest(v_norms(a) + (static_cast<int64_t>(b) * a.Hk + hk) * tiles, tiles, lane));
     f = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, f)));  // a scalar register
   }

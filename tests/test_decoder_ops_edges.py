@@ -559,3 +559,33 @@ def test_train_load_reports_both_counts():
     assert ld.op_flops == 3 * (14.0 * 2 * 96 * 97 / 2 * 256 + 12.0 * tokens * 256 * ff)
     assert ld.matrix_flops == 3 * (sum(decoder.attention_matrix_flops(2, 96, 2, 128)) + sum(decoder.swiglu_matrix_flops(tokens, 256, ff)))
     assert ld.matrix_flops > ld.op_flops
+
+
+@gpu
+def test_fp16_attention_captured(dev):
+    """Forward and backward in a graph, with all launches that fp16 takes, a split walk among them."""
+    def inputs(seed):
+        return attention_inputs(1, 900, 8, 1, 64, F16, dev, seed=seed)
+
+    def step(q, k, v, do):
+        out, saved = decoder.attention_fwd(q, k, v)
+        return (out, *decoder.attention_bwd(do, q, k, v, out, saved))
+
+    a = inputs(1)
+    step(*a)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = step(*a)
+        graphs.append((g, got))
+    for seed in (2, 3, 4):
+        for x, y in zip(a, inputs(seed)):
+            x.copy_(y * 2.0 ** -seed)
+        want = step(*a)
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, got in graphs:
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), seed
