@@ -446,8 +446,10 @@ def swiglu(x, w):
     x [..., width], w [2 inner, width] (the gate's rows first) of bfloat16 or float16, width
     and inner multiples of 8; any row strides with contiguous, 16-byte aligned rows are read
     in place.  Returns [..., inner].  At most 2^20 of width and of inner, 2^30 - 1 rows and
-    2^23 - 8 tiles of 256 x 256 in a product.  With a gradient wanted the two projections are kept
-    for the backward pass, 24 bits of each value.
+    2^23 - 8 tiles of 256 x 256 in a product.  With a gradient wanted the two projections are
+    kept for the backward pass, 24 bits of each value.  Its two products take the projections'
+    gradients (silu(g) dh and its like) in the tensors' type: in float16 they have to lie in
+    its range, like any gradient between two layers.
     """
     _no_tangents(x, w)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
@@ -667,9 +669,9 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
 
     In the residual's place the stream that ``add_norm_fwd`` returned with ``saved`` does as
     well: then the residual need not be kept, and without post_weight, gate and scale the
-    branch is not read either.  It has to be that tensor, or one of its memory and order
-    (``saved`` lies in the same memory, by which it is known); a copy of it is taken for a
-    residual.  Without post_weight, gate and scale dbranch is dresidual, the same tensor;
+    branch is not read either.  It has to be that tensor, or one of its memory and order, with
+    that ``saved``: they lie in one memory, by which it is known, and where either is a copy
+    the stream is taken for a residual.  Without post_weight, gate and scale dbranch is dresidual, the same tensor;
     gradients of absent weights are None."""
     if dstream is None and dout is None:
         raise ValueError("one of dstream and dout must be given")

@@ -15,15 +15,18 @@
 //
 // Scores, statistics, sums and accumulators are 32 bits.  Rounded to the tensors' type:
 // p and ds, as operands of a matrix instruction (half a step each, independent from
-// term to term), and the outputs.  The rounding of out would reach dq and dk through
+// term to term; out, dq, dk and dv are 1.1 to 1.4 times as far from a 64-bit result as with
+// p and ds in 32 bits), and the outputs.  The rounding of out would reach dq and dk through
 // delta (a third more error than theirs); so the forward pass that a backward follows
 // also keeps 8 bits of what it rounded off.
 //
-// Bound by the matrix units, at the clock the power limit leaves (busy 58 to 68 % of the
-// time), and for D = 64 by the softmax's arithmetic, which issues for longer than the
-// products.  1 x 16384, 8 heads of 128 on 2, bf16, causal: forward 538 us (1020 TFLOP/s),
-// dq 770 us (1070), dk and dv 990 us (1110).  4 x 2048, 32 heads: 155 us (890) and 500 us
-// (960).  8 x 1536, 12 heads of 64, fp16, no mask: 74 us (780).
+// Bound by the matrix units at the clock the power limit leaves where rows are long: 1 x
+// 16384, 8 heads of 128 on 2, bf16, causal: forward 538 us (1020 TFLOP/s, matrix units busy
+// 61 % of the time), dq 740 to 770 us (1070, 68 %), dk and dv 930 to 980 us (1110, 67 %).
+// Start, end and diagonal of a walk take more of 4 x 2048, 32 heads: 155 us (890, 45 %),
+// and dq with dk and dv 510 us (940, 44 and 57 %).  For D = 64 by the softmax's arithmetic,
+// which issues for longer than the products: 8 x 1536, 12 heads, fp16, no mask: 76 us (765;
+// vector instructions 66 %, matrix units 40 %).
 #include "decoder.h"
 #include "decoder_common.h"
 
