@@ -247,8 +247,8 @@ template <class T> __device__ __forceinline__ void finish(const KgsAddNorm& a, i
 // that fits the registers of 16 waves a CU.  Two chunks (rows over 8192 wide) do without,
 // and read the weights again for every row.  STORED: from the stream and its low bytes, one
 // byte an element less to read than residual and branch, with FULL one more (8192 x 4096:
-// 57 us, 63 us from the residual; 16384 x 8192 with all weights 310 us, 288 us; the forward,
-// which writes them, 7 and 24 us more).
+// 57 us, 63 us from the residual; 16384 x 8192 with all weights 310 us, 287 us; the forward,
+// which writes them, 5 and 28 us more).
 template <class T, bool WAVES, int NV, bool FULL, bool STORED, Fit FIT, int THREADS>
 __global__ __launch_bounds__(THREADS) void add_norm_bwd_kernel(KgsAddNorm a) {
   __shared__ float slots[2 * 16];
