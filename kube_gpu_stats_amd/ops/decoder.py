@@ -671,8 +671,10 @@ def add_norm_bwd(dstream, dout, residual, branch, weight, saved, *, post_weight=
     well: then the residual need not be kept, and without post_weight, gate and scale the
     branch is not read either.  It has to be that tensor, or one of its memory and order, with
     that ``saved``: they lie in one memory, by which it is known, and where either is a copy
-    the stream is taken for a residual.  Without post_weight, gate and scale dbranch is dresidual, the same tensor;
-    gradients of absent weights are None."""
+    the stream is taken for a residual.
+
+    Without post_weight, gate and scale dbranch is dresidual, the same tensor; gradients of
+    absent weights are None."""
     if dstream is None and dout is None:
         raise ValueError("one of dstream and dout must be given")
     _no_tangents(dstream, dout, residual, branch, weight, post_weight, gate)
